@@ -224,6 +224,63 @@ int rdb_dense_gemm_fp8_tuned(const uint8_t *A, const uint8_t *B, const float *sc
  * D [M,N] OVERWRITTEN (async_gemm<float>, same citations). */
 int rdb_dense_gemm_fp8_f32(const uint8_t *A, const uint8_t *B, float *D, int M, int N, int K, void *stream);
 
+/* ------------------------------------------------- microscaled 4-bit floating point
+ * Elements are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives; codes 0..7, + 8 for the sign), rounded to the
+ * nearest, ties to the even code, saturating at 6.  No reference counterpart (its lowest precision is fp8).
+ *   RDB_FP4_MXFP4  blocks of 32 along K share 2^e (one byte, e + 127): e = floor(log2(largest magnitude)) - 2, clamped
+ *                  to [-127, 127]; element = e2m1(x / 2^e).  This is the conversion of the OCP Microscaling Formats
+ *                  specification, version 1.0.
+ *   RDB_FP4_NVFP4  blocks of 16 along K share an e4m3 scale s, the tensor one fp32 scale t: t given, or the largest
+ *                  finite magnitude / 2688 (not below 2^-126; 1 if all are zero); s = e4m3_sat(block's largest
+ *                  magnitude / (6 t)); element = e2m1(x / (t s)), zero where s is.  6 t, t s and both quotients are
+ *                  rounded to fp32.  t must be a positive number.
+ * A block that holds an infinity or a NaN gets the scale type's NaN, and what is computed from it is NaN.
+ * A held tensor [rows, K], for any rows, K >= 1:
+ *   codes   [rows, rdb_fp4_row_bytes(K)] bytes (ceil(K / 32) * 16), two codes to a byte, the even index in the low half,
+ *           zero codes behind K;
+ *   scales  rdb_fp4_scale_bytes(format, rows, K) bytes in tiles of 128 rows x 4 blocks (512 bytes): row r, block b of a
+ *           tile at (r % 32) * 16 + (r / 32) * 4 + b; tiles run along K first, K filled up to a multiple of 256 with
+ *           zero bytes (the products read them); bytes of rows past the last are neither written nor used;
+ *   tensor_scale  one fp32 on the device (RDB_FP4_NVFP4 only, else NULL).
+ * codes and scales must be 16-byte aligned. */
+typedef enum rdb_fp4_format { RDB_FP4_MXFP4 = 0, RDB_FP4_NVFP4 = 1 } rdb_fp4_format;
+typedef enum rdb_type { RDB_TYPE_BF16 = 0, RDB_TYPE_FP16 = 1, RDB_TYPE_FP32 = 2 } rdb_type;
+#define RDB_FP4_WORKSPACE_FLOATS 1024
+size_t rdb_fp4_row_bytes(int K);
+size_t rdb_fp4_scale_bytes(int format, int rows, int K);     /* 0 for an unsupported argument */
+
+/* Quantises x [rows, K] (row pitch ldx elements, x_type one of rdb_type), with blocks along the rows into codes / scales
+ * and - or, where `codes` is NULL - with blocks along the columns into codes_t / scales_t, the held form of the
+ * TRANSPOSED tensor [K, rows] (what the gradients' products read).  Both directions share the tensor scale, which is
+ * written to tensor_scale[0], or read from it where scale_given is non-zero.  workspace: RDB_FP4_WORKSPACE_FLOATS floats
+ * of scratch for an RDB_FP4_NVFP4 call that computes its scale (else may be NULL); nothing in it outlives the call. */
+int rdb_quantize_fp4(const void *x, int x_type, long long ldx, int rows, int K, int format, float *tensor_scale,
+                     int scale_given, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
+                     float *workspace, void *stream);
+
+/* out [rows, K] (contiguous, out_type) = element * scale * tensor scale, the last product in fp32, then rounded once. */
+int rdb_dequantize_fp4(const uint8_t *codes, const uint8_t *scales, const float *tensor_scale, int format, int rows,
+                       int K, void *out, int out_type, void *stream);
+
+/* D[M,N] = out_type( (A . B^T) * tensor_scale_a * tensor_scale_b ), any M, N, K: A [M,K] and B [N,K] held tensors of one
+ * format, fp32 accumulation of exact products, D row-major, OVERWRITTEN.  The tensor scales are NULL for MXFP4.
+ * rdb_skinny_gemm_fp4: the same for M <= 32, tuned for streaming B; flags as for rdb_skinny_gemm_fp8_tuned
+ * (RDB_SKINNY_OVERLAP_PRIOR_KERNEL: B's codes and scales are requested before the preceding kernel of the stream has
+ * finished, which must not write them).  No workspace: calls on different streams may overlap. */
+int rdb_dense_gemm_fp4(const uint8_t *A, const uint8_t *scales_a, const float *tensor_scale_a, const uint8_t *B,
+                       const uint8_t *scales_b, const float *tensor_scale_b, void *D, int out_type, int M, int N, int K,
+                       int format, void *stream);
+int rdb_skinny_gemm_fp4(const uint8_t *A, const uint8_t *scales_a, const float *tensor_scale_a, const uint8_t *B,
+                        const uint8_t *scales_b, const float *tensor_scale_b, void *D, int out_type, int M, int N, int K,
+                        int format, unsigned flags, void *stream);
+
+/* rdb_skinny_gemm_fp4 with the kernel's own knobs, for measurements: columns_per_tile (64, 128, 192 or 256), split_k
+ * (1..8), stages; 0 = automatic. */
+int rdb_skinny_gemm_fp4_tuned(const uint8_t *A, const uint8_t *scales_a, const float *tensor_scale_a, const uint8_t *B,
+                              const uint8_t *scales_b, const float *tensor_scale_b, void *D, int out_type, int M, int N,
+                              int K, int format, int columns_per_tile, int split_k, int stages, unsigned flags,
+                              void *stream);
+
 /* -------------------------------------------------------- 2:4 sparse GEMM
  * D[M,N] = bf16( (A . W^T) * scale_a[0] * scale_b[0] ), M <= 256, K % 256 == 0,
  * where W [N,K] has at most two non-zero bytes in every aligned group of four

@@ -51,6 +51,13 @@ _SIGNATURES = {
     "rdb_sparse_file_pack_and_write": (i, [C.c_char_p, vp, C.c_float, i, i]),
     "rdb_sparse_file_info": (i, [C.c_char_p, vp, vp, vp]),
     "rdb_sparse_file_read": (i, [C.c_char_p, vp, C.c_size_t, vp, C.c_size_t]),
+    "rdb_fp4_row_bytes": (C.c_size_t, [i]),
+    "rdb_fp4_scale_bytes": (C.c_size_t, [i, i, i]),
+    "rdb_quantize_fp4": (i, [vp, i, C.c_longlong, i, i, i, vp, i, vp, vp, vp, vp, vp, vp]),
+    "rdb_dequantize_fp4": (i, [vp, vp, vp, i, i, i, vp, i, vp]),
+    "rdb_dense_gemm_fp4": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, vp]),
+    "rdb_skinny_gemm_fp4": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, C.c_uint, vp]),
+    "rdb_skinny_gemm_fp4_tuned": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, C.c_uint, vp]),
     "rdb_tiled_sum_reduce": (i, [vp, vp, vp, i, i, i, vp]),
     "rdb_globs": (i, [vp, vp]),
     "rdb_globs_n": (i, [vp, i, i, i, vp]),

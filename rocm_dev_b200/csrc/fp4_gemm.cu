@@ -1,0 +1,395 @@
+// Products of microscaled 4-bit tensors for sm_100a:  D[M,N] = (A . B^T) * ta * tb, operands held as fp4.cuh describes.
+//
+// tcgen05.mma kind::mxf4 / kind::mxf4nvf4 multiplies 64 elements of K per step and applies the block scales itself, from
+// TMEM; everything up to the fp32 accumulator is exact but the accumulation.  A pipeline stage is 256 elements of K: one
+// 128-byte swizzle row of codes per operand row, and the scale tiles of that stretch, which lie contiguous in memory and
+// go to shared memory with untiled copies and on to TMEM with tcgen05.cp.  Each ring slot owns TMEM columns for its
+// scales, so they are free again exactly when the slot is.
+//
+// split_kernel: one output tile of 128 x R per cluster, the cluster's S CTAs each taking a slice of K - for products that
+// are bound by streaming B (few rows of A) or that have too few tiles to fill the machine.  Roles per CTA as in the fp8
+// skinny kernel: warp 0 loads, warp 1 issues the MMAs, then all warps move the accumulator to shared memory, and each
+// rank sums its share of the columns over all ranks through distributed shared memory, in rank order: deterministic, no
+// workspace, no atomics.
+#include <cstdlib>
+#include <mutex>
+
+#include "fp4_mma.cuh"
+#include "host_util.h"
+
+RDB_DEFINE_WAIT_BUDGET_SETTER()
+
+namespace rdb {
+namespace fp4 {
+
+constexpr int SMEM_LIMIT = 232448;         // 227 KiB opt-in maximum per CTA
+constexpr int MAX_STAGES = 8;
+constexpr int SPLIT_THREADS = 192;
+constexpr int A_OPERAND_SPAN = 128 * 128;  // bytes the MMA reads for its 128-row A operand, whatever was loaded
+
+struct SplitParams {
+    void* D;
+    const uint8_t *sa, *sb;
+    const float *ta, *tb;       // tensor scales, nullptr: 1
+    int* status;
+    int M, N, num_kb;
+    int R, mbox;                // columns of the tile (a multiple of 64), rows of A that are loaded
+    int b_tiles;                // 128-row scale tiles that R columns touch
+    int sb_row_tiles;           // 128-row scale tiles of B in all
+    int nstages, tmem_cols;
+    int out_type, vec;
+    int early_b;                // B may be requested before the preceding kernel has finished
+};
+
+template <int FMT>
+__host__ __device__ constexpr int split_stage_bytes(int mbox, int R, int b_tiles) {
+    return (mbox + R) * 128 + Format<FMT>::TILES * TILE_BYTES * (1 + b_tiles);
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(SPLIT_THREADS, 1)
+split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const SplitParams p) {
+    constexpr int TILES = Format<FMT>::TILES, SCALES = TILES * TILE_BYTES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t bars[2 * MAX_STAGES + 1];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_s;
+    __shared__ float alpha_s;
+    volatile int* abort_flag = &abort_s;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = gridDim.x, rank = blockIdx.x, R = p.R, nstages = p.nstages;
+    const int n0 = blockIdx.y * R, m0 = blockIdx.z * 128;
+    const int rows = p.M - m0 < 128 ? p.M - m0 : 128;
+    const int kb_begin = static_cast<int>(static_cast<long long>(p.num_kb) * rank / S);
+    const int nkb = static_cast<int>(static_cast<long long>(p.num_kb) * (rank + 1) / S) - kb_begin;
+    const int A_BYTES = p.mbox * 128, B_BYTES = R * 128;
+    const int STAGE = split_stage_bytes<FMT>(p.mbox, R, p.b_tiles);
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + MAX_STAGES), done = smem_u32(bars + 2 * MAX_STAGES);
+    const uint32_t stage0 = smem_u32(smem);
+
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmB);
+        for (int s = 0; s < nstages; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(done, 1);
+        abort_s = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_slot), p.tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_slot;
+    pdl_launch_dependents();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint64_t pol_b = gridDim.z > 1 ? l2_policy_evict_last() : l2_policy_evict_first(), pol_a = l2_policy_evict_last();
+            const size_t sa_row = static_cast<size_t>(blockIdx.z) * p.num_kb * SCALES;
+            auto load_b = [&](int i, uint32_t dst, uint32_t bar) {
+                mbar_arrive_expect_tx(bar, STAGE);
+                tma_load_2d(dst + A_BYTES, &tmB, (kb_begin + i) * 128, n0, bar, pol_b);
+                for (int j = 0; j < p.b_tiles; j++) {
+                    int rt = n0 / 128 + j;
+                    if (rt >= p.sb_row_tiles) rt = p.sb_row_tiles - 1;       // columns past N: any scales do
+                    bulk_load_scales(dst + A_BYTES + B_BYTES + SCALES * (1 + j),
+                                     p.sb + (static_cast<size_t>(rt) * p.num_kb + kb_begin + i) * SCALES, SCALES, bar);
+                }
+            };
+            auto load_a = [&](int i, uint32_t dst, uint32_t bar) {
+                tma_load_2d(dst, &tmA, (kb_begin + i) * 128, m0, bar, pol_a);
+                bulk_load_scales(dst + A_BYTES + B_BYTES, p.sa + sa_row + static_cast<size_t>(kb_begin + i) * SCALES, SCALES, bar);
+            };
+            const int pre = nkb < nstages ? nkb : nstages;
+            if (!p.early_b) pdl_wait_prior();
+            for (int i = 0; i < pre; i++) load_b(i, stage0 + i * STAGE, full0 + 8 * i);
+            if (p.early_b) pdl_wait_prior();
+            for (int i = 0; i < pre; i++) load_a(i, stage0 + i * STAGE, full0 + 8 * i);
+            for (int i = pre; i < nkb; i++) {
+                const int s = i % nstages;
+                if (!mbar_wait(empty0 + 8 * s, ((i / nstages) & 1) ^ 1)) { *abort_flag = 1; report_timeout(p.status); break; }
+                load_b(i, stage0 + s * STAGE, full0 + 8 * s);
+                load_a(i, stage0 + s * STAGE, full0 + 8 * s);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const int slot_cols = TILES * 4 * (1 + p.b_tiles);
+            const int shift = (n0 & 127) / 32;               // a tile that starts inside a 128-row scale tile
+            for (int i = 0; i < nkb; i++) {
+                const int s = i % nstages;
+                if (!mbar_wait(full0 + 8 * s, (i / nstages) & 1)) { *abort_flag = 1; report_timeout(p.status); break; }
+                tc_fence_after_sync();
+                const uint32_t a = stage0 + s * STAGE, b = a + A_BYTES, sc = b + B_BYTES;
+                const uint32_t tsa = tmem_base + R + s * slot_cols, tsb = tsa + 4 * TILES;
+#pragma unroll
+                for (int t = 0; t < TILES; t++) {
+                    tmem_cp_scales<false>(tsa + 4 * t, sc + t * TILE_BYTES);
+                    for (int j = 0; j < p.b_tiles; j++)
+                        tmem_cp_scales<false>(tsb + 4 * (t * p.b_tiles + j), sc + SCALES * (1 + j) + t * TILE_BYTES);
+                }
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) {
+                    const int t = ks * TILES / 4, id = TILES == 4 ? 0 : 2 * (ks & 1);
+                    tc_mma_fp4<FMT, false>(tmem_base, smem_desc_k128(a + ks * 32), smem_desc_k128(b + ks * 32), idesc_fp4<FMT>(128, R, id),
+                                           tsa + 4 * t, tsb + 4 * t * p.b_tiles + shift, (i | ks) != 0);
+                }
+                tc_commit(empty0 + 8 * s);
+            }
+            tc_commit(done);                                 // also after an abort
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        if (lane == 0) {
+            pdl_wait_prior();
+            alpha_s = p.ta ? __ldg(p.ta) * __ldg(p.tb) : 1.0f;
+        }
+        __syncwarp();
+    }
+
+    // ---- the accumulator goes to shared memory, stg[row][R], over the drained ring.  A warp reads the TMEM lane quadrant
+    // warp % 4 (32 rows); warps 4 and 5 share quadrants 0 and 1 with warps 0 and 1.
+    float* stg = reinterpret_cast<float*>(smem);
+    const int pitch = R + 4;
+    const int quad = warp & 3;
+    if (quad * 32 < rows) {
+        bool ok = mbar_wait(done, 0);
+        if (!ok) { *abort_flag = 1; report_timeout(p.status); }
+        tc_fence_after_sync();
+        if (ok && *abort_flag == 0) {
+            float* row = stg + (quad * 32 + lane) * pitch;
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+            const int step = quad < 2 ? 64 : 32;
+#pragma unroll 1
+            for (int c0 = warp >= 4 ? 32 : 0; c0 < R; c0 += step) {
+                float v[32];
+                tmem_ld32(taddr + c0, v);
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(row + c0 + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            }
+        }
+        tc_fence_before_sync();
+    }
+    __syncthreads();
+    if (S > 1) {
+        cluster_arrive_release();
+        cluster_wait_acquire();                              // every rank's partial sums are in place
+    }
+    pdl_wait_prior();                                        // D may belong to the preceding kernel
+    const float alpha = alpha_s;
+    if (*abort_flag == 0) {
+        // columns in granules of four; rank r sums and stores [G r / S, G (r + 1) / S)
+        const int G = R / 4, g0 = G * rank / S, ng = G * (rank + 1) / S - g0;
+        for (int item = threadIdx.x; item < rows * ng; item += SPLIT_THREADS) {
+            const int m = item / ng, c = (g0 + item - m * ng) * 4;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            if (n0 + c < p.N) {
+                const float* mine = stg + m * pitch + c;
+                if (S == 1) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] = mine[j];
+                } else {
+                    const uint32_t at = smem_u32(mine);
+                    for (int src = 0; src < S; src++) {
+                        float x[4];
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(mapa_smem(at, src)) : "memory");
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[j] += x[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] *= alpha;
+                store4(p.D, p.out_type, p.N, m0 + m, n0 + c, v, p.vec);
+            }
+        }
+    } else {
+        for (int i = 0; i < 64; i++) __nanosleep(2000);      // copies in flight land before the memory is given back
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_base, p.tmem_cols);
+    if (S > 1) {                                             // no rank leaves while another still reads its memory
+        cluster_arrive_release();
+        cluster_wait_acquire();
+    }
+}
+
+// ------------------------------------------------------------------ host
+struct Product {
+    const uint8_t *A, *sa, *B, *sb;
+    const float *ta, *tb;
+    void* D;
+    int out_type, M, N, K;
+};
+
+struct SplitPlan {
+    int R, S, stages, mbox, b_tiles, tmem_cols, smem;
+};
+
+static int ring_limit(int format, int mbox, int R, int b_tiles) {
+    const int tiles = format == RDB_FP4_NVFP4 ? 4 : 2;
+    const int stage = format == RDB_FP4_NVFP4 ? split_stage_bytes<RDB_FP4_NVFP4>(mbox, R, b_tiles) : split_stage_bytes<RDB_FP4_MXFP4>(mbox, R, b_tiles);
+    int st = (512 - R) / (tiles * 4 * (1 + b_tiles));
+    while (st > 1 && 1024 + st * stage + A_OPERAND_SPAN > SMEM_LIMIT - 1024) st--;
+    return st < MAX_STAGES ? st : MAX_STAGES;
+}
+
+// Tile width and K split of the least estimated time; 0 hints mean free choice.
+static SplitPlan split_plan(int format, int M, int N, int K, int sm_count, int r_hint, int s_hint, int stages_hint) {
+    // clusters of 1..8 CTAs that are resident at once on 148 SMs (measured)
+    static const int resident[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+    const int num_kb = (K + STAGE_K - 1) / STAGE_K, m_tiles = (M + 127) / 128;
+    const int tiles = format == RDB_FP4_NVFP4 ? 4 : 2;
+    SplitPlan best = {};
+    best.mbox = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+    const int rows = M < 128 ? M : 128;
+    double best_cost = 1e30;
+    for (int R = 64; R <= 256; R += 64) {
+        if (r_hint > 0 && R != r_hint) continue;
+        const int b_tiles = (R + 127) / 128;
+        const double stage = (best.mbox + R) * 128.0 + tiles * TILE_BYTES * (1 + b_tiles);
+        for (int S = 1; S <= 8; S++) {
+            if ((s_hint > 0 && S != (s_hint < num_kb ? s_hint : num_kb)) || (S > 1 && S > num_kb)) continue;
+            const long long clusters = static_cast<long long>((N + R - 1) / R) * m_tiles;
+            int fit = resident[S] * sm_count / 148;
+            if (fit < 1) fit = 1;
+            const long long waves = (clusters + fit - 1) / fit;
+            const int kb = (num_kb + S - 1) / S;
+            // one SM takes ~60 GB/s through TMA, a stage of four MMAs and its hand-over ~360 ns, the chip ~6.3 TB/s;
+            // the epilogue ~25 ps a value (shared-memory round trip), a split ~0.7 us
+            const double t_load = kb * (stage / 60e9 > 360e-9 ? stage / 60e9 : 360e-9);
+            const double t_chip = static_cast<double>(clusters) * S * kb * stage / 6.3e12 / waves;
+            const double c = waves * ((t_load > t_chip ? t_load : t_chip) + 1.5e-6 + 25e-12 * rows * R / S + (S > 1 ? 0.7e-6 : 0.0));
+            if (c < best_cost) { best_cost = c; best.R = R; best.S = S; }
+        }
+    }
+    best.b_tiles = (best.R + 127) / 128;
+    best.stages = ring_limit(format, best.mbox, best.R, best.b_tiles);
+    if (stages_hint > 0 && stages_hint < best.stages) best.stages = stages_hint;
+    const int kb = (num_kb + best.S - 1) / best.S;
+    if (best.stages > kb) best.stages = kb;
+    best.tmem_cols = 32;
+    while (best.tmem_cols < best.R + best.stages * tiles * 4 * (1 + best.b_tiles)) best.tmem_cols *= 2;
+    const int stage = format == RDB_FP4_NVFP4 ? split_stage_bytes<RDB_FP4_NVFP4>(best.mbox, best.R, best.b_tiles)
+                                              : split_stage_bytes<RDB_FP4_MXFP4>(best.mbox, best.R, best.b_tiles);
+    // the ring, what the last stage's A operand reads beyond its rows, and the staging tile that reuses both
+    int bytes = best.stages * stage + A_OPERAND_SPAN;
+    const int stg = (rows + 31) / 32 * 32 * (best.R + 4) * 4;
+    if (bytes < stg) bytes = stg;
+    best.smem = 1024 + bytes;
+    return best;
+}
+
+template <int FMT>
+static int launch_split(const Product& q, const SplitPlan& pl, unsigned flags, const DeviceInfo* info, cudaStream_t stream) {
+    static bool attr_set[kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return RDB_CUDA_ERROR;
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(split_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT - 1024) != cudaSuccess) return RDB_CUDA_ERROR;
+        attr_set[dev] = true;
+    }
+    CUtensorMap tmA, tmB;
+    const uint64_t pitch = row_bytes(q.K);
+    int r = make_tmap_2d(&tmA, q.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.M, pitch, pitch, 128, pl.mbox, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r != RDB_SUCCESS) return r;
+    r = make_tmap_2d(&tmB, q.B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.N, pitch, pitch, 128, pl.R, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r != RDB_SUCCESS) return r;
+    SplitParams p;
+    p.D = q.D;
+    p.sa = q.sa; p.sb = q.sb; p.ta = q.ta; p.tb = q.tb;
+    p.status = info->status_dev;
+    p.M = q.M; p.N = q.N;
+    p.num_kb = (q.K + STAGE_K - 1) / STAGE_K;
+    p.R = pl.R; p.mbox = pl.mbox; p.b_tiles = pl.b_tiles;
+    p.sb_row_tiles = (q.N + 127) / 128;
+    p.nstages = pl.stages; p.tmem_cols = pl.tmem_cols;
+    p.out_type = q.out_type;
+    p.vec = q.N % 4 == 0 && (reinterpret_cast<uintptr_t>(q.D) & (q.out_type == RDB_TYPE_FP32 ? 15u : 7u)) == 0;
+    p.early_b = (flags & RDB_SKINNY_OVERLAP_PRIOR_KERNEL) != 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(pl.S, (q.N + pl.R - 1) / pl.R, (q.M + 127) / 128);
+    cfg.blockDim = dim3(SPLIT_THREADS);
+    cfg.dynamicSmemBytes = pl.smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = pl.S;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, split_kernel<FMT>, tmA, tmB, p) != cudaSuccess) { cudaGetLastError(); return RDB_CUDA_ERROR; }
+    return RDB_SUCCESS;
+}
+
+static int check(const Product& q, int format) {
+    if (q.M < 1 || q.N < 1 || q.K < 1) return RDB_BAD_SHAPE;
+    if (format != RDB_FP4_MXFP4 && format != RDB_FP4_NVFP4) return RDB_INVALID_CONFIG;
+    if (q.out_type != RDB_TYPE_BF16 && q.out_type != RDB_TYPE_FP16 && q.out_type != RDB_TYPE_FP32) return RDB_INVALID_CONFIG;
+    if (!q.A || !q.sa || !q.B || !q.sb || !q.D) return RDB_INVALID_CONFIG;
+    if (format == RDB_FP4_NVFP4 ? !q.ta || !q.tb : q.ta || q.tb) return RDB_INVALID_CONFIG;
+    if (!aligned16(q.A) || !aligned16(q.sa) || !aligned16(q.B) || !aligned16(q.sb) ||
+        reinterpret_cast<uintptr_t>(q.D) % (q.out_type == RDB_TYPE_FP32 ? 4 : 2) ||
+        (reinterpret_cast<uintptr_t>(q.ta) & 3u) || (reinterpret_cast<uintptr_t>(q.tb) & 3u))
+        return RDB_BAD_ALIGNMENT;
+    return RDB_SUCCESS;
+}
+
+static int run_split(const Product& q, int format, int r_hint, int s_hint, int stages_hint, unsigned flags, DeviceInfo* info, cudaStream_t stream) {
+    const SplitPlan pl = split_plan(format, q.M, q.N, q.K, info->sm_count, r_hint, s_hint, stages_hint);
+    // grid limits: 65535 tiles in y and z
+    if ((q.N + pl.R - 1) / pl.R > 65535 || (q.M + 127) / 128 > 65535) return RDB_SIZE_ABOVE_LIMIT;
+    return format == RDB_FP4_NVFP4 ? launch_split<RDB_FP4_NVFP4>(q, pl, flags, info, stream) : launch_split<RDB_FP4_MXFP4>(q, pl, flags, info, stream);
+}
+
+}  // namespace fp4
+}  // namespace rdb
+
+extern "C" {
+
+int rdb_skinny_gemm_fp4_tuned(const uint8_t* A, const uint8_t* scales_a, const float* tensor_scale_a, const uint8_t* B,
+                              const uint8_t* scales_b, const float* tensor_scale_b, void* D, int out_type, int M, int N, int K,
+                              int format, int columns_per_tile, int split_k, int stages, unsigned flags, void* stream) {
+    const rdb::fp4::Product q = {A, scales_a, B, scales_b, tensor_scale_a, tensor_scale_b, D, out_type, M, N, K};
+    const int ok = rdb::fp4::check(q, format);
+    if (ok != RDB_SUCCESS) return ok;
+    if (M > 32) return RDB_M_ABOVE_WARPTILE_M;
+    if (flags & ~RDB_SKINNY_OVERLAP_PRIOR_KERNEL) return RDB_INVALID_CONFIG;
+    if (columns_per_tile < 0 || columns_per_tile > 256 || columns_per_tile % 64 != 0 || split_k < 0 || split_k > 8 || stages < 0) return RDB_INVALID_CONFIG;
+    int err = 0;
+    rdb::DeviceInfo* info = rdb::device_info(&err);
+    if (!info) return err;
+    return rdb::fp4::run_split(q, format, columns_per_tile, split_k, stages, flags, info, static_cast<cudaStream_t>(stream));
+}
+
+int rdb_skinny_gemm_fp4(const uint8_t* A, const uint8_t* scales_a, const float* tensor_scale_a, const uint8_t* B,
+                        const uint8_t* scales_b, const float* tensor_scale_b, void* D, int out_type, int M, int N, int K, int format,
+                        unsigned flags, void* stream) {
+    return rdb_skinny_gemm_fp4_tuned(A, scales_a, tensor_scale_a, B, scales_b, tensor_scale_b, D, out_type, M, N, K, format, 0, 0, 0, flags, stream);
+}
+
+int rdb_dense_gemm_fp4(const uint8_t* A, const uint8_t* scales_a, const float* tensor_scale_a, const uint8_t* B, const uint8_t* scales_b,
+                       const float* tensor_scale_b, void* D, int out_type, int M, int N, int K, int format, void* stream) {
+    const rdb::fp4::Product q = {A, scales_a, B, scales_b, tensor_scale_a, tensor_scale_b, D, out_type, M, N, K};
+    const int ok = rdb::fp4::check(q, format);
+    if (ok != RDB_SUCCESS) return ok;
+    int err = 0;
+    rdb::DeviceInfo* info = rdb::device_info(&err);
+    if (!info) return err;
+    return rdb::fp4::run_split(q, format, 0, 0, 0, 0, info, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,369 @@
+"""Microscaled 4-bit floating point: quantisers bit for bit, products against a 64-bit product of the held values.
+
+Tolerance of a product, per element: half a step of the output type, 3 fp32 roundings for the tensor scales and their
+products, and the summation-order noise 4 sqrt(K) 2^-24 sum|a b| of an fp32 accumulation (as in the fp8 tests): the
+products themselves, and a block's scale times them, are exact."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+FORMATS = ["mxfp4", "nvfp4"]
+BLOCK = {"mxfp4": 32, "nvfp4": 16}
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}    # half a step near zero
+LEVELS = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6])
+
+
+# ------------------------------------------------------------------ plain implementation (numpy)
+def e2m1_codes(q):
+    """Nearest code by distance, ties to the even one, signs kept."""
+    a = np.minimum(np.abs(q.astype(np.float64)), 6.0)
+    d = np.abs(a[..., None] - LEVELS[:8])
+    best = d.min(axis=-1, keepdims=True)
+    near = d == best
+    even = near & (np.arange(8) % 2 == 0)
+    code = np.where(even.any(axis=-1), even.argmax(axis=-1), near.argmax(axis=-1))
+    return (code | (np.signbit(q) << 3)).astype(np.uint8)
+
+
+def e4m3_bytes(v):
+    """Non-negative fp32 -> e4m3 bytes, nearest, ties to even, saturating."""
+    all_ = torch.arange(0, 0x7F, dtype=torch.uint8).view(torch.float8_e4m3fn).to(torch.float64).numpy()
+    v = np.minimum(v.astype(np.float64), 448.0)
+    hi = np.clip(np.searchsorted(all_, v), 1, 0x7E)
+    lo = hi - 1
+    dl, dh = v - all_[lo], all_[hi] - v
+    return np.where((dl < dh) | ((dl == dh) & (lo % 2 == 0)), lo, hi).astype(np.uint8)
+
+
+def e4m3_values(b):
+    return torch.from_numpy(np.ascontiguousarray(b)).view(torch.float8_e4m3fn).float().numpy()
+
+
+def quantize(x, form, t=None):
+    """fp32 [rows, K] -> (codes [rows, K32] one per byte, scale bytes [rows, blocks of the padded K], tensor scale)."""
+    rows, K = x.shape
+    b, kp = BLOCK[form], (K + 31) // 32 * 32
+    v = np.zeros((rows, kp), np.float32)
+    v[:, :K] = x
+    v = v.reshape(rows, -1, b)
+    bad = ~np.isfinite(v).all(axis=2)
+    a = np.abs(v)
+    amax = a.max(axis=2)
+    with np.errstate(all="ignore"):
+        if form == "mxfp4":
+            e = np.where(amax > 0, np.frexp(np.where(bad, 1, amax))[1] - 3, -127).clip(-127, 127)
+            q = np.ldexp(v.astype(np.float64), -e[..., None])
+            s = (e + 127).astype(np.uint8)
+            s[bad] = 0xFF
+        else:
+            if t is None:
+                top = np.where(np.isfinite(v), a, 0).max()
+                t = np.float32(1) if top == 0 else np.maximum(np.float32(top) / np.float32(2688), np.float32(2.0 ** -126))
+            t = np.float32(t)
+            s = e4m3_bytes(np.where(bad, 0, amax / (t * np.float32(6))))
+            whole = e4m3_values(s) * t
+            q = np.where(s[..., None] > 0, v / np.where(s > 0, whole, 1).astype(np.float32)[..., None], 0)
+            s = np.where(bad, np.uint8(0x7F), s)
+        q = np.where(bad[..., None], 0, q)          # codes of a block without values are not compared
+    return e2m1_codes(q).reshape(rows, kp), s, t, bad
+
+
+def values(codes, scales, form, K, t=None):
+    """64-bit values of plain codes and scale bytes, without the tensor scale."""
+    v = LEVELS[codes]
+    s = np.where(scales == 0xFF, np.nan, 2.0 ** (scales.astype(np.float64) - 127)) if form == "mxfp4" else e4m3_values(scales).astype(np.float64)
+    return (v.reshape(v.shape[0], -1, BLOCK[form]) * s[..., None]).reshape(v.shape[0], -1)[:, :K]
+
+
+def plain(t):
+    """A held tensor on the device -> (codes one per byte, plain scale bytes, tensor scale) by the documented layout."""
+    import rocm_dev_b200 as R
+    c = t.codes.cpu().numpy()
+    codes = np.stack([c & 15, c >> 4], axis=-1).reshape(c.shape[0], -1)
+    b = BLOCK[t.format]
+    flat, across = t.scales.cpu().numpy(), (t.K + 255) // 256 * (256 // b) // 4
+    r, k = np.arange(t.rows)[:, None], np.arange(across * 4)[None, :]
+    s = flat[(r // 128 * across + k // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + k % 4]
+    nb = codes.shape[1] // b
+    assert not s[:, nb:].any(), "scales behind K must be zero"
+    assert np.array_equal(R.unpack_fp4_scales(t).cpu().numpy(), s[:, :(t.K + b - 1) // b])
+    return codes, s[:, :nb], None if t.tensor_scale is None else np.float32(t.tensor_scale.item())
+
+
+def check_quantized(got, x, form, t=None):
+    codes, scales, ts = plain(got)
+    wc, ws, wt, bad = quantize(x, form, t)
+    if form == "nvfp4":
+        assert ts == wt
+    assert np.array_equal(scales, ws)
+    keep = np.repeat(~bad, BLOCK[form], axis=1)
+    if form == "nvfp4":                              # a block whose scale is zero holds zeros of no sign
+        zero = np.repeat(ws == 0, BLOCK[form], axis=1)
+        assert not codes[zero & keep].any()
+        keep &= ~zero
+    assert np.array_equal(codes[keep], wc[keep])
+
+
+def draw(rows, K, seed, dtype=torch.bfloat16, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((rows, K), generator=g) * std * torch.exp2(torch.randint(-6, 7, (rows, 1), generator=g).float())
+    return x.to(dtype)
+
+
+def held(x, form, dev):
+    import rocm_dev_b200 as R
+    return R.quantize_fp4(x.to(dev), form)
+
+
+def check_product(got, A, B):
+    """`got` against the 64-bit product of what A and B hold."""
+    (ca, sa, ta), (cb, sb, tb) = plain(A), plain(B)
+    a, b = values(ca, sa, A.format, A.K), values(cb, sb, B.format, B.K)
+    alpha = 1.0 if ta is None else float(ta) * float(tb)
+    want, mag = a @ b.T * alpha, np.abs(a) @ np.abs(b).T * alpha
+    tol = HALF[got.dtype] * np.abs(want) + TINY[got.dtype] + (4 * np.sqrt(A.K) + 3) * 2.0 ** -24 * mag
+    err = np.abs(got.double().cpu().numpy() - want)
+    assert np.isfinite(err).all()
+    assert (err <= tol).all(), f"{(err > tol).sum()} of {err.size} outside, worst {np.max(err / np.maximum(tol, 1e-300)):.3g} times the tolerance"
+
+
+# ------------------------------------------------------------------ CPU
+def test_sizes_of_the_held_form():
+    import rocm_dev_b200 as R
+    from rocm_dev_b200 import fp4
+    L = R.lib()
+    for rows, K in [(1, 1), (127, 31), (128, 256), (129, 257), (5, 4100), (2 ** 20, 14336)]:
+        assert L.rdb_fp4_row_bytes(K) == fp4.row_bytes(K)
+        for f in FORMATS:
+            assert L.rdb_fp4_scale_bytes(fp4.FORMATS[f], rows, K) == fp4.scale_bytes(f, rows, K)
+    assert L.rdb_fp4_row_bytes(0) == 0 and L.rdb_fp4_scale_bytes(1, 0, 5) == 0 and L.rdb_fp4_scale_bytes(2, 5, 5) == 0
+
+
+def test_scale_tiles_round_trip():
+    import rocm_dev_b200 as R
+    for f, rows, K in [("mxfp4", 130, 700), ("nvfp4", 1, 16), ("nvfp4", 300, 1030)]:
+        s = torch.randint(0, 255, (rows, -(-K // BLOCK[f])), dtype=torch.uint8)
+        t = R.Fp4Tensor(None, R.pack_fp4_scales(s, f, K), None, f, rows, K)
+        assert torch.equal(R.unpack_fp4_scales(t), s)
+
+
+def test_refusals_before_anything_is_launched():
+    import rocm_dev_b200 as R
+    L = R.lib()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    Q = lambda **k: L.rdb_quantize_fp4(*{**dict(x=p, typ=0, ldx=64, rows=4, K=64, fmt=1, ts=p, given=0, codes=p, scales=p, ct=None, st=None, ws=p, stream=None), **k}.values())  # noqa: E731
+    assert Q(rows=0) == 8 and Q(K=0) == 8 and Q(ldx=63) == 8
+    assert Q(fmt=2) == 6 and Q(typ=3) == 6 and Q(x=None) == 6 and Q(codes=None) == 6 and Q(scales=None) == 6
+    assert Q(ts=None) == 6 and Q(ws=None) == 6 and Q(ct=p) == 6
+    assert Q(x=p + 1) == 7 and Q(codes=p + 8) == 7 and Q(scales=p + 4) == 7 and Q(ts=p + 2) == 7 and Q(typ=2, x=p + 2) == 7
+    D = lambda **k: L.rdb_dequantize_fp4(*{**dict(codes=p, scales=p, ts=p, fmt=1, rows=4, K=64, out=p, typ=0, stream=None), **k}.values())  # noqa: E731
+    assert D(rows=0) == 8 and D(fmt=-1) == 6 and D(typ=9) == 6 and D(ts=None) == 6 and D(out=None) == 6 and D(out=p + 1) == 7
+    base = dict(A=p, sa=p, ta=p, B=p, sb=p, tb=p, D=p, typ=0, M=4, N=8, K=64, fmt=1)
+    dense = lambda **k: L.rdb_dense_gemm_fp4(*{**base, **k}.values(), None)  # noqa: E731
+    skinny = lambda flags=0, **k: L.rdb_skinny_gemm_fp4(*{**base, **k}.values(), flags, None)  # noqa: E731
+    for call in (dense, skinny):
+        assert call(M=0) == 8 and call(N=0) == 8 and call(K=-1) == 8
+        assert call(fmt=5) == 6 and call(typ=-1) == 6 and call(A=None) == 6 and call(D=None) == 6 and call(ta=None) == 6
+        assert call(fmt=0) == 6                                     # mxfp4 has no tensor scales
+        assert call(A=p + 8) == 7 and call(sb=p + 1) == 7 and call(D=p + 1) == 7 and call(typ=2, D=p + 2) == 7
+    assert skinny(M=33) == 1 and skinny(flags=2) == 6
+    tuned = lambda **k: L.rdb_skinny_gemm_fp4_tuned(*{**base, **dict(cols=0, split=0, st=0, flags=0), **k}.values(), None)  # noqa: E731
+    assert tuned(cols=32) == 6 and tuned(cols=320) == 6 and tuned(split=9) == 6 and tuned(st=-1) == 6 and tuned(M=40) == 1
+
+
+def test_refusals_of_the_python_face():
+    import rocm_dev_b200 as R
+    x = torch.zeros(4, 64)
+    with pytest.raises(ValueError):
+        R.quantize_fp4(x, "fp4")
+    with pytest.raises(TypeError):
+        R.quantize_fp4(x.double())
+    with pytest.raises(AssertionError):
+        R.quantize_fp4(x)                                            # there is no CPU path
+
+
+# ------------------------------------------------------------------ quantisers
+SHAPES = [(1, 1), (1, 16), (2, 17), (3, 31), (5, 32), (8, 4096), (130, 257), (33, 1000), (257, 129), (700, 48)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,K", SHAPES)
+def test_quantize_bits(cuda_device, form, dtype, rows, K):
+    import rocm_dev_b200 as R
+    x = draw(rows, K, rows * 7 + K, dtype)
+    r, c = R.quantize_fp4_both(x.to(cuda_device), form)
+    one = R.quantize_fp4(x.to(cuda_device), form)
+    v = x.float().numpy()
+    check_quantized(r, v, form)
+    check_quantized(one, v, form)
+    check_quantized(c, np.ascontiguousarray(v.T), form)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("left,right", [(0, 8), (1, 2), (8, 24), (3, 0)])
+def test_quantize_rows_a_pitch_apart(cuda_device, form, dtype, left, right):
+    import rocm_dev_b200 as R
+    wide = draw(70, left + 272 + right, 5, dtype).to(cuda_device)
+    x = wide[:, left:left + 272]
+    r, c = R.quantize_fp4_both(x, form)
+    v = x.float().cpu().numpy()
+    check_quantized(r, v, form)
+    check_quantized(c, np.ascontiguousarray(v.T), form)
+    check_quantized(R.quantize_fp4(x.t(), form), np.ascontiguousarray(v.T), form)      # a view with no unit stride
+    check_quantized(R.quantize_fp4(x[:1].expand(5, -1), form), np.repeat(v[:1], 5, axis=0), form)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_quantize_every_bf16_number(cuda_device, form):
+    """All finite bf16 patterns: each value meets itself and larger ones in its block, subnormals and -0 included."""
+    import rocm_dev_b200 as R
+    bits = torch.arange(65536, dtype=torch.int32)
+    bits = bits[(bits & 0x7F80) != 0x7F80].to(torch.int16)
+    x = bits.view(torch.bfloat16).reshape(-1, 128)
+    for v in (x, x.t().contiguous()):
+        r, c = R.quantize_fp4_both(v.to(cuda_device), form)
+        check_quantized(r, v.float().numpy(), form)
+        check_quantized(c, v.float().numpy().T.copy(), form)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_quantize_borders(cuda_device, form, dtype):
+    """Quotients on the borders between two codes and one step of the input type to either side of them."""
+    import rocm_dev_b200 as R
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0], dtype=dtype)
+    around = torch.cat([ties, torch.nextafter(ties, ties * 0), torch.nextafter(ties, ties * 9)])
+    x = torch.zeros(64, 32, dtype=dtype)
+    x[:, :24] = around
+    x[:, 24:] = 6.0
+    x *= torch.linspace(1, 1.96875, 64, dtype=dtype)[:, None]
+    x[1::2] *= -1
+    t = None if form == "mxfp4" else torch.tensor([1.0])
+    for k in (t,) if form == "mxfp4" else (t, torch.tensor([0.0123]), None):
+        r, c = R.quantize_fp4_both(x.to(cuda_device), form, None if k is None else k.to(cuda_device))
+        check_quantized(r, x.float().numpy(), form, None if k is None else k.item())
+        check_quantized(c, x.float().numpy().T.copy(), form, None if k is None else k.item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_quantize_what_is_no_number(cuda_device, form):
+    """Infinities and NaNs take their own block's scale with them and leave the others - and the tensor scale - alone."""
+    import rocm_dev_b200 as R
+    x = draw(40, 320, 3, torch.float32)
+    x[0, 0], x[3, 70], x[3, 319], x[39, 160] = float("inf"), float("nan"), float("-inf"), float("nan")
+    x[5], x[6, :64] = 0.0, -0.0
+    for v in (x, x.bfloat16()):
+        r, c = R.quantize_fp4_both(v.to(cuda_device), form)
+        check_quantized(r, v.float().numpy(), form)
+        check_quantized(c, v.float().numpy().T.copy(), form)
+        d = R.dequantize_fp4(r, torch.float32).cpu()
+        b = BLOCK[form]
+        bad = ~torch.isfinite(v.float()).reshape(40, -1, b).all(dim=2)
+        assert torch.equal(torch.isnan(d).reshape(40, -1, b).all(dim=2), bad) and torch.equal(torch.isnan(d).reshape(40, -1, b).any(dim=2), bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("fill", [0.0, 1e-45, 1e-38, 3.3e38])
+def test_quantize_extreme_tensors(cuda_device, form, fill):
+    import rocm_dev_b200 as R
+    x = torch.full((20, 50), fill)
+    x[:, ::3] = -fill / 3
+    r, c = R.quantize_fp4_both(x.to(cuda_device), form)
+    check_quantized(r, x.numpy(), form)
+    check_quantized(c, x.numpy().T.copy(), form)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("rows,K", [(1, 1), (3, 33), (130, 512), (65, 1001), (16, 4096)])
+def test_dequantize(cuda_device, form, rows, K):
+    import rocm_dev_b200 as R
+    t = held(draw(rows, K, 9), form, cuda_device)
+    codes, scales, ts = plain(t)
+    want = values(codes, scales, form, K).astype(np.float32)         # exact in fp32
+    want = want if ts is None else want * ts
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        got = R.dequantize_fp4(t, dtype).cpu()
+        assert got.shape == (rows, K) and torch.equal(got, torch.from_numpy(want).to(dtype))
+
+
+# ------------------------------------------------------------------ products
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("where", ["skinny", "dense"])
+def test_one_hot_operands_find_their_codes_and_scales(cuda_device, form, where):
+    """A = rows of the identity (code 1.0, scale 1): D[m, n] is exactly the value B holds at (n, k(m))."""
+    import rocm_dev_b200 as R
+    M, N, K = (32 if where == "skinny" else 300), 330, 700
+    B = held(draw(N, K, 2), form, cuda_device)
+    k = (np.arange(M) * 37 + 5) % K
+    eye = torch.zeros(M, K)
+    eye[torch.arange(M), torch.from_numpy(k)] = 6.0                  # 6 -> code 6.0 (mxfp4: 4 * 1.5), a power-of-two scale
+    one = torch.ones(1, device=cuda_device)
+    A = R.quantize_fp4(eye.to(cuda_device), form, None if form == "mxfp4" else one)
+    got = (R.skinny_gemm_fp4 if where == "skinny" else R.dense_gemm_fp4)(A, B, out_dtype=torch.float32)
+    cb, sb, tb = plain(B)
+    want = (6 * values(cb, sb, form, K)[:, k].T).astype(np.float32) * (np.float32(1) if tb is None else tb)
+    torch.cuda.synchronize()
+    assert R.lib().rdb_device_status() == 0
+    assert np.array_equal(got.cpu().numpy(), want)
+
+
+PRODUCTS = [(1, 1, 1), (1, 8, 16), (5, 64, 256), (8, 130, 257), (16, 256, 512), (17, 1001, 300), (32, 192, 2048), (3, 515, 4100),
+            (31, 4096, 64), (1, 2048, 8192)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_skinny_product(cuda_device, form, dtype, M, N, K):
+    import rocm_dev_b200 as R
+    A, B = held(draw(M, K, 1, std=0.1), form, cuda_device), held(draw(N, K, 2, std=0.02), form, cuda_device)
+    got = R.skinny_gemm_fp4(A, B, out_dtype=dtype)
+    torch.cuda.synchronize()
+    assert R.lib().rdb_device_status() == 0
+    check_product(got, A, B)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("columns", [64, 128, 192, 256])
+@pytest.mark.parametrize("split,stages", [(1, 0), (1, 1), (2, 2), (3, 0), (8, 0)])
+def test_every_tile_width_and_split(cuda_device, form, columns, split, stages):
+    import rocm_dev_b200 as R
+    for M in (4, 29):
+        A, B = held(draw(M, 2500, 3, std=0.1), form, cuda_device), held(draw(900, 2500, 4, std=0.02), form, cuda_device)
+        out = torch.full((M, 900), float("nan"), device=cuda_device)
+        args, _, dev = R.fp4._product(A, B, out, None)
+        assert R.lib().rdb_skinny_gemm_fp4_tuned(*args, columns, split, stages, 0, torch.cuda.current_stream(dev).cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert R.lib().rdb_device_status() == 0
+        check_product(out, A, B)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("M,N,K,dtype", [(1, 1, 1, torch.float32), (33, 100, 96, torch.bfloat16), (64, 64, 64, torch.float16),
+                                         (65, 300, 1000, torch.float32), (128, 256, 256, torch.bfloat16), (129, 257, 513, torch.float32),
+                                         (200, 4096, 128, torch.bfloat16), (333, 1001, 4100, torch.float32),
+                                         (1024, 768, 2304, torch.bfloat16), (2, 5000, 320, torch.float16)])
+def test_dense_product(cuda_device, form, M, N, K, dtype):
+    import rocm_dev_b200 as R
+    A, B = held(draw(M, K, 1, std=0.1), form, cuda_device), held(draw(N, K, 2, std=0.02), form, cuda_device)
+    got = R.dense_gemm_fp4(A, B, out_dtype=dtype)
+    torch.cuda.synchronize()
+    assert R.lib().rdb_device_status() == 0
+    check_product(got, A, B)
