@@ -231,7 +231,7 @@ int rdb_dense_gemm_fp8_f32(const uint8_t *A, const uint8_t *B, float *D, int M, 
  *                  to [-127, 127]; element = e2m1(x / 2^e).  This is the conversion of the OCP Microscaling Formats
  *                  specification, version 1.0.
  *   RDB_FP4_NVFP4  blocks of 16 along K share an e4m3 scale s, the tensor one fp32 scale t: t given, or the largest
- *                  finite magnitude / 2688 (not below 2^-126; 1 if all are zero); s = e4m3_sat(block's largest
+ *                  finite magnitude times fp32(1 / 2688) (not below 2^-126; 1 if all are zero); s = e4m3_sat(block's largest
  *                  magnitude / (6 t)); element = e2m1(x / (t s)), zero where s is.  6 t, t s and both quotients are
  *                  rounded to fp32.  t must be a positive number.
  * A block that holds an infinity or a NaN gets the scale type's NaN, and what is computed from it is NaN.

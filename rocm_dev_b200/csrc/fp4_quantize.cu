@@ -2,8 +2,8 @@
 //
 // MXFP4: a block of 32 with largest magnitude a > 0 is scaled by 2^e, e = floor(log2 a) - 2 (2 = exponent of e2m1's
 // largest number) clamped to [-127, 127]; e = -127 for a = 0.  Element = e2m1(x * 2^-e).
-// NVFP4: the tensor has one fp32 scale t - given, or max|x| / 2688 (448 * 6) but no lower than 2^-126, 1 for an all-zero
-// tensor - and a block of 16 an e4m3 scale s = e4m3_sat(a / (6 t)).  Element = e2m1(x / (t s)), zero where s is.  6 t,
+// NVFP4: the tensor has one fp32 scale t - given, or max|x| * fp32(1 / 2688) (2688 = 448 * 6) but no lower than 2^-126, 1
+// for an all-zero tensor - and a block of 16 an e4m3 scale s = e4m3_sat(a / (6 t)).  Element = e2m1(x / (t s)), zero where s is.  6 t,
 // t s and both quotients are rounded to fp32 (IEEE), which makes the codes reproducible bit for bit.
 // e2m1 rounds to nearest, ties to the even code, and saturates at 6.  A block that holds an infinity or a NaN gets the
 // scale type's NaN (0xFF, 0x7F): whatever is computed from it is NaN, and the other blocks keep their values - t is the
@@ -152,7 +152,8 @@ __device__ __forceinline__ float tensor_scale(const float* given, const uint32_t
     uint32_t m = 0;
     for (int i = threadIdx.x & 31; i < count; i += 32) m = max(m, __ldcg(partial + i));
     m = __reduce_max_sync(0xffffffffu, m);
-    return m == 0 ? 1.0f : fmaxf(__fdiv_rn(__uint_as_float(m), 2688.0f), 1.17549435e-38f);
+    constexpr float inv = 1.0f / 2688.0f;            // rounded to fp32 before it multiplies: part of the definition
+    return m == 0 ? 1.0f : fmaxf(__fmul_rn(__uint_as_float(m), inv), 1.17549435e-38f);
 }
 
 template <class T>

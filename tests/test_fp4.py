@@ -61,7 +61,7 @@ def quantize(x, form, t=None):
         else:
             if t is None:
                 top = np.where(np.isfinite(v), a, 0).max()
-                t = np.float32(1) if top == 0 else np.maximum(np.float32(top) / np.float32(2688), np.float32(2.0 ** -126))
+                t = np.float32(1) if top == 0 else np.maximum(np.float32(top) * np.float32(1 / 2688), np.float32(2.0 ** -126))
             t = np.float32(t)
             s = e4m3_bytes(np.where(bad, 0, amax / (t * np.float32(6))))
             whole = e4m3_values(s) * t
