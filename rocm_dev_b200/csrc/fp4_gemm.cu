@@ -224,6 +224,199 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     }
 }
 
+// ------------------------------------------------------------- CTA pairs
+// pair_kernel: persistent clusters of two CTAs compute 256 x 256 tiles with cta_group::2 MMAs.  CTA r of the pair loads
+// rows [128 r, 128 r + 128) of the A tile and of the B tile, the scales of its A rows and those of ALL 256 B rows (each
+// SM scales its own 128 x 256 half of the tile); the even CTA issues the scale copies and the MMAs for both.
+// TMEM (512 columns): two accumulators of 256 columns that overlap by OVERLAP, then the scale slots.  The epilogue empties
+// the shared columns first, so the next tile's MMAs wait for those alone.
+namespace pairs {
+constexpr int THREADS = 224;                    // warp 0: A loads, 1: MMA, 2-5: epilogue, 6: B loads
+constexpr int ACC1 = 160, SCALE_COL = ACC1 + 256, GROUP_M = 16;
+template <int FMT>
+struct Cfg {
+    static constexpr int SCALES = Format<FMT>::TILES * TILE_BYTES;
+    static constexpr int STAGE = 2 * 128 * 128 + 3 * SCALES;
+    static constexpr int STAGES = FMT == RDB_FP4_NVFP4 ? 5 : 6;
+    static constexpr int SLOT = Format<FMT>::TILES * 12, SLOTS = (512 - SCALE_COL) / SLOT;      // 2 or 4
+    static constexpr int SMEM = 1024 + STAGES * STAGE;
+};
+}  // namespace pairs
+
+struct PairParams {
+    void* D;
+    const float *ta, *tb;
+    int* status;
+    int M, N, num_kb, tiles_m, tiles_n;
+    int out_type, vec;
+};
+
+__device__ __forceinline__ void tile_coords(int tile, int tiles_m, int tiles_n, int& mb, int& nb) {
+    const int per_group = pairs::GROUP_M * tiles_n;
+    const int g = tile / per_group, r = tile - g * per_group;
+    const int first = g * pairs::GROUP_M;
+    const int gsize = tiles_m - first < pairs::GROUP_M ? tiles_m - first : pairs::GROUP_M;
+    mb = first + r % gsize;
+    nb = r / gsize;
+}
+
+template <int FMT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pairs::THREADS, 1)
+pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
+            const __grid_constant__ CUtensorMap tmSB, const PairParams p) {
+    using C = pairs::Cfg<FMT>;
+    constexpr int STAGES = C::STAGES, STAGE = C::STAGE, SCALES = C::SCALES, TILES = Format<FMT>::TILES, HALF = 128 * 128;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t bars[2 * STAGES + 2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_s;
+    volatile int* abort_flag = &abort_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair_id = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+    const uint32_t acc_full = smem_u32(bars + 2 * STAGES), acc_free = smem_u32(bars + 2 * STAGES + 1);
+    const uint32_t stage0 = smem_u32(smem);
+
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmB);
+        prefetch_tensormap(&tmSA);
+        prefetch_tensormap(&tmSB);
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_free, 8);                 // four epilogue warps in each CTA of the pair
+        abort_s = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(&tmem_slot), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_arrive_release();                   // both CTAs' barriers and TMEM exist before either touches the other
+    cluster_wait_acquire();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_slot;
+    const int num_tiles = p.tiles_m * p.tiles_n;
+    pdl_launch_dependents();
+    pdl_wait_prior();
+
+    if (warp == 0 || warp == 6) {
+        if (lane == 0) {
+            const bool is_a = warp == 0;
+            const CUtensorMap* tm = is_a ? &tmA : &tmB;
+            const CUtensorMap* ts = is_a ? &tmSA : &tmSB;
+            const uint32_t off = is_a ? 0u : static_cast<uint32_t>(HALF), soff = 2 * HALF + (is_a ? 0 : SCALES);
+            const uint64_t pol = l2_policy_evict_last();
+            const uint32_t full_even0 = mapa_smem(full0, 0);
+            int it = 0;
+            bool ok = true;
+            for (int tile = pair_id; tile < num_tiles && ok && *abort_flag == 0; tile += num_pairs) {
+                int mb, nb;
+                tile_coords(tile, p.tiles_m, p.tiles_n, mb, nb);
+                const int row = (is_a ? mb : nb) * 256 + static_cast<int>(rank) * 128;
+                const int plane = is_a ? mb * 2 + static_cast<int>(rank) : nb * 2;
+                for (int kb = 0; kb < p.num_kb; kb++, it++) {
+                    const int s = it % STAGES;
+                    if (!mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1)) { ok = false; break; }
+                    if (is_a && rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * STAGE);
+                    tma_load_2d_pair(stage0 + s * STAGE + off, tm, kb * 128, row, full_even0 + 8 * s, pol);
+                    tma_load_3d_pair(stage0 + s * STAGE + soff, ts, 0, kb * (SCALES / 256), plane, full_even0 + 8 * s, pol);
+                }
+            }
+            // every commit aimed at this CTA's `empty` barriers must land before the CTA may exit
+            for (int i = 0; i < STAGES && ok && *abort_flag == 0; i++, it++) {
+                const int s = it % STAGES;
+                if (!mbar_wait(empty0 + 8 * s, ((it / STAGES) & 1) ^ 1)) ok = false;
+            }
+            if (!ok) { *abort_flag = 1; report_timeout(p.status); }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int it = 0, t = 0;
+            bool ok = true;
+            for (int tile = pair_id; tile < num_tiles && ok && *abort_flag == 0; tile += num_pairs, t++) {
+                const uint32_t d = tmem_base + (t & 1) * pairs::ACC1;
+                for (int kb = 0; kb < p.num_kb; kb++, it++) {
+                    const int s = it % STAGES;
+                    // the scale slot is free when the MMAs of SLOTS stages ago have finished
+                    if (it >= C::SLOTS) {
+                        const int old = it - C::SLOTS;
+                        if (!mbar_wait(empty0 + 8 * (old % STAGES), (old / STAGES) & 1)) { ok = false; break; }
+                    }
+                    if (!mbar_wait(full0 + 8 * s, (it / STAGES) & 1)) { ok = false; break; }
+                    tc_fence_after_sync();
+                    const uint32_t a = stage0 + s * STAGE, b = a + HALF, sc = b + HALF;
+                    const uint32_t tsa = tmem_base + pairs::SCALE_COL + (it % C::SLOTS) * C::SLOT, tsb = tsa + 4 * TILES;
+#pragma unroll
+                    for (int i = 0; i < TILES; i++) {
+                        tmem_cp_scales<true>(tsa + 4 * i, sc + i * TILE_BYTES);
+                        tmem_cp_scales<true>(tsb + 8 * i, sc + SCALES + i * TILE_BYTES);
+                        tmem_cp_scales<true>(tsb + 8 * i + 4, sc + 2 * SCALES + i * TILE_BYTES);
+                    }
+                    if (kb == 0 && t > 0) {
+                        if (!mbar_wait_cluster(acc_free, (t - 1) & 1)) { ok = false; break; }
+                        tc_fence_after_sync();
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 4; ks++) {
+                        const int i = ks * TILES / 4, id = TILES == 4 ? 0 : 2 * (ks & 1);
+                        tc_mma_fp4<FMT, true>(d, smem_desc_k128(a + ks * 32), smem_desc_k128(b + ks * 32), idesc_fp4<FMT>(256, 256, id),
+                                              tsa + 4 * i, tsb + 8 * i, (kb | ks) != 0);
+                    }
+                    tc_commit_pair_both(empty0 + 8 * s);
+                    if (kb == p.num_kb - 1) tc_commit_pair_both(acc_full);
+                }
+            }
+            if (!ok) { *abort_flag = 1; report_timeout(p.status); }
+        }
+        __syncwarp();
+    } else {
+        const int quad = warp & 3;
+        const float alpha = p.ta ? __ldg(p.ta) * __ldg(p.tb) : 1.0f;
+        const uint32_t free_even = mapa_smem(acc_free, 0);
+        int t = 0;
+        for (int tile = pair_id; tile < num_tiles; tile += num_pairs, t++) {
+            int mb, nb;
+            tile_coords(tile, p.tiles_m, p.tiles_n, mb, nb);
+            if (!mbar_wait(acc_full, t & 1)) { *abort_flag = 1; report_timeout(p.status); }
+            if (*abort_flag != 0) break;
+            tc_fence_after_sync();
+            const int row = mb * 256 + static_cast<int>(rank) * 128 + quad * 32 + lane;
+            const uint32_t taddr = tmem_base + (t & 1) * pairs::ACC1 + (static_cast<uint32_t>(quad * 32) << 16);
+            // columns shared with the other accumulator first: the last 96 of the first, the first 96 of the second
+#pragma unroll 1
+            for (int i = 0; i < 8; i++) {
+                const int c0 = (t & 1) ? 32 * i : (i < 3 ? pairs::ACC1 + 32 * i : 32 * (i - 3));
+                float v[32];
+                tmem_ld32(taddr + c0, v);
+                if (i == 2) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(free_even);
+                }
+                if (row < p.M && nb * 256 + c0 < p.N) store32(p.D, p.out_type, p.N, row, nb * 256 + c0, v, alpha, p.vec);
+            }
+        }
+    }
+
+    if (*abort_flag != 0) {
+        for (int i = 0; i < 64; i++) __nanosleep(2000);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_arrive_release();                   // neither CTA frees TMEM or exits while the other may still signal it
+    cluster_wait_acquire();
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
 // ------------------------------------------------------------------ host
 struct Product {
     const uint8_t *A, *sa, *B, *sb;
@@ -335,6 +528,50 @@ static int launch_split(const Product& q, const SplitPlan& pl, unsigned flags, c
     return RDB_SUCCESS;
 }
 
+template <int FMT>
+static int launch_pair(const Product& q, int max_ctas, const DeviceInfo* info, cudaStream_t stream) {
+    using C = pairs::Cfg<FMT>;
+    static bool attr_set[kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return RDB_CUDA_ERROR;
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(pair_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return RDB_CUDA_ERROR;
+        attr_set[dev] = true;
+    }
+    PairParams p;
+    p.D = q.D;
+    p.ta = q.ta; p.tb = q.tb;
+    p.status = info->status_dev;
+    p.M = q.M; p.N = q.N;
+    p.num_kb = (q.K + STAGE_K - 1) / STAGE_K;
+    p.tiles_m = (q.M + 255) / 256;
+    p.tiles_n = (q.N + 255) / 256;
+    p.out_type = q.out_type;
+    p.vec = q.N % (q.out_type == RDB_TYPE_FP32 ? 4 : 8) == 0 && aligned16(q.D);
+    CUtensorMap tmA, tmB, tmSA, tmSB;
+    const uint64_t pitch = row_bytes(q.K), scale_rows = static_cast<uint64_t>(p.num_kb) * C::SCALES / 256;
+    int r = make_tmap_2d(&tmA, q.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.M, pitch, pitch, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r == RDB_SUCCESS) r = make_tmap_2d(&tmB, q.B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.N, pitch, pitch, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r == RDB_SUCCESS) r = make_tmap_bytes256(&tmSA, q.sa, scale_rows, (q.M + 127) / 128, C::SCALES / 256, 1);
+    if (r == RDB_SUCCESS) r = make_tmap_bytes256(&tmSB, q.sb, scale_rows, (q.N + 127) / 128, C::SCALES / 256, 2);
+    if (r != RDB_SUCCESS) return r;
+    int num_pairs = p.tiles_m * p.tiles_n, cap = info->sm_count / 2;
+    if (max_ctas > 0 && max_ctas / 2 < cap) cap = max_ctas / 2 > 0 ? max_ctas / 2 : 1;
+    if (num_pairs > cap) num_pairs = (num_pairs + (num_pairs + cap - 1) / cap - 1) / ((num_pairs + cap - 1) / cap);    // same waves, fewest CTAs
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * num_pairs);
+    cfg.blockDim = dim3(pairs::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, pair_kernel<FMT>, tmA, tmB, tmSA, tmSB, p) != cudaSuccess) { cudaGetLastError(); return RDB_CUDA_ERROR; }
+    return RDB_SUCCESS;
+}
+
 static int check(const Product& q, int format) {
     if (q.M < 1 || q.N < 1 || q.K < 1) return RDB_BAD_SHAPE;
     if (format != RDB_FP4_MXFP4 && format != RDB_FP4_NVFP4) return RDB_INVALID_CONFIG;
@@ -381,15 +618,29 @@ int rdb_skinny_gemm_fp4(const uint8_t* A, const uint8_t* scales_a, const float* 
     return rdb_skinny_gemm_fp4_tuned(A, scales_a, tensor_scale_a, B, scales_b, tensor_scale_b, D, out_type, M, N, K, format, 0, 0, 0, flags, stream);
 }
 
-int rdb_dense_gemm_fp4(const uint8_t* A, const uint8_t* scales_a, const float* tensor_scale_a, const uint8_t* B, const uint8_t* scales_b,
-                       const float* tensor_scale_b, void* D, int out_type, int M, int N, int K, int format, void* stream) {
+int rdb_dense_gemm_fp4_tuned(const uint8_t* A, const uint8_t* scales_a, const float* tensor_scale_a, const uint8_t* B,
+                             const uint8_t* scales_b, const float* tensor_scale_b, void* D, int out_type, int M, int N, int K,
+                             int format, int tiling, int max_ctas, void* stream) {
     const rdb::fp4::Product q = {A, scales_a, B, scales_b, tensor_scale_a, tensor_scale_b, D, out_type, M, N, K};
     const int ok = rdb::fp4::check(q, format);
     if (ok != RDB_SUCCESS) return ok;
+    if (tiling < 0 || tiling > 2 || max_ctas < 0) return RDB_INVALID_CONFIG;
     int err = 0;
     rdb::DeviceInfo* info = rdb::device_info(&err);
     if (!info) return err;
-    return rdb::fp4::run_split(q, format, 0, 0, 0, 0, info, static_cast<cudaStream_t>(stream));
+    auto st = static_cast<cudaStream_t>(stream);
+    const long long tiles = static_cast<long long>((M + 255ll) / 256) * ((N + 255ll) / 256);
+    if (tiles > (1ll << 30)) return RDB_SIZE_ABOVE_LIMIT;
+    if (tiling == 0) tiling = tiles >= 32 || M > 2048 ? 2 : 1;
+    if (tiling == 2)
+        return format == RDB_FP4_NVFP4 ? rdb::fp4::launch_pair<RDB_FP4_NVFP4>(q, max_ctas, info, st)
+                                       : rdb::fp4::launch_pair<RDB_FP4_MXFP4>(q, max_ctas, info, st);
+    return rdb::fp4::run_split(q, format, 0, 0, 0, 0, info, st);
+}
+
+int rdb_dense_gemm_fp4(const uint8_t* A, const uint8_t* scales_a, const float* tensor_scale_a, const uint8_t* B, const uint8_t* scales_b,
+                       const float* tensor_scale_b, void* D, int out_type, int M, int N, int K, int format, void* stream) {
+    return rdb_dense_gemm_fp4_tuned(A, scales_a, tensor_scale_a, B, scales_b, tensor_scale_b, D, out_type, M, N, K, format, 0, 0, stream);
 }
 
 }  // extern "C"

@@ -57,6 +57,47 @@ __device__ __forceinline__ void bulk_load_scales(uint32_t dst_smem, const void* 
                  ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
 }
 
+// 32 consecutive outputs of row m from column n on; vec: 16-byte stores are aligned.
+__device__ __forceinline__ void store32(void* D, int type, size_t N, int m, int n, const float* v, float alpha, bool vec) {
+    const size_t at = static_cast<size_t>(m) * N + n;
+    const bool whole = vec && n + 32 <= N;
+    if (type == RDB_TYPE_FP32) {
+        float* p = reinterpret_cast<float*>(D) + at;
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j] * alpha, v[j + 1] * alpha, v[j + 2] * alpha, v[j + 3] * alpha);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+                if (n + j < N) p[j] = v[j] * alpha;
+        }
+        return;
+    }
+    uint16_t* p = reinterpret_cast<uint16_t*>(D) + at;
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = v[j + 2 * i] * alpha, y = v[j + 2 * i + 1] * alpha;
+            if (type == RDB_TYPE_BF16) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(x, y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        if (whole) {
+            *reinterpret_cast<uint4*>(p + j) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (n + j + i < N) p[j + i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+        }
+    }
+}
+
 // Four consecutive outputs of row m at column n, rounded once; vec: 4 outputs can be stored at once.
 __device__ __forceinline__ void store4(void* D, int type, size_t N, int m, int n, const float* v, bool vec) {
     const size_t at = static_cast<size_t>(m) * N + n;

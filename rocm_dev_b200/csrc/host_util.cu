@@ -87,6 +87,19 @@ int make_tmap_kchunks(CUtensorMap* out, const void* base, uint64_t rows, uint64_
     return r == CUDA_SUCCESS ? RDB_SUCCESS : RDB_CUDA_ERROR;
 }
 
+int make_tmap_bytes256(CUtensorMap* out, const void* base, uint64_t rows, uint64_t planes, uint32_t box_rows, uint32_t box_planes) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return RDB_CUDA_ERROR;
+    cuuint64_t dims[3] = {256, rows, planes};
+    cuuint64_t strides[2] = {256, rows * 256};
+    cuuint32_t box[3] = {256, box_rows, box_planes};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? RDB_SUCCESS : RDB_CUDA_ERROR;
+}
+
 }  // namespace rdb
 
 extern "C" {

@@ -34,6 +34,10 @@ DeviceInfo* device_info(int* err);
 int make_tmap_kchunks(CUtensorMap* out, const void* base, uint64_t rows, uint64_t k_bytes, uint64_t pitch_bytes,
                       uint32_t box_rows, uint32_t box_chunks);
 
+// Byte array [planes][rows of 256 bytes] (scale tiles of a microscaled tensor: one plane per 128 rows), a box of box_rows
+// x box_planes; planes past the end read as zeros.
+int make_tmap_bytes256(CUtensorMap* out, const void* base, uint64_t rows, uint64_t planes, uint32_t box_rows, uint32_t box_planes);
+
 int make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t rows,
                  uint64_t cols, uint64_t pitch_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle,
                  CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);

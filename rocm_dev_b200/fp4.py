@@ -164,12 +164,13 @@ def _product(A: Fp4Tensor, B: Fp4Tensor, out, out_dtype):
 
 
 def dense_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
-                   out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+                   out_dtype: torch.dtype = torch.bfloat16, tiling: int = 0, max_ctas: int = 0) -> torch.Tensor:
     """D[M,N] = A . B^T over the values of A [M,K] and B [N,K], any sizes; fp32 accumulation, rounded once to
-    ``out_dtype`` (``out``'s type where it is given)."""
+    ``out_dtype`` (``out``'s type where it is given).  ``tiling``, ``max_ctas``: the tuner's knobs, 0 = automatic."""
     args, out, dev = _product(A, B, out, out_dtype)
     with _on(dev):
-        check(lib().rdb_dense_gemm_fp4(*args, torch.cuda.current_stream(dev).cuda_stream), "rdb_dense_gemm_fp4")
+        check(lib().rdb_dense_gemm_fp4_tuned(*args, tiling, max_ctas, torch.cuda.current_stream(dev).cuda_stream),
+              "rdb_dense_gemm_fp4")
     return out
 
 

@@ -171,6 +171,8 @@ def test_refusals_before_anything_is_launched():
         assert call(fmt=0) == 6                                     # mxfp4 has no tensor scales
         assert call(A=p + 8) == 7 and call(sb=p + 1) == 7 and call(D=p + 1) == 7 and call(typ=2, D=p + 2) == 7
     assert skinny(M=33) == 1 and skinny(flags=2) == 6
+    tiled = lambda **k: L.rdb_dense_gemm_fp4_tuned(*{**base, **dict(tiling=0, ctas=0), **k}.values(), None)  # noqa: E731
+    assert tiled(tiling=3) == 6 and tiled(tiling=-1) == 6 and tiled(ctas=-1) == 6 and tiled(M=0) == 8
     tuned = lambda **k: L.rdb_skinny_gemm_fp4_tuned(*{**base, **dict(cols=0, split=0, st=0, flags=0), **k}.values(), None)  # noqa: E731
     assert tuned(cols=32) == 6 and tuned(cols=320) == 6 and tuned(split=9) == 6 and tuned(st=-1) == 6 and tuned(M=40) == 1
 
@@ -352,6 +354,21 @@ def test_every_tile_width_and_split(cuda_device, form, columns, split, stages):
         torch.cuda.synchronize()
         assert R.lib().rdb_device_status() == 0
         check_product(out, A, B)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("tiling,max_ctas", [(1, 0), (2, 0), (2, 2)])
+@pytest.mark.parametrize("M,N,K,dtype", [(256, 256, 256, torch.float32), (256, 256, 2048, torch.bfloat16), (300, 700, 1100, torch.float32),
+                                         (1, 1030, 64, torch.float16), (700, 513, 3000, torch.bfloat16), (1300, 1025, 520, torch.float32)])
+def test_both_tilings(cuda_device, form, tiling, max_ctas, M, N, K, dtype):
+    """max_ctas = 2: one pair walks every tile, through both accumulators."""
+    import rocm_dev_b200 as R
+    A, B = held(draw(M, K, 1, std=0.1), form, cuda_device), held(draw(N, K, 2, std=0.02), form, cuda_device)
+    got = R.dense_gemm_fp4(A, B, out_dtype=dtype, tiling=tiling, max_ctas=max_ctas)
+    torch.cuda.synchronize()
+    assert R.lib().rdb_device_status() == 0
+    check_product(got, A, B)
 
 
 @pytest.mark.gpu
