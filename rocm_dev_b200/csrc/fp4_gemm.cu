@@ -122,31 +122,35 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0) {
-            const int slot_cols = TILES * 4 * (1 + p.b_tiles);
-            const int shift = (n0 & 127) / 32;               // a tile that starts inside a 128-row scale tile
-            for (int i = 0; i < nkb; i++) {
-                const int s = i % nstages;
-                if (!mbar_wait(full0 + 8 * s, (i / nstages) & 1)) { *abort_flag = 1; report_timeout(p.status); break; }
-                tc_fence_after_sync();
-                const uint32_t a = stage0 + s * STAGE, b = a + A_BYTES, sc = b + B_BYTES;
-                const uint32_t tsa = tmem_base + R + s * slot_cols, tsb = tsa + 4 * TILES;
-#pragma unroll
-                for (int t = 0; t < TILES; t++) {
-                    tmem_cp_scales<false>(tsa + 4 * t, sc + t * TILE_BYTES);
-                    for (int j = 0; j < p.b_tiles; j++)
-                        tmem_cp_scales<false>(tsb + 4 * (t * p.b_tiles + j), sc + SCALES * (1 + j) + t * TILE_BYTES);
-                }
-#pragma unroll
-                for (int ks = 0; ks < 4; ks++) {
-                    const int t = ks * TILES / 4, id = TILES == 4 ? 0 : 2 * (ks & 1);
-                    tc_mma_fp4<FMT, false>(tmem_base, smem_desc_k128(a + ks * 32), smem_desc_k128(b + ks * 32), idesc_fp4<FMT>(128, R, id),
-                                           tsa + 4 * t, tsb + 4 * t * p.b_tiles + shift, (i | ks) != 0);
-                }
-                tc_commit(empty0 + 8 * s);
+        // all lanes; see fp4_mma.cuh
+        const uint32_t leader = elect_one();
+        const int slot_cols = TILES * 4 * (1 + p.b_tiles);
+        const int shift = (n0 & 127) / 32;               // a tile that starts inside a 128-row scale tile
+        const uint32_t idesc0 = idesc_fp4<FMT>(128, R, 0), idesc2 = idesc_fp4<FMT>(128, R, 2);
+        for (int i = 0; i < nkb; i++) {
+            const int s = i % nstages;
+            if (!mbar_wait(full0 + 8 * s, (i / nstages) & 1)) {
+                if (leader) { *abort_flag = 1; report_timeout(p.status); }
+                break;
             }
-            tc_commit(done);                                 // also after an abort
+            tc_fence_after_sync();
+            const uint32_t a = desc_lo_operand(stage0 + s * STAGE), b = a + (A_BYTES >> 4), sc = desc_lo_scales(stage0 + s * STAGE + A_BYTES + B_BYTES);
+            const uint32_t tsa = tmem_base + R + s * slot_cols, tsb = tsa + 4 * TILES;
+#pragma unroll
+            for (int t = 0; t < TILES; t++) {
+                tmem_cp_scales<false>(leader, tsa + 4 * t, sc + t * (TILE_BYTES >> 4));
+                tmem_cp_scales<false>(leader, tsb + 4 * t * p.b_tiles, sc + ((SCALES + t * TILE_BYTES) >> 4));
+                if (p.b_tiles > 1) tmem_cp_scales<false>(leader, tsb + 4 * (t * p.b_tiles + 1), sc + ((2 * SCALES + t * TILE_BYTES) >> 4));
+            }
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++) {
+                const int t = ks * TILES / 4;
+                tc_mma_fp4<FMT, false>(leader, tmem_base, a + ks * 2, b + ks * 2, TILES == 2 && (ks & 1) ? idesc2 : idesc0, tsa + 4 * t,
+                                       tsb + 4 * t * p.b_tiles + shift, (i | ks) != 0);
+            }
+            commit(leader, empty0 + 8 * s);
         }
+        commit(leader, done);                                // also after an abort
         __syncwarp();
     } else if (warp == 2) {
         if (lane == 0) {
@@ -339,7 +343,9 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {                        // all lanes; see fp4_mma.cuh
+            const uint32_t leader = elect_one();
+            const uint32_t op0 = desc_lo_operand(stage0), sc0 = desc_lo_scales(stage0 + 2 * HALF);
             int it = 0, t = 0;
             bool ok = true;
             for (int tile = pair_id; tile < num_tiles && ok && *abort_flag == 0; tile += num_pairs, t++) {
@@ -353,13 +359,13 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                     }
                     if (!mbar_wait(full0 + 8 * s, (it / STAGES) & 1)) { ok = false; break; }
                     tc_fence_after_sync();
-                    const uint32_t a = stage0 + s * STAGE, b = a + HALF, sc = b + HALF;
+                    const uint32_t a = op0 + s * (STAGE >> 4), b = a + (HALF >> 4), sc = sc0 + s * (STAGE >> 4);
                     const uint32_t tsa = tmem_base + pairs::SCALE_COL + (it % C::SLOTS) * C::SLOT, tsb = tsa + 4 * TILES;
 #pragma unroll
                     for (int i = 0; i < TILES; i++) {
-                        tmem_cp_scales<true>(tsa + 4 * i, sc + i * TILE_BYTES);
-                        tmem_cp_scales<true>(tsb + 8 * i, sc + SCALES + i * TILE_BYTES);
-                        tmem_cp_scales<true>(tsb + 8 * i + 4, sc + 2 * SCALES + i * TILE_BYTES);
+                        tmem_cp_scales<true>(leader, tsa + 4 * i, sc + i * (TILE_BYTES >> 4));
+                        tmem_cp_scales<true>(leader, tsb + 8 * i, sc + ((SCALES + i * TILE_BYTES) >> 4));
+                        tmem_cp_scales<true>(leader, tsb + 8 * i + 4, sc + ((2 * SCALES + i * TILE_BYTES) >> 4));
                     }
                     if (kb == 0 && t > 0) {
                         if (!mbar_wait_cluster(acc_free, (t - 1) & 1)) { ok = false; break; }
@@ -368,14 +374,13 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                     for (int ks = 0; ks < 4; ks++) {
                         const int i = ks * TILES / 4, id = TILES == 4 ? 0 : 2 * (ks & 1);
-                        tc_mma_fp4<FMT, true>(d, smem_desc_k128(a + ks * 32), smem_desc_k128(b + ks * 32), idesc_fp4<FMT>(256, 256, id),
-                                              tsa + 4 * i, tsb + 8 * i, (kb | ks) != 0);
+                        tc_mma_fp4<FMT, true>(leader, d, a + ks * 2, b + ks * 2, idesc_fp4<FMT>(256, 256, id), tsa + 4 * i, tsb + 8 * i, (kb | ks) != 0);
                     }
-                    tc_commit_pair_both(empty0 + 8 * s);
-                    if (kb == p.num_kb - 1) tc_commit_pair_both(acc_full);
+                    commit_both(leader, empty0 + 8 * s);
+                    if (kb == p.num_kb - 1) commit_both(leader, acc_full);
                 }
             }
-            if (!ok) { *abort_flag = 1; report_timeout(p.status); }
+            if (!ok && leader) { *abort_flag = 1; report_timeout(p.status); }
         }
         __syncwarp();
     } else {

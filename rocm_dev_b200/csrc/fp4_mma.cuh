@@ -16,31 +16,47 @@ __host__ __device__ constexpr uint32_t idesc_fp4(int umma_m, int umma_n, int sca
            (static_cast<uint32_t>(umma_m >> 4) << 24) | (static_cast<uint32_t>(scale_id) << 4) | (static_cast<uint32_t>(scale_id) << 29);
 }
 
-// Shared-memory descriptor of a scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups 128 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t addr) {
-    return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
-}
+// The issuing warp runs its loop with all lanes, so that addresses and descriptors stay in uniform registers, and only the
+// tcgen05 instructions themselves are predicated by `leader` (one elected lane): a loop inside `if (lane == 0)` has to
+// move every operand from the vector registers first, and that was what a stage's issue time went into.
+
+// Descriptors as their low word; the high one is a constant of the layout.
+// Operand: 128-byte rows, SWIZZLE_128B, 8-row groups 1024 bytes apart.  Scale tile: 32 rows of 16 bytes, no swizzle, 8-row
+// groups 128 bytes apart.
+constexpr uint32_t DESC_HI_OPERAND = (1024u >> 4) | (1u << 14) | (2u << 29), DESC_HI_SCALES = (128u >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t desc_lo_operand(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_lo_scales(uint32_t smem_addr) { return (smem_addr & 0x3FFFFu) >> 4; }
 
 // 512 bytes -> four TMEM columns, the 32 rows repeated in each of the four lane quadrants.  Ordered before later MMAs of
 // the issuing thread.
 template <bool PAIR>
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t smem_addr) {
-    if constexpr (PAIR)
-        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc_scales(smem_addr)) : "memory");
-    else
-        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc_scales(smem_addr)) : "memory");
+__device__ __forceinline__ void tmem_cp_scales(uint32_t leader, uint32_t taddr, uint32_t desc_lo) {
+#define RDB_CP_SCALES(GROUP)                                                                            \
+    asm volatile(                                                                                       \
+        "{\n\t.reg .pred q;\n\t.reg .b64 d;\n\t"                                                       \
+        "setp.ne.b32 q, %0, 0;\n\t"                                                                     \
+        "mov.b64 d, {%2, %3};\n\t"                                                                      \
+        "@q tcgen05.cp.cta_group::" GROUP ".32x128b.warpx4 [%1], d;\n\t}"                                \
+        ::"r"(leader), "r"(taddr), "r"(desc_lo), "r"(DESC_HI_SCALES) : "memory")
+    if constexpr (PAIR) RDB_CP_SCALES("2");
+    else RDB_CP_SCALES("1");
+#undef RDB_CP_SCALES
 }
 
 // D[tmem] (+)= A[smem] * B[smem]^T with block scales from TMEM, one step of 64 elements of K.
 template <int FMT, bool PAIR>
-__device__ __forceinline__ void tc_mma_fp4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t scale_a,
-                                           uint32_t scale_b, bool accumulate) {
+__device__ __forceinline__ void tc_mma_fp4(uint32_t leader, uint32_t tmem_d, uint32_t desc_a, uint32_t desc_b, uint32_t idesc,
+                                           uint32_t scale_a, uint32_t scale_b, bool accumulate) {
 #define RDB_MMA_FP4(GROUP, KIND)                                                                        \
     asm volatile(                                                                                       \
-        "{\n\t.reg .pred p;\n\t"                                                                        \
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"                                                 \
         "setp.ne.b32 p, %6, 0;\n\t"                                                                     \
-        "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}"         \
-        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(static_cast<uint32_t>(accumulate)) : "memory")
+        "setp.ne.b32 q, %8, 0;\n\t"                                                                     \
+        "mov.b64 a, {%1, %7};\n\t"                                                                      \
+        "mov.b64 b, {%2, %7};\n\t"                                                                      \
+        "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], a, b, %3, [%4], [%5], p;\n\t}"         \
+        ::"r"(tmem_d), "r"(desc_a), "r"(desc_b), "r"(idesc), "r"(scale_a), "r"(scale_b),                \
+          "r"(static_cast<uint32_t>(accumulate)), "r"(DESC_HI_OPERAND), "r"(leader) : "memory")
     if constexpr (FMT == RDB_FP4_NVFP4) {
         if constexpr (PAIR) RDB_MMA_FP4("2", "mxf4nvf4.block_scale.scale_vec::4X");
         else RDB_MMA_FP4("1", "mxf4nvf4.block_scale.scale_vec::4X");
@@ -49,6 +65,20 @@ __device__ __forceinline__ void tc_mma_fp4(uint32_t tmem_d, uint64_t desc_a, uin
         else RDB_MMA_FP4("1", "mxf4.block_scale.scale_vec::2X");
     }
 #undef RDB_MMA_FP4
+}
+
+// Arrive on an mbarrier (in both CTAs of a pair, at the same offset) when everything the leader issued has finished.
+__device__ __forceinline__ void commit(uint32_t leader, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}"
+        ::"r"(leader), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit_both(uint32_t leader, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%1], %2;\n\t}"
+        ::"r"(leader), "r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 
 // A stage of scale tiles is contiguous in memory: one untiled copy.
