@@ -237,13 +237,15 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
 namespace pairs {
 constexpr int THREADS = 224;                    // warp 0: A loads, 1: MMA, 2-5: epilogue, 6: B loads
 constexpr int ACC1 = 160, SCALE_COL = ACC1 + 256, GROUP_M = 16;
+constexpr int OUT_BYTES = 32 * 128;             // 32 rows of 128 bytes: what one output copy stores
 template <int FMT>
 struct Cfg {
     static constexpr int SCALES = Format<FMT>::TILES * TILE_BYTES;
     static constexpr int STAGE = 2 * 128 * 128 + 3 * SCALES;
-    static constexpr int STAGES = FMT == RDB_FP4_NVFP4 ? 5 : 6;
+    static constexpr int STAGES = 5;
     static constexpr int SLOT = Format<FMT>::TILES * 12, SLOTS = (512 - SCALE_COL) / SLOT;      // 2 or 4
-    static constexpr int SMEM = 1024 + STAGES * STAGE;
+    static constexpr int OUT = 4 * 2 * OUT_BYTES;                            // two output buffers per epilogue warp
+    static constexpr int SMEM = 1024 + STAGES * STAGE + OUT;
 };
 }  // namespace pairs
 
@@ -252,7 +254,7 @@ struct PairParams {
     const float *ta, *tb;
     int* status;
     int M, N, num_kb, tiles_m, tiles_n;
-    int out_type, vec;
+    int out_type, tma_out;      // tma_out: rows of D start on 16-byte boundaries
 };
 
 __device__ __forceinline__ void tile_coords(int tile, int tiles_m, int tiles_n, int& mb, int& nb) {
@@ -267,7 +269,7 @@ __device__ __forceinline__ void tile_coords(int tile, int tiles_m, int tiles_n, 
 template <int FMT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pairs::THREADS, 1)
 pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSA,
-            const __grid_constant__ CUtensorMap tmSB, const PairParams p) {
+            const __grid_constant__ CUtensorMap tmSB, const __grid_constant__ CUtensorMap tmD, const PairParams p) {
     using C = pairs::Cfg<FMT>;
     constexpr int STAGES = C::STAGES, STAGE = C::STAGE, SCALES = C::SCALES, TILES = Format<FMT>::TILES, HALF = 128 * 128;
     extern __shared__ uint8_t smem_raw[];
@@ -387,6 +389,41 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         const int quad = warp & 3;
         const float alpha = p.ta ? __ldg(p.ta) * __ldg(p.tb) : 1.0f;
         const uint32_t free_even = mapa_smem(acc_free, 0);
+        uint8_t* out = smem + STAGES * STAGE + quad * 2 * pairs::OUT_BYTES;
+        int turn = 0;
+        // 32 columns of this warp's 32 rows: into shared memory in the layout of the copy's swizzle (128 or 64 bytes a
+        // row, no bank conflicts), then one copy out.  A thread holds a row: its own stores would touch 32 lines each.
+        auto put = [&](int m0, int n, const float* v) {
+            if (m0 >= p.M || n >= p.N) return;
+            if (!p.tma_out) {
+                if (m0 + lane < p.M) store32(p.D, p.out_type, p.N, m0 + lane, n, v, alpha);
+                return;
+            }
+            uint8_t* buf = out + (turn & 1) * pairs::OUT_BYTES;
+            tma_store_wait_read<1>();                    // lane 0: the copy that last read this buffer is done with it
+            __syncwarp();
+            if (p.out_type == RDB_TYPE_FP32) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                        make_float4(v[4 * j] * alpha, v[4 * j + 1] * alpha, v[4 * j + 2] * alpha, v[4 * j + 3] * alpha);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) w[i] = pack2(p.out_type, v[8 * j + 2 * i] * alpha, v[8 * j + 2 * i + 1] * alpha);
+                    *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(&tmD, smem_u32(buf), n, m0);
+                tma_store_commit();
+            }
+            turn++;
+        };
         int t = 0;
         for (int tile = pair_id; tile < num_tiles; tile += num_pairs, t++) {
             int mb, nb;
@@ -394,22 +431,27 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             if (!mbar_wait(acc_full, t & 1)) { *abort_flag = 1; report_timeout(p.status); }
             if (*abort_flag != 0) break;
             tc_fence_after_sync();
-            const int row = mb * 256 + static_cast<int>(rank) * 128 + quad * 32 + lane;
+            const int row0 = mb * 256 + static_cast<int>(rank) * 128 + quad * 32;
             const uint32_t taddr = tmem_base + (t & 1) * pairs::ACC1 + (static_cast<uint32_t>(quad * 32) << 16);
             // columns shared with the other accumulator first: the last 96 of the first, the first 96 of the second
+            float v[96];
+            const int c0 = (t & 1) ? 0 : pairs::ACC1;
+            tmem_ld64(taddr + c0, v);
+            tmem_ld32(taddr + c0 + 64, v + 64);
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(free_even);
+            const int n0 = nb * 256;
+#pragma unroll
+            for (int i = 0; i < 3; i++) put(row0, n0 + c0 + 32 * i, v + 32 * i);
+            const int c1 = (t & 1) ? 96 : 0;
 #pragma unroll 1
-            for (int i = 0; i < 8; i++) {
-                const int c0 = (t & 1) ? 32 * i : (i < 3 ? pairs::ACC1 + 32 * i : 32 * (i - 3));
-                float v[32];
-                tmem_ld32(taddr + c0, v);
-                if (i == 2) {
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(free_even);
-                }
-                if (row < p.M && nb * 256 + c0 < p.N) store32(p.D, p.out_type, p.N, row, nb * 256 + c0, v, alpha, p.vec);
+            for (int i = 0; i < 5; i++) {
+                tmem_ld32(taddr + c1 + 32 * i, v);
+                put(row0, n0 + c1 + 32 * i, v);
             }
         }
+        tma_store_wait<0>();
     }
 
     if (*abort_flag != 0) {
@@ -552,13 +594,17 @@ static int launch_pair(const Product& q, int max_ctas, const DeviceInfo* info, c
     p.tiles_m = (q.M + 255) / 256;
     p.tiles_n = (q.N + 255) / 256;
     p.out_type = q.out_type;
-    p.vec = q.N % (q.out_type == RDB_TYPE_FP32 ? 4 : 8) == 0 && aligned16(q.D);
-    CUtensorMap tmA, tmB, tmSA, tmSB;
+    const int out_size = q.out_type == RDB_TYPE_FP32 ? 4 : 2;
+    p.tma_out = q.N * static_cast<size_t>(out_size) % 16 == 0 && aligned16(q.D);
+    CUtensorMap tmA, tmB, tmSA, tmSB, tmD = {};
     const uint64_t pitch = row_bytes(q.K), scale_rows = static_cast<uint64_t>(p.num_kb) * C::SCALES / 256;
     int r = make_tmap_2d(&tmA, q.A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.M, pitch, pitch, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r == RDB_SUCCESS) r = make_tmap_2d(&tmB, q.B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.N, pitch, pitch, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r == RDB_SUCCESS) r = make_tmap_bytes256(&tmSA, q.sa, scale_rows, (q.M + 127) / 128, C::SCALES / 256, 1);
     if (r == RDB_SUCCESS) r = make_tmap_bytes256(&tmSB, q.sb, scale_rows, (q.N + 127) / 128, C::SCALES / 256, 2);
+    if (r == RDB_SUCCESS && p.tma_out)
+        r = make_tmap_2d(&tmD, q.D, q.out_type == RDB_TYPE_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, out_size, q.M, q.N,
+                         static_cast<uint64_t>(q.N) * out_size, 32, 32, out_size == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     if (r != RDB_SUCCESS) return r;
     int num_pairs = p.tiles_m * p.tiles_n, cap = info->sm_count / 2;
     if (max_ctas > 0 && max_ctas / 2 < cap) cap = max_ctas / 2 > 0 ? max_ctas / 2 : 1;
@@ -573,7 +619,7 @@ static int launch_pair(const Product& q, int max_ctas, const DeviceInfo* info, c
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, pair_kernel<FMT>, tmA, tmB, tmSA, tmSB, p) != cudaSuccess) { cudaGetLastError(); return RDB_CUDA_ERROR; }
+    if (cudaLaunchKernelEx(&cfg, pair_kernel<FMT>, tmA, tmB, tmSA, tmSB, tmD, p) != cudaSuccess) { cudaGetLastError(); return RDB_CUDA_ERROR; }
     return RDB_SUCCESS;
 }
 

@@ -87,43 +87,30 @@ __device__ __forceinline__ void bulk_load_scales(uint32_t dst_smem, const void* 
                  ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
 }
 
-// 32 consecutive outputs of row m from column n on; vec: 16-byte stores are aligned.
-__device__ __forceinline__ void store32(void* D, int type, size_t N, int m, int n, const float* v, float alpha, bool vec) {
+__device__ __forceinline__ uint32_t pack2(int type, float x, float y) {
+    if (type == RDB_TYPE_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 32 consecutive outputs of row m from column n on, element by element.
+__device__ __forceinline__ void store32(void* D, int type, size_t N, int m, int n, const float* v, float alpha) {
     const size_t at = static_cast<size_t>(m) * N + n;
-    const bool whole = vec && n + 32 <= N;
     if (type == RDB_TYPE_FP32) {
         float* p = reinterpret_cast<float*>(D) + at;
-        if (whole) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(p + j) = make_float4(v[j] * alpha, v[j + 1] * alpha, v[j + 2] * alpha, v[j + 3] * alpha);
-        } else {
+        for (int j = 0; j < 32; j++)
+            if (n + j < N) p[j] = v[j] * alpha;
+    } else {
+        uint16_t* p = reinterpret_cast<uint16_t*>(D) + at;
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-                if (n + j < N) p[j] = v[j] * alpha;
-        }
-        return;
-    }
-    uint16_t* p = reinterpret_cast<uint16_t*>(D) + at;
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float x = v[j + 2 * i] * alpha, y = v[j + 2 * i + 1] * alpha;
-            if (type == RDB_TYPE_BF16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-                const __half2 h = __floats2half2_rn(x, y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-        }
-        if (whole) {
-            *reinterpret_cast<uint4*>(p + j) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (n + j + i < N) p[j + i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+        for (int j = 0; j < 32; j += 2) {
+            const uint32_t w = pack2(type, v[j] * alpha, v[j + 1] * alpha);
+            if (n + j < N) p[j] = static_cast<uint16_t>(w);
+            if (n + j + 1 < N) p[j + 1] = static_cast<uint16_t>(w >> 16);
         }
     }
 }
@@ -140,17 +127,7 @@ __device__ __forceinline__ void store4(void* D, int type, size_t N, int m, int n
                 if (n + j < N) p[j] = v[j];
         return;
     }
-    uint32_t w[2];
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        if (type == RDB_TYPE_BF16) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
-            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-    }
+    const uint32_t w[2] = {pack2(type, v[0], v[1]), pack2(type, v[2], v[3])};
     uint16_t* p = reinterpret_cast<uint16_t*>(D) + at;
     if (vec && n + 4 <= N) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else
