@@ -240,7 +240,7 @@ int rdb_dense_gemm_fp8_f32(const uint8_t *A, const uint8_t *B, float *D, int M, 
  *           zero codes behind K;
  *   scales  rdb_fp4_scale_bytes(format, rows, K) bytes in tiles of 128 rows x 4 blocks (512 bytes): row r, block b of a
  *           tile at (r % 32) * 16 + (r / 32) * 4 + b; tiles run along K first, K filled up to a multiple of 256 with
- *           zero bytes (the products read them); bytes of rows past the last are neither written nor used;
+ *           zero bytes (the products read them); bytes of rows past the last are of no meaning;
  *   tensor_scale  one fp32 on the device (RDB_FP4_NVFP4 only, else NULL).
  * codes and scales must be 16-byte aligned. */
 typedef enum rdb_fp4_format { RDB_FP4_MXFP4 = 0, RDB_FP4_NVFP4 = 1 } rdb_fp4_format;
@@ -250,8 +250,8 @@ size_t rdb_fp4_row_bytes(int K);
 size_t rdb_fp4_scale_bytes(int format, int rows, int K);     /* 0 for an unsupported argument */
 
 /* Quantises x [rows, K] (row pitch ldx elements, x_type one of rdb_type), with blocks along the rows into codes / scales
- * and - or, where `codes` is NULL - with blocks along the columns into codes_t / scales_t, the held form of the
- * TRANSPOSED tensor [K, rows] (what the gradients' products read).  Both directions share the tensor scale, which is
+ * and, where codes_t is not NULL, with blocks along the columns into codes_t / scales_t, the held form of the TRANSPOSED
+ * tensor [K, rows] (what the gradients' products read); x is read once for both.  Both directions share the tensor scale, which is
  * written to tensor_scale[0], or read from it where scale_given is non-zero.  workspace: RDB_FP4_WORKSPACE_FLOATS floats
  * of scratch for an RDB_FP4_NVFP4 call that computes its scale (else may be NULL); nothing in it outlives the call. */
 int rdb_quantize_fp4(const void *x, int x_type, long long ldx, int rows, int K, int format, float *tensor_scale,

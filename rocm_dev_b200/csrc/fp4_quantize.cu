@@ -13,7 +13,6 @@
 #include <type_traits>
 
 #include "fp4.cuh"
-#include "fp8_codec.cuh"
 #include "host_util.h"
 #include "ptx.cuh"
 
@@ -38,7 +37,7 @@ __device__ __forceinline__ void ldg32(const void* p, uint32_t* w) {
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
 }
 
-// The words of a vector load as floats.
+// Words of memory as floats.
 template <class T, int N>
 __device__ __forceinline__ void unpack(const uint32_t* w, float* v) {
     if constexpr (sizeof(T) == 4) {
@@ -60,27 +59,38 @@ __device__ __forceinline__ void unpack(const uint32_t* w, float* v) {
     }
 }
 
-// N elements from p, of which the first `valid` exist; the others read as zero.
+// Largest magnitude of N elements held in words, as fp32 bits: non-negative floats order like integers, infinities and
+// NaNs above every number.  16-bit types are compared two at a time.
 template <class T, int N>
-__device__ __forceinline__ void load_block(const T* p, int valid, bool vec, float* v) {
-    if (vec && valid >= N) {
-        constexpr int WORDS = N * sizeof(T) / 4;
-        uint32_t w[WORDS];
+__device__ __forceinline__ uint32_t magnitude(const uint32_t* w) {
+    uint32_t m = 0;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < WORDS; i += 8) ldg32(reinterpret_cast<const uint32_t*>(p) + i, w + i);
-        unpack<T, N>(w, v);
+        for (int i = 0; i < N; i++) m = max(m, w[i] & 0x7FFFFFFFu);
+        return m;
     } else {
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = i < valid ? to_f32(p[i]) : 0.0f;
+        for (int i = 0; i < N / 2; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        m = max(m & 0xFFFFu, m >> 16);
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) return m << 16;
+        else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
     }
 }
 
-// Largest magnitude as fp32 bits: non-negative floats order like integers, infinities and NaNs above every number.
-template <int N>
-__device__ __forceinline__ uint32_t magnitude(const float* v) {
-    uint32_t m = 0;
+// The same over the finite elements alone.
+template <class T, int N>
+__device__ __forceinline__ uint32_t finite_magnitude(const uint32_t* w) {
+    uint32_t m = magnitude<T, N>(w);
+    if (m >= kInf) {
+        float v[N];
+        unpack<T, N>(w, v);
+        m = 0;
 #pragma unroll
-    for (int i = 0; i < N; i++) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        for (int i = 0; i < N; i++) {
+            const uint32_t a = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+            if (a < kInf) m = max(m, a);
+        }
+    }
     return m;
 }
 
@@ -97,23 +107,30 @@ __device__ __forceinline__ uint32_t pack8(const float* q) {
     return r;
 }
 
-// x / s rounded to fp32 like the IEEE division, for a divisor shared by a block (BlockDivisor's correction step).  bf16
-// numerators need one step; wider ones a second, whose starting point is within one unit of the quotient's last place -
-// the first product can miss by one and a half.
-template <class T>
-__device__ __forceinline__ void divide8(const ar::BlockDivisor& d, const float* x, float* q) {
-    d.div8(x, q);
-    if constexpr (!std::is_same_v<T, __nv_bfloat16>) {
-        if (d.fast) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) q[i] = copysignf(__fmaf_rn(__fmaf_rn(-q[i], d.s, x[i]), d.inv, q[i]), x[i]);
-        }
+// a / d rounded to fp32 like the IEEE division, for a divisor shared by many numerators: with inv = RN(1 / d) and q within a
+// unit of the last place of a / d, RN(q + inv * (a - q d)) is the rounded quotient (Markstein).  The first product can
+// miss by one and a half units; the step repairs that for all but quotients within 2^-22 units of a rounding border, and a
+// second step for those too (numerators of 16 bits do not come that near: they get one).  Divisors far from 1 are moved
+// by 2^64 together with the numerator, which is exact wherever the quotient is not below e2m1's first border anyway.
+struct Divisor {
+    float d, inv, move;
+    __device__ __forceinline__ void set(float x) {
+        move = x < 8.6736174e-19f ? 18446744073709551616.0f : x > 1.1529215e18f ? 5.4210109e-20f : 1.0f;
+        d = x * move;
+        inv = __frcp_rn(d);
     }
-}
+    template <int STEPS>
+    __device__ __forceinline__ float quotient(float a) const {       // a already moved
+        float q = __fmul_rn(a, inv);
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) q = __fmaf_rn(__fmaf_rn(-q, d, a), inv, q);
+        return q;
+    }
+};
 
-// One block: v[BLOCK] -> BLOCK / 8 words of codes, returns the scale byte.  t, t6: the tensor scale and 6 t (NVFP4).
+// One block: v[BLOCK] -> BLOCK / 8 words of codes, returns the scale byte.  t: the tensor scale, t6: 6 t as a divisor.
 template <class T, int FMT>
-__device__ __forceinline__ uint32_t encode_block(const float* v, uint32_t amax, float t, float t6, uint32_t* codes) {
+__device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, float t, const Divisor& t6, uint32_t* codes) {
     constexpr int B = Format<FMT>::BLOCK;
     uint32_t byte;
     if constexpr (FMT == RDB_FP4_MXFP4) {
@@ -130,59 +147,100 @@ __device__ __forceinline__ uint32_t encode_block(const float* v, uint32_t amax, 
         }
         if (amax >= kInf) byte = 0xFF;
     } else {
-        byte = __nv_cvt_float_to_fp8(__fdiv_rn(__uint_as_float(amax), t6), __NV_SATFINITE, __NV_E4M3) & 0x7F;
-        __nv_fp8_e4m3 s8;
-        s8.__x = static_cast<__nv_fp8_storage_t>(byte);
-        ar::BlockDivisor d;
-        d.set(static_cast<float>(s8) * t);
+        const float a = fminf(__uint_as_float(amax), 3.4028235e38f) * t6.move;
+        byte = __nv_cvt_float_to_fp8(t6.quotient<2>(a), __NV_SATFINITE, __NV_E4M3);
+        if (byte != 0) {
+            __nv_fp8_e4m3 s8;
+            s8.__x = static_cast<__nv_fp8_storage_t>(byte);
+            Divisor s;
+            s.set(static_cast<float>(s8) * t);
+            if (s.move != 1.0f) {
 #pragma unroll
-        for (int g = 0; g < B / 8; g++) {
-            float q[8];
-            divide8<T>(d, v + 8 * g, q);
-            codes[g] = byte != 0 ? pack8(q) : 0;
+                for (int i = 0; i < B; i++) v[i] *= s.move;
+            }
+#pragma unroll
+            for (int g = 0; g < B / 8; g++) {
+                float q[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) q[i] = copysignf(s.quotient<sizeof(T) == 4 ? 2 : 1>(v[8 * g + i]), v[8 * g + i]);    // keeps -0
+                codes[g] = pack8(q);
+            }
+        } else {
+#pragma unroll
+            for (int g = 0; g < B / 8; g++) codes[g] = 0;
         }
         if (amax >= kInf) byte = 0x7F;
     }
     return byte;
 }
 
-// The tensor scale from the first pass's partial maxima (every warp for itself: they are in L2), or the given one.
-__device__ __forceinline__ float tensor_scale(const float* given, const uint32_t* partial, int count) {
-    if (!partial) return *given;
-    uint32_t m = 0;
-    for (int i = threadIdx.x & 31; i < count; i += 32) m = max(m, __ldcg(partial + i));
-    m = __reduce_max_sync(0xffffffffu, m);
-    constexpr float inv = 1.0f / 2688.0f;            // rounded to fp32 before it multiplies: part of the definition
-    return m == 0 ? 1.0f : fmaxf(__fmul_rn(__uint_as_float(m), inv), 1.17549435e-38f);
+// t (NVFP4: given, or from the first pass's partial maxima) and 6 t, for the whole block: every thread takes part.
+template <int FMT>
+__device__ __forceinline__ void fetch_scale(float* tscale, const uint32_t* partial, int partials, float& t, Divisor& t6) {
+    t = 1.0f;
+    if constexpr (FMT == RDB_FP4_NVFP4) {
+        if (partial) {
+            __shared__ uint32_t warp_max[kThreads / 32];
+            uint32_t m = 0;
+            for (int i = threadIdx.x; i < partials; i += kThreads) m = max(m, __ldcg(partial + i));
+            m = __reduce_max_sync(0xffffffffu, m);
+            if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kThreads / 32; w++) m = max(m, warp_max[w]);
+            constexpr float inv = 1.0f / 2688.0f;            // rounded to fp32 before it multiplies: part of the definition
+            if (m != 0) t = fmaxf(__fmul_rn(__uint_as_float(m), inv), 1.17549435e-38f);
+            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *tscale = t;
+        } else {
+            t = *tscale;
+        }
+    }
+    t6.set(t * 6.0f);
 }
 
+// First pass of a call that computes the tensor scale: one partial maximum per CTA.  A warp takes stretches of 1024
+// elements of a row: single elements up to the first 16-byte boundary and behind the last, whole vectors between them.
+constexpr int kAmaxStretch = 1024;
 template <class T>
-__global__ void __launch_bounds__(kThreads) amax_kernel(const T* __restrict__ x, long long ldx, int rows, int K, bool vec,
-                                                        uint32_t* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads) amax_kernel(const T* __restrict__ x, long long ldx, int rows, int K, uint32_t* __restrict__ partial) {
     __shared__ uint32_t warp_max[kThreads / 32];
     pdl_launch_dependents();
     pdl_wait_prior();
-    constexpr int N = 32 / sizeof(T);
-    const long long per_row = (K + N - 1) / N, chunks = per_row * rows;
+    constexpr int N = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31;
+    const int per_row = (K - 1) / kAmaxStretch + 1;
+    const long long units = static_cast<long long>(per_row) * rows;
     uint32_t m = 0;
-    for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < chunks; i += static_cast<long long>(gridDim.x) * kThreads) {
-        const long long r = i / per_row;
-        const int k = static_cast<int>(i - r * per_row) * N;
-        float v[N];
-        load_block<T, N>(x + r * ldx + k, K - k, vec, v);
-        uint32_t a = magnitude<N>(v);
-        if (a >= kInf) {                     // only then element by element: the finite ones count
-            a = 0;
+    for (long long u = blockIdx.x * static_cast<long long>(kThreads / 32) + (threadIdx.x >> 5); u < units; u += static_cast<long long>(gridDim.x) * (kThreads / 32)) {
+        const long long r = u / per_row;
+        const int k = static_cast<int>(u - r * per_row) * kAmaxStretch;
+        const int n = K - k < kAmaxStretch ? K - k : kAmaxStretch;
+        const T* p = x + r * ldx + k;
+        int head = static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+        if (head > n) head = n;
+        const int vectors = (n - head) / N, tail = head + vectors * N;
+        auto single = [&](int i) {
+            const uint32_t a = __float_as_uint(to_f32(p[i])) & 0x7FFFFFFFu;
+            if (a < kInf) m = max(m, a);
+        };
+        if (lane < head) single(lane);
+        if (tail + lane < n) single(tail + lane);
+        const uint4* q = reinterpret_cast<const uint4*>(p + head);
+        int i = lane;
+        for (; i + 96 < vectors; i += 128) {
+            uint4 w[4];
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-                if (b < kInf) a = max(a, b);
-            }
+            for (int j = 0; j < 4; j++) w[j] = __ldg(q + i + 32 * j);
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = max(m, finite_magnitude<T, N>(&w[j].x));
         }
-        m = max(m, a);
+        for (; i < vectors; i += 32) {
+            const uint4 w = __ldg(q + i);
+            m = max(m, finite_magnitude<T, N>(&w.x));
+        }
     }
     m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
+    if (lane == 0) warp_max[threadIdx.x >> 5] = m;
     __syncthreads();
     if (threadIdx.x == 0) {
 #pragma unroll
@@ -197,76 +255,226 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t* c) {
     else *reinterpret_cast<uint4*>(p) = make_uint4(c[0], c[1], c[2], c[3]);
 }
 
-// Blocks along the rows: one thread per block; the four threads of a scale word join their bytes.
-template <class T, int FMT>
-__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int rows, int K, bool vec,
-                                                                 float* tscale, const uint32_t* partial, int partials,
-                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    constexpr int B = Format<FMT>::BLOCK;
+// Blocks along the rows, x on 16-byte boundaries and K a multiple of the block: a thread holds a whole block, so nothing
+// but the scale bytes passes between threads.  A warp takes 32 blocks of the rows r, r + 32, r + 64, r + 96 of a 128-row
+// tile: four loads in flight, and the four scale words of a lane quartet are 16 consecutive bytes of the scale tile.
+// ALIGN: 32 or 16 bytes.
+template <class T, int FMT, int ALIGN>
+__global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int rows, int K, float* tscale,
+                                                                 const uint32_t* partial, int partials, uint8_t* __restrict__ codes,
+                                                                 uint8_t* __restrict__ scales) {
+    constexpr int B = Format<FMT>::BLOCK, WORDS = B * sizeof(T) / 4, HELD = WORDS > 16 ? 2 : 4;
     pdl_launch_dependents();
     pdl_wait_prior();
-    float t = 1.0f, t6 = 6.0f;
-    if constexpr (FMT == RDB_FP4_NVFP4) {
-        t = tensor_scale(tscale, partial, partials);
-        t6 = t * 6.0f;
-        if (partial && blockIdx.x == 0 && threadIdx.x == 0) *tscale = t;
-    }
+    float t;
+    Divisor t6;
+    fetch_scale<FMT>(tscale, partial, partials, t, t6);
     const size_t pitch = row_bytes(K);
-    const int tiles = scale_tiles_per_row(FMT, K), per_row = 4 * tiles;     // a multiple of 8: words never straddle rows
-    const long long total = static_cast<long long>(rows) * per_row;
-    for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i - (threadIdx.x & 31) < total;
-         i += static_cast<long long>(gridDim.x) * kThreads) {
-        uint32_t byte = 0;
-        const long long r = i / per_row;
-        const int b = static_cast<int>(i - r * per_row);
-        if (i < total && static_cast<size_t>(b) * (B / 2) < pitch) {
-            float v[B];
-            const int k = b * B;
-            load_block<T, B>(x + r * ldx + k, K - k, vec, v);
-            uint32_t c[B / 8];
-            byte = encode_block<T, FMT>(v, magnitude<B>(v), t, t6, c);
-            store_codes<B>(codes + r * pitch + static_cast<size_t>(b) * (B / 2), c);
+    const int tiles = scale_tiles_per_row(FMT, K);
+    const int lane = threadIdx.x & 31, b = blockIdx.x * 32 + lane, blocks = K / B;
+    const int octets = static_cast<int>((rows + 127ll) / 128 * 4);
+    for (int o = blockIdx.y; o < octets; o += gridDim.y) {
+        const int r0 = (o >> 2) * 128 + (o & 3) * 8 + (threadIdx.x >> 5);
+        if (r0 >= rows) continue;
+        uint32_t byte[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < 4; h += HELD) {
+            uint32_t w[HELD][WORDS];
+#pragma unroll
+            for (int j = 0; j < HELD; j++) {
+                const int r = r0 + 32 * (h + j);
+                if (r < rows && b < blocks) {
+                    const uint32_t* p = reinterpret_cast<const uint32_t*>(x + r * ldx + static_cast<size_t>(b) * B);
+                    if constexpr (ALIGN == 32) {
+#pragma unroll
+                        for (int i = 0; i < WORDS; i += 8) ldg32(p + i, w[j] + i);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4*>(w[j] + i) = __ldg(reinterpret_cast<const uint4*>(p + i));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < WORDS; i++) w[j][i] = 0;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < HELD; j++) {
+                const int r = r0 + 32 * (h + j);
+                if (r >= rows) break;
+                float v[B];
+                unpack<T, B>(w[j], v);
+                uint32_t c[B / 8];
+                byte[h + j] = encode_block<T, FMT>(v, magnitude<T, B>(w[j]), t, t6, c);
+                if (static_cast<size_t>(b) * (B / 2) < pitch) store_codes<B>(codes + r * pitch + static_cast<size_t>(b) * (B / 2), c);
+            }
         }
-        uint32_t word = byte << (8 * (threadIdx.x & 3));
-        word |= __shfl_xor_sync(0xffffffffu, word, 1);
-        word |= __shfl_xor_sync(0xffffffffu, word, 2);
-        if ((threadIdx.x & 3) == 0 && i < total) *reinterpret_cast<uint32_t*>(scales + scale_word(r, b >> 2, tiles)) = word;
+        uint32_t word[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            word[j] = byte[j] << (8 * (lane & 3));
+            word[j] |= __shfl_xor_sync(0xffffffffu, word[j], 1);
+            word[j] |= __shfl_xor_sync(0xffffffffu, word[j], 2);
+        }
+        if ((lane & 3) == 0 && (b >> 2) < tiles)
+            *reinterpret_cast<uint4*>(scales + scale_word(r0, b >> 2, tiles)) = make_uint4(word[0], word[1], word[2], word[3]);
     }
 }
 
-// Blocks along the columns: one thread per block of one column of x, i.e. along a row of the transposed tensor.
+// Blocks along the rows, along the columns, or both, of a 128 x 128 tile in shared memory: x is read once whatever its
+// alignment, and both directions' scale bytes make whole 512-byte tiles.  Shared memory: rows of W words, in which the
+// 8-word group g of row r lies at g ^ (r / B) % 4 - a column's reader takes words of four row blocks at once (lane = 8
+// words x 4 row blocks), which the exchange puts into different banks.
 template <class T, int FMT>
-__global__ void __launch_bounds__(kThreads) quantize_cols_kernel(const T* __restrict__ x, long long ldx, int rows, int K,
-                                                                 float* tscale, const uint32_t* partial, int partials,
-                                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    constexpr int B = Format<FMT>::BLOCK;
+struct TileCfg {
+    static constexpr int B = Format<FMT>::BLOCK, NB = 128 / B;      // blocks across the tile
+    static constexpr int W = 32 * sizeof(T);                        // words of a row
+    static constexpr int CPW = 4 / sizeof(T);                       // columns in a word
+    static constexpr int SMEM = 128 * W * 4 + 2 * NB * 128;
+};
+
+// 16 bytes of a row from element c on, zeros behind its K elements.  Off a 16-byte boundary: the two aligned vectors that
+// hold them, shifted together - where both lie inside the row; else element by element.
+template <class T>
+__device__ __forceinline__ uint4 load_vector(const T* row, long long c, int K, bool aligned) {
+    constexpr int VE = 16 / sizeof(T);
+    const T* p = row + c;
+    if (aligned && c + VE <= K) return __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const int before = static_cast<int>(off / sizeof(T));
+    if (c >= before && c - before + 2 * VE <= K) {
+        const uint4* q = reinterpret_cast<const uint4*>(p - before);
+        const uint4 lo = __ldg(q), hi = __ldg(q + 1);
+        uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (off & 8) {
+#pragma unroll
+            for (int i = 0; i < 6; i++) w[i] = w[i + 2];
+        }
+        if (off & 4) {
+#pragma unroll
+            for (int i = 0; i < 5; i++) w[i] = w[i + 1];
+        }
+        if constexpr (sizeof(T) == 2) {
+            if (off & 2) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = __byte_perm(w[i], w[i + 1], 0x5432);
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    alignas(16) T e[VE];
+#pragma unroll
+    for (int i = 0; i < VE; i++) e[i] = c + i < K ? p[i] : from_f32<T>(0.0f);
+    return *reinterpret_cast<const uint4*>(e);
+}
+
+template <class T, int FMT, bool COLS>
+__global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, int vec, unsigned tiles_x, float* tscale,
+                                                                 const uint32_t* partial, int partials, uint8_t* __restrict__ codes,
+                                                                 uint8_t* __restrict__ scales, uint8_t* __restrict__ codes_t,
+                                                                 uint8_t* __restrict__ scales_t) {
+    using C = TileCfg<T, FMT>;
+    constexpr int B = C::B, NB = C::NB, W = C::W, CPW = C::CPW, BW = B * sizeof(T) / 4;
+    extern __shared__ __align__(16) uint32_t tile[];
+    uint8_t* sc = reinterpret_cast<uint8_t*>(tile + 128 * W);       // [NB / 4][512] along the rows
+    uint8_t* sc_t = sc + NB * 128;                                  // the same along the columns
     pdl_launch_dependents();
     pdl_wait_prior();
-    float t = 1.0f, t6 = 6.0f;
-    if constexpr (FMT == RDB_FP4_NVFP4) {
-        t = tensor_scale(tscale, partial, partials);
-        t6 = t * 6.0f;
-        if (partial && blockIdx.x == 0 && threadIdx.x == 0) *tscale = t;
+    // the last tiles first: the first pass read them last, and they may still be in L2
+    const unsigned id = gridDim.x - 1 - blockIdx.x;
+    const long long tr = id / tiles_x, tc = id - tr * tiles_x;
+    const long long r0 = tr * 128, c0 = tc * 128;
+    auto at = [](int r, int w) { return r * W + (w ^ (((r / B) & 3) << 3)); };
+
+    // ---- x -> shared memory, zeros outside
+    constexpr int V = W / 4, VE = 16 / sizeof(T);                   // vectors of a row, elements of a vector
+#pragma unroll 4
+    for (int i = threadIdx.x; i < 128 * V; i += kThreads) {
+        const int r = i / V, v = i % V;
+        const long long c = c0 + v * VE;
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (r0 + r < rows && c < K) q = load_vector(x + (r0 + r) * ldx, c, K, vec);
+        *reinterpret_cast<uint4*>(tile + at(r, 4 * v)) = q;
     }
-    const size_t pitch = row_bytes(rows);
-    const int tiles = scale_tiles_per_row(FMT, rows);
-    const long long total = static_cast<long long>(K) * tiles;              // a thread does the four blocks of a word
-    for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * kThreads) {
-        const int col = static_cast<int>(i / K);
-        const size_t c = i - static_cast<long long>(col) * K;               // neighbours take neighbouring columns
-        uint32_t word = 0;
-        for (int j = 0; j < 4; j++) {
-            const long long r0 = (4ll * col + j) * B;
-            if (static_cast<size_t>(r0 / 2) >= pitch) break;
-            float v[B];
+    float t;
+    Divisor t6;
+    fetch_scale<FMT>(tscale, partial, partials, t, t6);
+    __syncthreads();
+
+    // ---- blocks along the rows
+    {
+        const size_t pitch = row_bytes(K);
 #pragma unroll
-            for (int q = 0; q < B; q++) v[q] = r0 + q < rows ? to_f32(x[(r0 + q) * ldx + c]) : 0.0f;
-            uint32_t o[B / 8];
-            word |= encode_block<T, FMT>(v, magnitude<B>(v), t, t6, o) << (8 * j);
-            store_codes<B>(codes + c * pitch + r0 / 2, o);
+        for (int i = threadIdx.x; i < 128 * NB; i += kThreads) {
+            const int r = i / NB, b = i % NB;
+            uint32_t w[BW];
+#pragma unroll
+            for (int j = 0; j < BW; j += 4) *reinterpret_cast<uint4*>(w + j) = *reinterpret_cast<const uint4*>(tile + at(r, b * BW + j));
+            float v[B];
+            unpack<T, B>(w, v);
+            uint32_t c[B / 8];
+            sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT>(v, magnitude<T, B>(w), t, t6, c));
+            const size_t k2 = (c0 + b * B) / 2;
+            if (r0 + r < rows && k2 < pitch) store_codes<B>(codes + (r0 + r) * pitch + k2, c);
         }
-        *reinterpret_cast<uint32_t*>(scales + scale_word(c, col, tiles)) = word;
     }
+    // ---- blocks along the columns
+    if constexpr (COLS) {
+        const size_t pitch = row_bytes(rows);
+        const int lane = threadIdx.x & 31, g = lane >> 3;
+#pragma unroll 1
+        for (int i = threadIdx.x >> 5; i < (W / 8) * (NB / 4); i += kThreads / 32) {
+            const int word = (i % (W / 8)) * 8 + (lane & 7), rb = (i / (W / 8)) * 4 + g;      // this thread's word, row block
+            uint32_t raw[B];
+#pragma unroll
+            for (int j = 0; j < B; j++) raw[j] = tile[at(rb * B + j, word)];
+#pragma unroll
+            for (int h = 0; h < CPW; h++) {
+                uint32_t w[BW];
+                if constexpr (CPW == 1) {
+#pragma unroll
+                    for (int j = 0; j < B; j++) w[j] = raw[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < B / 2; j++) w[j] = __byte_perm(raw[2 * j], raw[2 * j + 1], h ? 0x7632 : 0x5410);
+                }
+                float v[B];
+                unpack<T, B>(w, v);
+                uint32_t c[B / 8];
+                const int col = word * CPW + h;
+                sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT>(v, magnitude<T, B>(w), t, t6, c));
+                const size_t k2 = (r0 + rb * B) / 2;
+                if (c0 + col < K && k2 < pitch) store_codes<B>(codes_t + (c0 + col) * pitch + k2, c);
+            }
+        }
+    }
+    __syncthreads();
+    // ---- whole scale tiles
+    constexpr int VECS = NB / 4 * 32;
+    if (threadIdx.x < VECS) {
+        if (r0 < rows) {
+            const int tiles = scale_tiles_per_row(FMT, K);
+            *reinterpret_cast<uint4*>(scales + (tr * tiles + tc * (NB / 4)) * TILE_BYTES + threadIdx.x * 16) = reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+        }
+    } else if (COLS && threadIdx.x < 2 * VECS) {
+        if (c0 < K) {
+            const int tiles = scale_tiles_per_row(FMT, rows), i = threadIdx.x - VECS;
+            *reinterpret_cast<uint4*>(scales_t + (tc * tiles + tr * (NB / 4)) * TILE_BYTES + i * 16) = reinterpret_cast<const uint4*>(sc_t)[i];
+        }
+    }
+}
+
+// Eight codes -> eight halves (exact).
+__device__ __forceinline__ void decode8(uint32_t w, __half2* h) {
+    uint32_t o[4];
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = *reinterpret_cast<const __half2*>(o + i);
 }
 
 // Scale byte -> the value that multiplies e2m1, without the tensor scale.
@@ -281,44 +489,91 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     }
 }
 
-__device__ __forceinline__ float element_value(uint32_t code) {
-    const uint32_t m = code & 7;
-    // exponent field 1..3 -> 2^(e - 1) (1 + m / 2); 0 -> m / 2
-    const float a = m < 2 ? 0.5f * m : __uint_as_float(((m >> 1) + 126) << 23 | (m & 1) << 22);
-    return code & 8 ? -a : a;
-}
-
 template <class T, int FMT>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                                              const float* tscale, int rows, int K, T* __restrict__ out) {
-    constexpr int B = Format<FMT>::BLOCK;
-    pdl_launch_dependents();
-    pdl_wait_prior();
-    const float t = FMT == RDB_FP4_NVFP4 ? *tscale : 1.0f;
-    const size_t pitch = row_bytes(K);
-    const int tiles = scale_tiles_per_row(FMT, K);
-    const long long per_row = (K + 1) / 2, total = per_row * rows;
-    for (long long i = blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x; i < total; i += static_cast<long long>(gridDim.x) * kThreads) {
-        const long long r = i / per_row;
-        const int k = static_cast<int>(i - r * per_row) * 2, b = k / B;
-        const uint32_t c = codes[r * pitch + k / 2];
-        const float s = scale_value<FMT>(scales[scale_word(r, b >> 2, tiles) + (b & 3)]);
-        T* o = out + r * static_cast<size_t>(K) + k;
-        o[0] = from_f32<T>(element_value(c & 15) * s * t);
-        if (k + 1 < K) o[1] = from_f32<T>(element_value(c >> 4) * s * t);
+__device__ __forceinline__ void decode_block(uint32_t codes, uint32_t scale, float t, T* v) {
+    const float f = scale_value<FMT>(scale);
+    __half2 h[4];
+    decode8(codes, h);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 e = __half22float2(h[i]);
+        v[2 * i] = from_f32<T>(e.x * f * t);
+        v[2 * i + 1] = from_f32<T>(e.y * f * t);
     }
 }
 
-static int launch(const void* kernel, long long items, long long cap, void** args, cudaStream_t stream, int* grid_out = nullptr) {
-    long long blocks = (items + kThreads - 1) / kThreads;
-    if (blocks > cap) blocks = cap;
-    if (blocks < 1) blocks = 1;
-    if (grid_out) *grid_out = static_cast<int>(blocks);
+// A warp takes 256 elements (8 per lane) of the rows r, r + 32, r + 64, r + 96 of a 128-row tile: their scale words are one
+// 16-byte load.  element * scale is exact in fp32, the tensor scale's product rounds, the output type rounds again.
+// vec: rows of the output start on 16-byte boundaries; else the values pass through shared memory, so that neighbouring
+// lanes store neighbouring elements.
+template <class T, int FMT>
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                              const float* tscale, int rows, int K, int vec, T* __restrict__ out) {
+    constexpr int B = Format<FMT>::BLOCK;
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    __shared__ __align__(16) T stage[kThreads / 32][256];
+    const float t = FMT == RDB_FP4_NVFP4 ? *tscale : 1.0f;
+    const size_t pitch = row_bytes(K);
+    const int tiles = scale_tiles_per_row(FMT, K);
+    const int lane = threadIdx.x & 31;
+    const long long k0 = blockIdx.x * 256ll;
+    const int octets = static_cast<int>((rows + 127ll) / 128 * 4);
+    for (int o = blockIdx.y; o < octets; o += gridDim.y) {
+        const int r0 = (o >> 2) * 128 + (o & 3) * 8 + (threadIdx.x >> 5);
+        if (r0 >= rows) continue;
+        if (vec) {
+            const long long k = k0 + 8 * lane;
+            if (k >= K) continue;
+            uint32_t c[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) c[j] = r0 + 32 * j < rows ? __ldg(reinterpret_cast<const uint32_t*>(codes + (r0 + 32 * j) * pitch + k / 2)) : 0;
+            const int b = static_cast<int>(k / B);
+            const uint4 s4 = __ldg(reinterpret_cast<const uint4*>(scales + scale_word(r0, b >> 2, tiles)));
+            const uint32_t s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = r0 + 32 * j;
+                if (r >= rows) break;
+                alignas(16) T v[8];
+                decode_block<T, FMT>(c[j], (s[j] >> (8 * (b & 3))) & 0xFF, t, v);
+                uint4* p = reinterpret_cast<uint4*>(out + r * static_cast<size_t>(K) + k);
+#pragma unroll
+                for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; i++) p[i] = reinterpret_cast<const uint4*>(v)[i];
+            }
+        } else {
+            T* mine = stage[threadIdx.x >> 5];
+            const long long k = k0 + 8 * lane;
+            const int b = static_cast<int>(k / B);
+            const uint4 s4 = k < K ? __ldg(reinterpret_cast<const uint4*>(scales + scale_word(r0, b >> 2, tiles))) : make_uint4(0, 0, 0, 0);
+            const uint32_t s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int r = r0 + 32 * j;
+                if (r >= rows) break;
+                const uint32_t c = k < K ? __ldg(reinterpret_cast<const uint32_t*>(codes + r * pitch + k / 2)) : 0;
+                alignas(16) T v[8];
+                decode_block<T, FMT>(c, (s[j] >> (8 * (b & 3))) & 0xFF, t, v);
+#pragma unroll
+                for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; i++) reinterpret_cast<uint4*>(mine + 8 * lane)[i] = reinterpret_cast<const uint4*>(v)[i];
+                __syncwarp();
+                T* to = out + r * static_cast<size_t>(K) + k0;
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    if (k0 + 32 * i + lane < K) to[32 * i + lane] = mine[32 * i + lane];
+                __syncwarp();
+            }
+        }
+    }
+}
+
+// Every kernel of this file waits for its predecessor before it touches memory: the early start only hides the launch.
+static int launch(const void* kernel, dim3 grid, int smem, void** args, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    // every kernel of this file waits for its predecessor before it touches memory: the early start only hides the launch
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -328,42 +583,68 @@ static int launch(const void* kernel, long long items, long long cap, void** arg
     return RDB_SUCCESS;
 }
 
+// Grid of the kernels that walk octets of rows (grid.y strides).
+static dim3 octet_grid(int rows, long long columns) {
+    long long y = rows < 32 ? (rows + 7) / 8 : (static_cast<long long>(rows) + 127) / 128 * 4;
+    return dim3(static_cast<unsigned>(columns), static_cast<unsigned>(y < 65535 ? y : 65532));
+}
+
+template <class T, int FMT, bool COLS>
+static int launch_tiles(int rows, int K, void** args, unsigned* tiles_x, cudaStream_t stream) {
+    using C = TileCfg<T, FMT>;
+    static bool attr_set[kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return RDB_CUDA_ERROR;
+    auto kernel = quantize_tile_kernel<T, FMT, COLS>;
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return RDB_CUDA_ERROR;
+        attr_set[dev] = true;
+    }
+    // scales are filled up to 256 elements along either direction that is quantised
+    const long long x = (static_cast<long long>(K) + 255) / 256 * 2;
+    const long long y = COLS ? (static_cast<long long>(rows) + 255) / 256 * 2 : (static_cast<long long>(rows) + 127) / 128;
+    if (x * y > 0x7FFFFFFFll) return RDB_SIZE_ABOVE_LIMIT;
+    *tiles_x = static_cast<unsigned>(x);
+    return launch(reinterpret_cast<const void*>(kernel), dim3(static_cast<unsigned>(x * y)), C::SMEM, args, stream);
+}
+
 template <class T, int FMT>
 static int quantize(const void* x_, long long ldx, int rows, int K, float* tscale, bool given, uint8_t* codes, uint8_t* scales,
                     uint8_t* codes_t, uint8_t* scales_t, float* workspace, const DeviceInfo* info, cudaStream_t stream) {
+    constexpr int B = Format<FMT>::BLOCK;
     const T* x = static_cast<const T*>(x_);
-    bool vec = (reinterpret_cast<uintptr_t>(x) & 31u) == 0 && (static_cast<size_t>(ldx) * sizeof(T)) % 32 == 0;
-    const long long cap = info->sm_count * 8ll;
+    const size_t row = static_cast<size_t>(ldx) * sizeof(T);
+    const bool by32 = (reinterpret_cast<uintptr_t>(x) & 31u) == 0 && row % 32 == 0, by16 = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && row % 16 == 0;
     uint32_t* partial = nullptr;
     int partials = 0;
     if (FMT == RDB_FP4_NVFP4 && !given) {
         partial = reinterpret_cast<uint32_t*>(workspace);
-        void* args[] = {&x, &ldx, &rows, &K, &vec, &partial};
-        const int per_row = (K + 32 / static_cast<int>(sizeof(T)) - 1) / (32 / static_cast<int>(sizeof(T)));
-        const int r = launch(reinterpret_cast<const void*>(amax_kernel<T>), static_cast<long long>(per_row) * rows,
-                             cap < kAmaxBlocks ? cap : kAmaxBlocks, args, stream, &partials);
+        const long long units = ((K - 1) / kAmaxStretch + 1ll) * rows, blocks = (units + 7) / 8;
+        partials = static_cast<int>(blocks < kAmaxBlocks ? blocks : kAmaxBlocks);
+        if (partials > info->sm_count * 6) partials = info->sm_count * 6;
+        void* args[] = {&x, &ldx, &rows, &K, &partial};
+        const int r = launch(reinterpret_cast<const void*>(amax_kernel<T>), dim3(partials), 0, args, stream);
         if (r != RDB_SUCCESS) return r;
     }
-    if (codes) {
-        void* args[] = {&x, &ldx, &rows, &K, &vec, &tscale, &partial, &partials, &codes, &scales};
-        const int r = launch(reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT>), 4ll * scale_tiles_per_row(FMT, K) * rows, cap, args, stream);
-        if (r != RDB_SUCCESS) return r;
+    if (!codes_t && by16 && K % B == 0) {
+        void* args[] = {&x, &ldx, &rows, &K, &tscale, &partial, &partials, &codes, &scales};
+        const dim3 grid = octet_grid(rows, (4ll * scale_tiles_per_row(FMT, K) + 31) / 32);
+        return launch(by32 ? reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT, 32>) : reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT, 16>),
+                      grid, 0, args, stream);
     }
-    if (codes_t) {
-        void* args[] = {&x, &ldx, &rows, &K, &tscale, &partial, &partials, &codes_t, &scales_t};
-        const int r = launch(reinterpret_cast<const void*>(quantize_cols_kernel<T, FMT>), static_cast<long long>(scale_tiles_per_row(FMT, rows)) * K, cap, args, stream);
-        if (r != RDB_SUCCESS) return r;
-    }
-    return RDB_SUCCESS;
+    int vec = by16;
+    unsigned tiles_x = 0;
+    void* args[] = {&x, &ldx, &rows, &K, &vec, &tiles_x, &tscale, &partial, &partials, &codes, &scales, &codes_t, &scales_t};
+    return codes_t ? launch_tiles<T, FMT, true>(rows, K, args, &tiles_x, stream) : launch_tiles<T, FMT, false>(rows, K, args, &tiles_x, stream);
 }
 
 template <class T>
-static int dequantize(const uint8_t* codes, const uint8_t* scales, const float* tscale, int format, int rows, int K, void* out_,
-                      const DeviceInfo* info, cudaStream_t stream) {
+static int dequantize(const uint8_t* codes, const uint8_t* scales, const float* tscale, int format, int rows, int K, void* out_, cudaStream_t stream) {
     T* out = static_cast<T*>(out_);
-    void* args[] = {&codes, &scales, &tscale, &rows, &K, &out};
+    int vec = aligned16(out) && K * sizeof(T) % 16 == 0 && K % 8 == 0;
+    void* args[] = {&codes, &scales, &tscale, &rows, &K, &vec, &out};
     return launch(format == RDB_FP4_NVFP4 ? reinterpret_cast<const void*>(dequantize_kernel<T, RDB_FP4_NVFP4>) : reinterpret_cast<const void*>(dequantize_kernel<T, RDB_FP4_MXFP4>),
-                  (static_cast<long long>(K) + 1) / 2 * rows, info->sm_count * 8ll, args, stream);
+                  octet_grid(rows, (static_cast<long long>(K) + 255) / 256), 0, args, stream);
 }
 
 static int check(int type, int rows, int K, int format) {
@@ -391,7 +672,7 @@ int rdb_quantize_fp4(const void* x, int x_type, long long ldx, int rows, int K, 
     const int ok = check(x_type, rows, K, format);
     if (ok != RDB_SUCCESS) return ok;
     if (ldx < K) return RDB_BAD_SHAPE;
-    if (!x || (!codes && !codes_t) || (codes && !scales) || (codes_t && !scales_t)) return RDB_INVALID_CONFIG;
+    if (!x || !codes || !scales || (codes_t == nullptr) != (scales_t == nullptr)) return RDB_INVALID_CONFIG;
     if (format == RDB_FP4_NVFP4 && (!tensor_scale || (!scale_given && !workspace))) return RDB_INVALID_CONFIG;
     const uintptr_t size = x_type == RDB_TYPE_FP32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(x) % size || !rdb::aligned16(codes) || !rdb::aligned16(scales) || !rdb::aligned16(codes_t) ||
@@ -417,13 +698,10 @@ int rdb_dequantize_fp4(const uint8_t* codes, const uint8_t* scales, const float*
     if (!rdb::aligned16(codes) || !rdb::aligned16(scales) || reinterpret_cast<uintptr_t>(out) % (out_type == RDB_TYPE_FP32 ? 4 : 2) ||
         (reinterpret_cast<uintptr_t>(tensor_scale) & 3u))
         return RDB_BAD_ALIGNMENT;
-    int err = 0;
-    rdb::DeviceInfo* info = rdb::device_info(&err);
-    if (!info) return err;
     auto s = static_cast<cudaStream_t>(stream);
-    if (out_type == RDB_TYPE_BF16) return dequantize<__nv_bfloat16>(codes, scales, tensor_scale, format, rows, K, out, info, s);
-    if (out_type == RDB_TYPE_FP16) return dequantize<__half>(codes, scales, tensor_scale, format, rows, K, out, info, s);
-    return dequantize<float>(codes, scales, tensor_scale, format, rows, K, out, info, s);
+    if (out_type == RDB_TYPE_BF16) return dequantize<__nv_bfloat16>(codes, scales, tensor_scale, format, rows, K, out, s);
+    if (out_type == RDB_TYPE_FP16) return dequantize<__half>(codes, scales, tensor_scale, format, rows, K, out, s);
+    return dequantize<float>(codes, scales, tensor_scale, format, rows, K, out, s);
 }
 
 }  // extern "C"

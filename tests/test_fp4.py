@@ -271,6 +271,7 @@ def test_quantize_what_is_no_number(cuda_device, form):
         check_quantized(c, v.float().numpy().T.copy(), form)
         d = R.dequantize_fp4(r, torch.float32).cpu()
         b = BLOCK[form]
+        assert torch.equal(torch.isnan(R.dequantize_fp4(c).cpu()).reshape(320, -1), torch.isnan(torch.from_numpy(values(*plain(c)[:2], form, 40))))
         bad = ~torch.isfinite(v.float()).reshape(40, -1, b).all(dim=2)
         assert torch.equal(torch.isnan(d).reshape(40, -1, b).all(dim=2), bad) and torch.equal(torch.isnan(d).reshape(40, -1, b).any(dim=2), bad)
 
