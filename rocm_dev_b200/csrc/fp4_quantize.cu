@@ -59,21 +59,30 @@ __device__ __forceinline__ void unpack(const uint32_t* w, float* v) {
     }
 }
 
-// Largest magnitude of N elements held in words, as fp32 bits: non-negative floats order like integers, infinities and
-// NaNs above every number.  16-bit types are compared two at a time.
+// Largest magnitude of elements held in words, as fp32 bits: non-negative floats order like integers, infinities and NaNs
+// above every number.  16-bit types are compared two at a time: the halves of the result are the maxima of the halves.
+template <int WORDS>
+__device__ __forceinline__ uint32_t halves_magnitude(const uint32_t* w) {
+    uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int i = 1; i < WORDS; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    return m;
+}
+template <class T>
+__device__ __forceinline__ uint32_t bits_of_half(uint32_t h) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) return h << 16;
+    else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(h))));
+}
 template <class T, int N>
 __device__ __forceinline__ uint32_t magnitude(const uint32_t* w) {
-    uint32_t m = 0;
     if constexpr (sizeof(T) == 4) {
+        uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < N; i++) m = max(m, w[i] & 0x7FFFFFFFu);
         return m;
     } else {
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
-        m = max(m & 0xFFFFu, m >> 16);
-        if constexpr (std::is_same_v<T, __nv_bfloat16>) return m << 16;
-        else return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+        const uint32_t m = halves_magnitude<N / 2>(w);
+        return bits_of_half<T>(max(m & 0xFFFFu, m >> 16));
     }
 }
 
@@ -107,77 +116,100 @@ __device__ __forceinline__ uint32_t pack8(const float* q) {
     return r;
 }
 
-// a / d rounded to fp32 like the IEEE division, for a divisor shared by many numerators: with inv = RN(1 / d) and q within a
-// unit of the last place of a / d, RN(q + inv * (a - q d)) is the rounded quotient (Markstein).  The first product can
-// miss by one and a half units; the step repairs that for all but quotients within 2^-22 units of a rounding border, and a
-// second step for those too (numerators of 16 bits do not come that near: they get one).  Divisors far from 1 are moved
-// by 2^64 together with the numerator, which is exact wherever the quotient is not below e2m1's first border anyway.
-struct Divisor {
-    float d, inv, move;
-    __device__ __forceinline__ void set(float x) {
-        move = x < 8.6736174e-19f ? 18446744073709551616.0f : x > 1.1529215e18f ? 5.4210109e-20f : 1.0f;
-        d = x * move;
-        inv = __frcp_rn(d);
-    }
-    template <int STEPS>
-    __device__ __forceinline__ float quotient(float a) const {       // a already moved
-        float q = __fmul_rn(a, inv);
-#pragma unroll
-        for (int i = 0; i < STEPS; i++) q = __fmaf_rn(__fmaf_rn(-q, d, a), inv, q);
-        return q;
-    }
-};
+// Two fp32 operations in one instruction (sm_100).
+struct Pair { uint64_t v; };
+__device__ __forceinline__ Pair pair(float x, float y) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ void split(Pair p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p.v)); }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+    return p;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return p;
+}
 
-// One block: v[BLOCK] -> BLOCK / 8 words of codes, returns the scale byte.  t: the tensor scale, t6: 6 t as a divisor.
+// The NEGATIVE of a / d rounded to fp32 like the IEEE division, for a divisor d > 0 shared by many numerators: with
+// inv = RN(1 / d) and q within a unit of the last place of a / d, RN(q + inv * (a - q d)) is the rounded quotient
+// (Markstein).  The first product can miss by one and a half units; the step repairs that for all but quotients within
+// 2^-22 units of a rounding border, and a second step for those too (numerators of 16 bits do not come that near: they
+// get one).  The negative, because -q and -1 / d in the steps keep the sign of a zero.
+// Tensors whose scale is far from 1 have numerators and divisors moved by `move`, a power of two: exact wherever the
+// quotient is not far below e2m1's first border.
+struct Scale {
+    float t, t6, n6;             // tensor scale, 6 t moved, -RN(1 / t6)
+    float move;
+};
+template <int STEPS>
+__device__ __forceinline__ float neg_quotient(float a, float d, float ninv) {
+    float q = a * ninv;
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) q = __fmaf_rn(__fmaf_rn(q, d, a), ninv, q);
+    return q;
+}
+
+// One block: v[BLOCK] -> BLOCK / 8 words of codes, returns the scale byte.
 template <class T, int FMT>
-__device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, float t, const Divisor& t6, uint32_t* codes) {
-    constexpr int B = Format<FMT>::BLOCK;
+__device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, const Scale& sc, uint32_t* codes) {
+    constexpr int B = Format<FMT>::BLOCK, STEPS = sizeof(T) == 4 ? 2 : 1;
     uint32_t byte;
     if constexpr (FMT == RDB_FP4_MXFP4) {
         // the exponent field of the largest magnitude is floor(log2) + 127 (0 for subnormals, whose clamp is 0 too)
         const uint32_t e = amax >> 23;
         byte = e >= 2 ? e - 2 : 0;
         const float inv = __uint_as_float((254 - byte) << 23);       // 2^(127 - byte), exact products below
+        const Pair inv2 = pair(inv, inv);
 #pragma unroll
         for (int g = 0; g < B / 8; g++) {
             float q[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) q[i] = v[8 * g + i] * inv;
+            for (int i = 0; i < 8; i += 2) split(mul2(pair(v[8 * g + i], v[8 * g + i + 1]), inv2), q[i], q[i + 1]);
             codes[g] = pack8(q);
         }
         if (amax >= kInf) byte = 0xFF;
     } else {
-        const float a = fminf(__uint_as_float(amax), 3.4028235e38f) * t6.move;
-        byte = __nv_cvt_float_to_fp8(t6.quotient<2>(a), __NV_SATFINITE, __NV_E4M3);
+        const float a = fminf(__uint_as_float(amax), 3.4028235e38f) * sc.move;
+        byte = __nv_cvt_float_to_fp8(-neg_quotient<STEPS>(a, sc.t6, sc.n6), __NV_SATFINITE, __NV_E4M3);
+#pragma unroll
+        for (int g = 0; g < B / 8; g++) codes[g] = 0;
         if (byte != 0) {
             __nv_fp8_e4m3 s8;
             s8.__x = static_cast<__nv_fp8_storage_t>(byte);
-            Divisor s;
-            s.set(static_cast<float>(s8) * t);
-            if (s.move != 1.0f) {
+            const float d = static_cast<float>(s8) * sc.t * sc.move, ninv = -__frcp_rn(d);
+            const Pair d2 = pair(d, d), n2 = pair(ninv, ninv);
+            if (sc.move != 1.0f) {
 #pragma unroll
-                for (int i = 0; i < B; i++) v[i] *= s.move;
+                for (int i = 0; i < B; i++) v[i] *= sc.move;
             }
 #pragma unroll
             for (int g = 0; g < B / 8; g++) {
                 float q[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) q[i] = copysignf(s.quotient<sizeof(T) == 4 ? 2 : 1>(v[8 * g + i]), v[8 * g + i]);    // keeps -0
-                codes[g] = pack8(q);
-            }
-        } else {
+                for (int i = 0; i < 8; i += 2) {
+                    const Pair x = pair(v[8 * g + i], v[8 * g + i + 1]);
+                    Pair y = mul2(x, n2);
 #pragma unroll
-            for (int g = 0; g < B / 8; g++) codes[g] = 0;
+                    for (int k = 0; k < STEPS; k++) y = fma2(fma2(y, d2, x), n2, y);
+                    split(y, q[i], q[i + 1]);
+                }
+                codes[g] = pack8(q) ^ 0x88888888u;
+            }
         }
         if (amax >= kInf) byte = 0x7F;
     }
     return byte;
 }
 
-// t (NVFP4: given, or from the first pass's partial maxima) and 6 t, for the whole block: every thread takes part.
+// The tensor scale (NVFP4: given, or from the first pass's partial maxima), for the whole block: every thread takes part.
 template <int FMT>
-__device__ __forceinline__ void fetch_scale(float* tscale, const uint32_t* partial, int partials, float& t, Divisor& t6) {
-    t = 1.0f;
+__device__ __forceinline__ Scale fetch_scale(float* tscale, const uint32_t* partial, int partials) {
+    Scale sc = {1.0f, 6.0f, 0.0f, 1.0f};
     if constexpr (FMT == RDB_FP4_NVFP4) {
         if (partial) {
             __shared__ uint32_t warp_max[kThreads / 32];
@@ -189,13 +221,16 @@ __device__ __forceinline__ void fetch_scale(float* tscale, const uint32_t* parti
 #pragma unroll
             for (int w = 0; w < kThreads / 32; w++) m = max(m, warp_max[w]);
             constexpr float inv = 1.0f / 2688.0f;            // rounded to fp32 before it multiplies: part of the definition
-            if (m != 0) t = fmaxf(__fmul_rn(__uint_as_float(m), inv), 1.17549435e-38f);
-            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *tscale = t;
+            if (m != 0) sc.t = fmaxf(__fmul_rn(__uint_as_float(m), inv), 1.17549435e-38f);
+            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *tscale = sc.t;
         } else {
-            t = *tscale;
+            sc.t = *tscale;
         }
+        sc.move = sc.t < 8.6736174e-19f ? 18446744073709551616.0f : sc.t > 1.1529215e18f ? 5.4210109e-20f : 1.0f;   // 2^-60, 2^64; 2^60, 2^-64
+        sc.t6 = sc.t * 6.0f * sc.move;
+        sc.n6 = -__frcp_rn(sc.t6);
     }
-    t6.set(t * 6.0f);
+    return sc;
 }
 
 // First pass of a call that computes the tensor scale: one partial maximum per CTA.  A warp takes stretches of 1024
@@ -266,9 +301,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     constexpr int B = Format<FMT>::BLOCK, WORDS = B * sizeof(T) / 4, HELD = WORDS > 16 ? 2 : 4;
     pdl_launch_dependents();
     pdl_wait_prior();
-    float t;
-    Divisor t6;
-    fetch_scale<FMT>(tscale, partial, partials, t, t6);
+    const Scale scale = fetch_scale<FMT>(tscale, partial, partials);
     const size_t pitch = row_bytes(K);
     const int tiles = scale_tiles_per_row(FMT, K);
     const int lane = threadIdx.x & 31, b = blockIdx.x * 32 + lane, blocks = K / B;
@@ -304,7 +337,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
                 float v[B];
                 unpack<T, B>(w[j], v);
                 uint32_t c[B / 8];
-                byte[h + j] = encode_block<T, FMT>(v, magnitude<T, B>(w[j]), t, t6, c);
+                byte[h + j] = encode_block<T, FMT>(v, magnitude<T, B>(w[j]), scale, c);
                 if (static_cast<size_t>(b) * (B / 2) < pitch) store_codes<B>(codes + r * pitch + static_cast<size_t>(b) * (B / 2), c);
             }
         }
@@ -395,9 +428,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const T* __rest
         if (r0 + r < rows && c < K) q = load_vector(x + (r0 + r) * ldx, c, K, vec);
         *reinterpret_cast<uint4*>(tile + at(r, 4 * v)) = q;
     }
-    float t;
-    Divisor t6;
-    fetch_scale<FMT>(tscale, partial, partials, t, t6);
+    const Scale scale = fetch_scale<FMT>(tscale, partial, partials);
     __syncthreads();
 
     // ---- blocks along the rows
@@ -412,7 +443,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const T* __rest
             float v[B];
             unpack<T, B>(w, v);
             uint32_t c[B / 8];
-            sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT>(v, magnitude<T, B>(w), t, t6, c));
+            sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT>(v, magnitude<T, B>(w), scale, c));
             const size_t k2 = (c0 + b * B) / 2;
             if (r0 + r < rows && k2 < pitch) store_codes<B>(codes + (r0 + r) * pitch + k2, c);
         }
@@ -427,21 +458,26 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const T* __rest
             uint32_t raw[B];
 #pragma unroll
             for (int j = 0; j < B; j++) raw[j] = tile[at(rb * B + j, word)];
+            uint32_t amax[CPW];
+            if constexpr (CPW == 1) {
+                amax[0] = magnitude<T, B>(raw);
+            } else {                                                // a word holds two columns: their maxima together
+                const uint32_t m = halves_magnitude<B>(raw);
+                amax[0] = bits_of_half<T>(m & 0xFFFFu);
+                amax[1] = bits_of_half<T>(m >> 16);
+            }
 #pragma unroll
             for (int h = 0; h < CPW; h++) {
-                uint32_t w[BW];
-                if constexpr (CPW == 1) {
-#pragma unroll
-                    for (int j = 0; j < B; j++) w[j] = raw[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < B / 2; j++) w[j] = __byte_perm(raw[2 * j], raw[2 * j + 1], h ? 0x7632 : 0x5410);
-                }
                 float v[B];
-                unpack<T, B>(w, v);
+#pragma unroll
+                for (int j = 0; j < B; j++) {
+                    if constexpr (CPW == 1) v[j] = __uint_as_float(raw[j]);
+                    else if constexpr (std::is_same_v<T, __nv_bfloat16>) v[j] = __uint_as_float(h ? raw[j] & 0xFFFF0000u : raw[j] << 16);
+                    else v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(h ? raw[j] >> 16 : raw[j])));
+                }
                 uint32_t c[B / 8];
                 const int col = word * CPW + h;
-                sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT>(v, magnitude<T, B>(w), t, t6, c));
+                sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT>(v, amax[h], scale, c));
                 const size_t k2 = (r0 + rb * B) / 2;
                 if (c0 + col < K && k2 < pitch) store_codes<B>(codes_t + (c0 + col) * pitch + k2, c);
             }
