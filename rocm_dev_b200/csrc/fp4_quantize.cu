@@ -135,34 +135,35 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
     return p;
 }
 
-// The NEGATIVE of a / d rounded to fp32 like the IEEE division, for a divisor d > 0 shared by many numerators: with
-// inv = RN(1 / d) and q within a unit of the last place of a / d, RN(q + inv * (a - q d)) is the rounded quotient
-// (Markstein).  The first product can miss by one and a half units; the step repairs that for all but quotients within
-// 2^-22 units of a rounding border, and a second step for those too (numerators of 16 bits do not come that near: they
-// get one).  The negative, because -q and -1 / d in the steps keep the sign of a zero.
-// Tensors whose scale is far from 1 have numerators and divisors moved by `move`, a power of two: exact wherever the
-// quotient is not far below e2m1's first border.
+// Quotients a / d of many numerators by one divisor d > 0, rounded to fp32 as the IEEE division does as far as the result
+// tells.  With inv near 1 / d: q = a * inv, then the step q + inv * (a - q d).  It is NEGATIVE quotients that are
+// computed: with -q and -1 / d the step keeps the sign of a zero.
+// fp32 numerators: inv = RN(1 / d) and two steps - after the first, q is within a unit of the last place, and from such a q
+// the second gives the rounded quotient (Markstein).  16-bit numerators: the approximate reciprocal (one unit off) and one
+// step leave q within 2^-21 units of the quotient before its rounding; a quotient of a significand of 11 bits by one of 24
+// comes no nearer than 2^-19 units to the rounding borders next to a border of e2m1 or e4m3 (all of them were solved
+// for), so the code or scale byte that follows is the same.
 struct Scale {
-    float t, t6, n6;             // tensor scale, 6 t moved, -RN(1 / t6)
-    float move;
+    float t, t6, n6;             // tensor scale; 6 t and -1 / (6 t), both for numerators that are multiplied by `move`
+    float move;                  // 1, or a power of two for tensor scales so far from 1 that the steps would leave fp32
 };
-template <int STEPS>
-__device__ __forceinline__ float neg_quotient(float a, float d, float ninv) {
-    float q = a * ninv;
-#pragma unroll
-    for (int i = 0; i < STEPS; i++) q = __fmaf_rn(__fmaf_rn(q, d, a), ninv, q);
-    return q;
+template <class T>
+__device__ __forceinline__ float neg_reciprocal(float d) {
+    if constexpr (sizeof(T) == 4) return -__frcp_rn(d);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return -r;
 }
+template <class T>
+constexpr int kSteps = sizeof(T) == 4 ? 2 : 1;
 
-// One block: v[BLOCK] -> BLOCK / 8 words of codes, returns the scale byte.
-template <class T, int FMT>
+// One block: v[BLOCK] -> BLOCK / 8 words of codes, returns the scale byte.  MOVED: sc.move is not 1.
+template <class T, int FMT, bool MOVED>
 __device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, const Scale& sc, uint32_t* codes) {
-    constexpr int B = Format<FMT>::BLOCK, STEPS = sizeof(T) == 4 ? 2 : 1;
-    uint32_t byte;
+    constexpr int B = Format<FMT>::BLOCK;
     if constexpr (FMT == RDB_FP4_MXFP4) {
         // the exponent field of the largest magnitude is floor(log2) + 127 (0 for subnormals, whose clamp is 0 too)
-        const uint32_t e = amax >> 23;
-        byte = e >= 2 ? e - 2 : 0;
+        const uint32_t byte = max(static_cast<int>(amax >> 23) - 2, 0);
         const float inv = __uint_as_float((254 - byte) << 23);       // 2^(127 - byte), exact products below
         const Pair inv2 = pair(inv, inv);
 #pragma unroll
@@ -172,54 +173,61 @@ __device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, const 
             for (int i = 0; i < 8; i += 2) split(mul2(pair(v[8 * g + i], v[8 * g + i + 1]), inv2), q[i], q[i + 1]);
             codes[g] = pack8(q);
         }
-        if (amax >= kInf) byte = 0xFF;
+        return amax >= kInf ? 0xFF : byte;
     } else {
-        const float a = fminf(__uint_as_float(amax), 3.4028235e38f) * sc.move;
-        byte = __nv_cvt_float_to_fp8(-neg_quotient<STEPS>(a, sc.t6, sc.n6), __NV_SATFINITE, __NV_E4M3);
+        float a = __uint_as_float(amax);
+        if constexpr (MOVED) a *= sc.move;
+        const float top = 1024.0f * sc.t6;                           // beyond it everything saturates (given scales only)
+        if (!(a <= top)) {
+            a = top;
+            const float most = MOVED ? top / sc.move : top;
 #pragma unroll
-        for (int g = 0; g < B / 8; g++) codes[g] = 0;
-        if (byte != 0) {
-            __nv_fp8_e4m3 s8;
-            s8.__x = static_cast<__nv_fp8_storage_t>(byte);
-            const float d = static_cast<float>(s8) * sc.t * sc.move, ninv = -__frcp_rn(d);
-            const Pair d2 = pair(d, d), n2 = pair(ninv, ninv);
-            if (sc.move != 1.0f) {
-#pragma unroll
-                for (int i = 0; i < B; i++) v[i] *= sc.move;
-            }
-#pragma unroll
-            for (int g = 0; g < B / 8; g++) {
-                float q[8];
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const Pair x = pair(v[8 * g + i], v[8 * g + i + 1]);
-                    Pair y = mul2(x, n2);
-#pragma unroll
-                    for (int k = 0; k < STEPS; k++) y = fma2(fma2(y, d2, x), n2, y);
-                    split(y, q[i], q[i + 1]);
-                }
-                codes[g] = pack8(q) ^ 0x88888888u;
-            }
+            for (int i = 0; i < B; i++) v[i] = fminf(fmaxf(v[i], -most), most);
         }
-        if (amax >= kInf) byte = 0x7F;
+        float n = a * sc.n6;
+#pragma unroll
+        for (int k = 0; k < kSteps<T>; k++) n = __fmaf_rn(__fmaf_rn(n, sc.t6, a), sc.n6, n);
+        uint16_t e;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(e) : "f"(0.0f), "f"(-n));
+        uint32_t h2;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(e));
+        const uint32_t byte = e;
+        float d = __half2float(__ushort_as_half(static_cast<unsigned short>(h2))) * sc.t;
+        if constexpr (MOVED) d *= sc.move;
+        const float ninv = neg_reciprocal<T>(d);
+        const Pair d2 = pair(d, d), n2 = pair(ninv, ninv);
+#pragma unroll
+        for (int g = 0; g < B / 8; g++) {
+            float q[8];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                Pair x = pair(v[8 * g + i], v[8 * g + i + 1]);
+                if constexpr (MOVED) x = mul2(x, pair(sc.move, sc.move));
+                Pair y = mul2(x, n2);
+#pragma unroll
+                for (int k = 0; k < kSteps<T>; k++) y = fma2(fma2(y, d2, x), n2, y);
+                split(y, q[i], q[i + 1]);
+            }
+            codes[g] = byte != 0 ? pack8(q) ^ 0x88888888u : 0u;      // a scale of zero: zeros
+        }
+        return amax >= kInf ? 0x7F : byte;
     }
-    return byte;
 }
 
 // The tensor scale (NVFP4: given, or from the first pass's partial maxima), for the whole block: every thread takes part.
-template <int FMT>
+template <class T, int FMT, int THREADS>
 __device__ __forceinline__ Scale fetch_scale(float* tscale, const uint32_t* partial, int partials) {
     Scale sc = {1.0f, 6.0f, 0.0f, 1.0f};
     if constexpr (FMT == RDB_FP4_NVFP4) {
         if (partial) {
-            __shared__ uint32_t warp_max[kThreads / 32];
+            __shared__ uint32_t warp_max[THREADS / 32];
             uint32_t m = 0;
-            for (int i = threadIdx.x; i < partials; i += kThreads) m = max(m, __ldcg(partial + i));
+            for (int i = threadIdx.x; i < partials; i += THREADS) m = max(m, __ldcg(partial + i));
             m = __reduce_max_sync(0xffffffffu, m);
             if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < kThreads / 32; w++) m = max(m, warp_max[w]);
+            for (int w = 0; w < THREADS / 32; w++) m = max(m, warp_max[w]);
             constexpr float inv = 1.0f / 2688.0f;            // rounded to fp32 before it multiplies: part of the definition
             if (m != 0) sc.t = fmaxf(__fmul_rn(__uint_as_float(m), inv), 1.17549435e-38f);
             if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *tscale = sc.t;
@@ -228,7 +236,7 @@ __device__ __forceinline__ Scale fetch_scale(float* tscale, const uint32_t* part
         }
         sc.move = sc.t < 8.6736174e-19f ? 18446744073709551616.0f : sc.t > 1.1529215e18f ? 5.4210109e-20f : 1.0f;   // 2^-60, 2^64; 2^60, 2^-64
         sc.t6 = sc.t * 6.0f * sc.move;
-        sc.n6 = -__frcp_rn(sc.t6);
+        sc.n6 = neg_reciprocal<T>(sc.t6);
     }
     return sc;
 }
@@ -301,98 +309,105 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     constexpr int B = Format<FMT>::BLOCK, WORDS = B * sizeof(T) / 4, HELD = WORDS > 16 ? 2 : 4;
     pdl_launch_dependents();
     pdl_wait_prior();
-    const Scale scale = fetch_scale<FMT>(tscale, partial, partials);
+    const Scale scale = fetch_scale<T, FMT, kThreads>(tscale, partial, partials);
     const size_t pitch = row_bytes(K);
     const int tiles = scale_tiles_per_row(FMT, K);
     const int lane = threadIdx.x & 31, b = blockIdx.x * 32 + lane, blocks = K / B;
     const int octets = static_cast<int>((rows + 127ll) / 128 * 4);
-    for (int o = blockIdx.y; o < octets; o += gridDim.y) {
-        const int r0 = (o >> 2) * 128 + (o & 3) * 8 + (threadIdx.x >> 5);
-        if (r0 >= rows) continue;
-        uint32_t byte[4] = {0, 0, 0, 0};
+    auto body = [&](auto moved) {
+        for (int o = blockIdx.y; o < octets; o += gridDim.y) {
+            const int r0 = (o >> 2) * 128 + (o & 3) * 8 + (threadIdx.x >> 5);
+            if (r0 >= rows) continue;
+            uint32_t byte[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < 4; h += HELD) {
-            uint32_t w[HELD][WORDS];
+            for (int h = 0; h < 4; h += HELD) {
+                uint32_t w[HELD][WORDS];
 #pragma unroll
-            for (int j = 0; j < HELD; j++) {
-                const int r = r0 + 32 * (h + j);
-                if (r < rows && b < blocks) {
-                    const uint32_t* p = reinterpret_cast<const uint32_t*>(x + r * ldx + static_cast<size_t>(b) * B);
-                    if constexpr (ALIGN == 32) {
+                for (int j = 0; j < HELD; j++) {
+                    const int r = r0 + 32 * (h + j);
+                    if (r < rows && b < blocks) {
+                        const uint32_t* p = reinterpret_cast<const uint32_t*>(x + r * ldx + static_cast<size_t>(b) * B);
+                        if constexpr (ALIGN == 32) {
 #pragma unroll
-                        for (int i = 0; i < WORDS; i += 8) ldg32(p + i, w[j] + i);
+                            for (int i = 0; i < WORDS; i += 8) ldg32(p + i, w[j] + i);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4*>(w[j] + i) = __ldg(reinterpret_cast<const uint4*>(p + i));
+                        }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < WORDS; i += 4) *reinterpret_cast<uint4*>(w[j] + i) = __ldg(reinterpret_cast<const uint4*>(p + i));
+                        for (int i = 0; i < WORDS; i++) w[j][i] = 0;
                     }
-                } else {
+                }
 #pragma unroll
-                    for (int i = 0; i < WORDS; i++) w[j][i] = 0;
+                for (int j = 0; j < HELD; j++) {
+                    const int r = r0 + 32 * (h + j);
+                    if (r >= rows) break;
+                    float v[B];
+                    unpack<T, B>(w[j], v);
+                    uint32_t c[B / 8];
+                    byte[h + j] = encode_block<T, FMT, decltype(moved)::value>(v, magnitude<T, B>(w[j]), scale, c);
+                    if (static_cast<size_t>(b) * (B / 2) < pitch) store_codes<B>(codes + r * pitch + static_cast<size_t>(b) * (B / 2), c);
                 }
             }
+            uint32_t word[4];
 #pragma unroll
-            for (int j = 0; j < HELD; j++) {
-                const int r = r0 + 32 * (h + j);
-                if (r >= rows) break;
-                float v[B];
-                unpack<T, B>(w[j], v);
-                uint32_t c[B / 8];
-                byte[h + j] = encode_block<T, FMT>(v, magnitude<T, B>(w[j]), scale, c);
-                if (static_cast<size_t>(b) * (B / 2) < pitch) store_codes<B>(codes + r * pitch + static_cast<size_t>(b) * (B / 2), c);
+            for (int j = 0; j < 4; j++) {
+                word[j] = byte[j] << (8 * (lane & 3));
+                word[j] |= __shfl_xor_sync(0xffffffffu, word[j], 1);
+                word[j] |= __shfl_xor_sync(0xffffffffu, word[j], 2);
             }
+            if ((lane & 3) == 0 && (b >> 2) < tiles)
+                *reinterpret_cast<uint4*>(scales + scale_word(r0, b >> 2, tiles)) = make_uint4(word[0], word[1], word[2], word[3]);
         }
-        uint32_t word[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            word[j] = byte[j] << (8 * (lane & 3));
-            word[j] |= __shfl_xor_sync(0xffffffffu, word[j], 1);
-            word[j] |= __shfl_xor_sync(0xffffffffu, word[j], 2);
-        }
-        if ((lane & 3) == 0 && (b >> 2) < tiles)
-            *reinterpret_cast<uint4*>(scales + scale_word(r0, b >> 2, tiles)) = make_uint4(word[0], word[1], word[2], word[3]);
-    }
+    };
+    if (FMT == RDB_FP4_NVFP4 && scale.move != 1.0f) body(std::true_type());
+    else body(std::false_type());
 }
 
-// Blocks along the rows, along the columns, or both, of a 128 x 128 tile in shared memory: x is read once whatever its
+// Blocks along the rows, and along the columns too, of 128 x 128 tiles in shared memory: x is read once whatever its
 // alignment, and both directions' scale bytes make whole 512-byte tiles.  Shared memory: rows of W words, in which the
 // 8-word group g of row r lies at g ^ (r / B) % 4 - a column's reader takes words of four row blocks at once (lane = 8
-// words x 4 row blocks), which the exchange puts into different banks.
+// words x 4 row blocks), which the exchange puts into different banks.  Persistent blocks: while a tile is encoded, the
+// next one is copied into the other buffer (x on 16-byte boundaries; else the copy waits).
+constexpr int kTileThreads = 512;
 template <class T, int FMT>
 struct TileCfg {
     static constexpr int B = Format<FMT>::BLOCK, NB = 128 / B;      // blocks across the tile
     static constexpr int W = 32 * sizeof(T);                        // words of a row
     static constexpr int CPW = 4 / sizeof(T);                       // columns in a word
-    static constexpr int SMEM = 128 * W * 4 + 2 * NB * 128;
+    static constexpr int TILE_WORDS = 128 * W;
+    static constexpr int BUFFERS = 2;
+    static constexpr int SMEM = BUFFERS * TILE_WORDS * 4 + 2 * NB * 128;
+    static constexpr int PER_SM = sizeof(T) == 2 ? 2 : 1;
 };
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* src, bool exists) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(src), "r"(exists ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// 16 bytes of a row from element c on, zeros behind its K elements.  Off a 16-byte boundary: the two aligned vectors that
-// hold them, shifted together - where both lie inside the row; else element by element.
+// 16 bytes of a row from element c on, zeros behind its K elements.  Off a 16-byte boundary: the aligned words that hold
+// them, shifted together - where all lie inside the row; else element by element.
 template <class T>
 __device__ __forceinline__ uint4 load_vector(const T* row, long long c, int K, bool aligned) {
     constexpr int VE = 16 / sizeof(T);
     const T* p = row + c;
     if (aligned && c + VE <= K) return __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 15u;
-    const int before = static_cast<int>(off / sizeof(T));
-    if (c >= before && c - before + 2 * VE <= K) {
-        const uint4* q = reinterpret_cast<const uint4*>(p - before);
-        const uint4 lo = __ldg(q), hi = __ldg(q + 1);
-        uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        if (off & 8) {
-#pragma unroll
-            for (int i = 0; i < 6; i++) w[i] = w[i + 2];
+    if constexpr (sizeof(T) == 4) {
+        if (c + VE <= K) {
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+            return make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
         }
-        if (off & 4) {
-#pragma unroll
-            for (int i = 0; i < 5; i++) w[i] = w[i + 1];
+    } else {
+        const int odd = (reinterpret_cast<uintptr_t>(p) >> 1) & 1;
+        if (c >= odd && c + VE + odd <= K) {
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(p - odd);
+            const uint32_t w[5] = {__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3), odd ? __ldg(q + 4) : 0u};
+            const uint32_t s = 16 * odd;
+            return make_uint4(__funnelshift_r(w[0], w[1], s), __funnelshift_r(w[1], w[2], s), __funnelshift_r(w[2], w[3], s), __funnelshift_r(w[3], w[4], s));
         }
-        if constexpr (sizeof(T) == 2) {
-            if (off & 2) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = __byte_perm(w[i], w[i + 1], 0x5432);
-            }
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
     }
     alignas(16) T e[VE];
 #pragma unroll
@@ -401,102 +416,148 @@ __device__ __forceinline__ uint4 load_vector(const T* row, long long c, int K, b
 }
 
 template <class T, int FMT, bool COLS>
-__global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, int vec, unsigned tiles_x, float* tscale,
-                                                                 const uint32_t* partial, int partials, uint8_t* __restrict__ codes,
-                                                                 uint8_t* __restrict__ scales, uint8_t* __restrict__ codes_t,
-                                                                 uint8_t* __restrict__ scales_t) {
+__global__ void __launch_bounds__(kTileThreads, TileCfg<T, FMT>::PER_SM)
+quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, int vec, unsigned tiles_x, unsigned tiles_all, float* tscale,
+                     const uint32_t* partial, int partials, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                     uint8_t* __restrict__ codes_t, uint8_t* __restrict__ scales_t) {
     using C = TileCfg<T, FMT>;
     constexpr int B = C::B, NB = C::NB, W = C::W, CPW = C::CPW, BW = B * sizeof(T) / 4;
-    extern __shared__ __align__(16) uint32_t tile[];
-    uint8_t* sc = reinterpret_cast<uint8_t*>(tile + 128 * W);       // [NB / 4][512] along the rows
-    uint8_t* sc_t = sc + NB * 128;                                  // the same along the columns
+    extern __shared__ __align__(16) uint32_t buffers[];
+    uint8_t* sc = reinterpret_cast<uint8_t*>(buffers + C::BUFFERS * C::TILE_WORDS);     // [NB / 4][512] along the rows
+    uint8_t* sc_t = sc + NB * 128;                                                      // the same along the columns
     pdl_launch_dependents();
     pdl_wait_prior();
-    // the last tiles first: the first pass read them last, and they may still be in L2
-    const unsigned id = gridDim.x - 1 - blockIdx.x;
-    const long long tr = id / tiles_x, tc = id - tr * tiles_x;
-    const long long r0 = tr * 128, c0 = tc * 128;
     auto at = [](int r, int w) { return r * W + (w ^ (((r / B) & 3) << 3)); };
+    const size_t pitch = row_bytes(K), pitch_t = row_bytes(rows);
+    constexpr int V = W / 4, VE = 16 / sizeof(T), STEP = kTileThreads / V;     // vectors of a row, elements of a vector, rows a pass
 
-    // ---- x -> shared memory, zeros outside
-    constexpr int V = W / 4, VE = 16 / sizeof(T);                   // vectors of a row, elements of a vector
-#pragma unroll 4
-    for (int i = threadIdx.x; i < 128 * V; i += kThreads) {
-        const int r = i / V, v = i % V;
-        const long long c = c0 + v * VE;
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (r0 + r < rows && c < K) q = load_vector(x + (r0 + r) * ldx, c, K, vec);
-        *reinterpret_cast<uint4*>(tile + at(r, 4 * v)) = q;
-    }
-    const Scale scale = fetch_scale<FMT>(tscale, partial, partials);
-    __syncthreads();
-
-    // ---- blocks along the rows
-    {
-        const size_t pitch = row_bytes(K);
+    // The block's tiles are n = blockIdx.x, + gridDim.x, ... counted from the last one: the maximum's pass read those
+    // last, and they may still be in L2.  (tr, tc): row and column of tile n; moving on by gridDim.x tiles.
+    const unsigned tiles_y = tiles_all / tiles_x, hop_y = gridDim.x / tiles_x, hop_x = gridDim.x - hop_y * tiles_x;
+    auto advance = [&](int& tr, int& tc) {
+        tr -= hop_y;
+        tc -= hop_x;
+        if (tc < 0) { tc += tiles_x; tr--; }
+    };
+    // tile -> buffer, zeros outside x
+    const int fr = threadIdx.x / V, fv = threadIdx.x % V;
+    auto fetch = [&](int tr, int tc, uint32_t* tile) {
+        const long long c = tc * 128ll + fv * VE, row = tr * 128ll + fr;
+        const T* p = x + row * ldx;
+        if (vec && c + VE <= K) {
+            if (tr * 128ll + 128 <= rows) {
+                p += c;
 #pragma unroll
-        for (int i = threadIdx.x; i < 128 * NB; i += kThreads) {
-            const int r = i / NB, b = i % NB;
-            uint32_t w[BW];
+                for (int j = 0; j < 128 / STEP; j++, p += STEP * ldx) cp_async16(smem_u32(tile + at(fr + j * STEP, 4 * fv)), p, true);
+            } else {
 #pragma unroll
-            for (int j = 0; j < BW; j += 4) *reinterpret_cast<uint4*>(w + j) = *reinterpret_cast<const uint4*>(tile + at(r, b * BW + j));
-            float v[B];
-            unpack<T, B>(w, v);
-            uint32_t c[B / 8];
-            sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT>(v, magnitude<T, B>(w), scale, c));
-            const size_t k2 = (c0 + b * B) / 2;
-            if (r0 + r < rows && k2 < pitch) store_codes<B>(codes + (r0 + r) * pitch + k2, c);
-        }
-    }
-    // ---- blocks along the columns
-    if constexpr (COLS) {
-        const size_t pitch = row_bytes(rows);
-        const int lane = threadIdx.x & 31, g = lane >> 3;
-#pragma unroll 1
-        for (int i = threadIdx.x >> 5; i < (W / 8) * (NB / 4); i += kThreads / 32) {
-            const int word = (i % (W / 8)) * 8 + (lane & 7), rb = (i / (W / 8)) * 4 + g;      // this thread's word, row block
-            uint32_t raw[B];
-#pragma unroll
-            for (int j = 0; j < B; j++) raw[j] = tile[at(rb * B + j, word)];
-            uint32_t amax[CPW];
-            if constexpr (CPW == 1) {
-                amax[0] = magnitude<T, B>(raw);
-            } else {                                                // a word holds two columns: their maxima together
-                const uint32_t m = halves_magnitude<B>(raw);
-                amax[0] = bits_of_half<T>(m & 0xFFFFu);
-                amax[1] = bits_of_half<T>(m >> 16);
-            }
-#pragma unroll
-            for (int h = 0; h < CPW; h++) {
-                float v[B];
-#pragma unroll
-                for (int j = 0; j < B; j++) {
-                    if constexpr (CPW == 1) v[j] = __uint_as_float(raw[j]);
-                    else if constexpr (std::is_same_v<T, __nv_bfloat16>) v[j] = __uint_as_float(h ? raw[j] & 0xFFFF0000u : raw[j] << 16);
-                    else v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(h ? raw[j] >> 16 : raw[j])));
+                for (int j = 0; j < 128 / STEP; j++) {
+                    const bool exists = row + j * STEP < rows;
+                    cp_async16(smem_u32(tile + at(fr + j * STEP, 4 * fv)), exists ? p + j * STEP * ldx + c : x, exists);
                 }
+            }
+        } else {
+            uint4 q[128 / STEP];
+#pragma unroll
+            for (int j = 0; j < 128 / STEP; j++)
+                q[j] = row + j * STEP < rows && c < K ? load_vector(p + j * STEP * ldx, c, K, vec) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 128 / STEP; j++) *reinterpret_cast<uint4*>(tile + at(fr + j * STEP, 4 * fv)) = q[j];
+        }
+        cp_async_commit();
+    };
+
+    int tr = static_cast<int>(tiles_y - 1 - blockIdx.x / tiles_x), tc = static_cast<int>(tiles_x - 1 - blockIdx.x % tiles_x);
+    int ntr = tr, ntc = tc, turn = 0;
+    fetch(tr, tc, buffers);
+    const Scale scale = fetch_scale<T, FMT, kTileThreads>(tscale, partial, partials);
+    auto body = [&](auto moved) {
+    for (unsigned n = blockIdx.x; n < tiles_all; n += gridDim.x, turn ^= 1, tr = ntr, tc = ntc) {
+        if (n + gridDim.x < tiles_all) {
+            advance(ntr, ntc);
+            fetch(ntr, ntc, buffers + (turn ^ 1) * C::TILE_WORDS);
+            cp_async_wait<1>();
+        } else {
+            cp_async_wait<0>();
+        }
+        __syncthreads();
+        const int rows_left = static_cast<int>(rows - tr * 128ll < 128 ? rows - tr * 128ll : 128);       // may be negative: scales only
+        const int cols_left = static_cast<int>(K - tc * 128ll < 128 ? K - tc * 128ll : 128);
+        const uint32_t* tile = buffers + turn * C::TILE_WORDS;
+
+        // ---- blocks along the rows
+        if (rows_left > 0) {
+            const int b = threadIdx.x % NB;
+            const size_t k2 = tc * 64ull + b * (B / 2);
+            uint8_t* to = codes + (tr * 128ull + threadIdx.x / NB) * pitch + k2;
+            const bool inside = k2 < pitch;
+#pragma unroll
+            for (int j = 0; j < 128 * NB / kTileThreads; j++) {
+                const int r = threadIdx.x / NB + j * (kTileThreads / NB);
+                uint32_t w[BW];
+#pragma unroll
+                for (int i = 0; i < BW; i += 4) *reinterpret_cast<uint4*>(w + i) = *reinterpret_cast<const uint4*>(tile + at(r, b * BW + i));
+                float v[B];
+                unpack<T, B>(w, v);
                 uint32_t c[B / 8];
-                const int col = word * CPW + h;
-                sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT>(v, amax[h], scale, c));
-                const size_t k2 = (r0 + rb * B) / 2;
-                if (c0 + col < K && k2 < pitch) store_codes<B>(codes_t + (c0 + col) * pitch + k2, c);
+                sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(moved)::value>(v, magnitude<T, B>(w), scale, c));
+                if (inside && r < rows_left) store_codes<B>(to + static_cast<size_t>(j * (kTileThreads / NB)) * pitch, c);
             }
         }
-    }
-    __syncthreads();
-    // ---- whole scale tiles
-    constexpr int VECS = NB / 4 * 32;
-    if (threadIdx.x < VECS) {
-        if (r0 < rows) {
-            const int tiles = scale_tiles_per_row(FMT, K);
-            *reinterpret_cast<uint4*>(scales + (tr * tiles + tc * (NB / 4)) * TILE_BYTES + threadIdx.x * 16) = reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+        // ---- blocks along the columns: a warp takes 8 words x 4 row blocks; where that makes fewer tasks than warps, each
+        // of a word's two columns is a task
+        if constexpr (COLS) {
+            constexpr int TASKS = (W / 8) * (NB / 4), SPLIT = TASKS < kTileThreads / 32 ? CPW : 1;
+            const int lane = threadIdx.x & 31, g = lane >> 3;
+#pragma unroll 1
+            for (int i = threadIdx.x >> 5; i < TASKS * SPLIT; i += kTileThreads / 32) {
+                const int task = i % TASKS, h0 = SPLIT > 1 ? i / TASKS : 0;
+                const int word = (task % (W / 8)) * 8 + (lane & 7), rb = (task / (W / 8)) * 4 + g;
+                uint32_t raw[B];
+                const uint32_t* from = tile + at(rb * B, word);
+#pragma unroll
+                for (int j = 0; j < B; j++) raw[j] = from[j * W];
+                uint32_t m = 0;                                     // a word holds two columns: their maxima together
+                if constexpr (CPW == 2) m = halves_magnitude<B>(raw);
+                const size_t k2 = tr * 64ull + rb * (B / 2);
+                uint8_t* to = codes_t + (tc * 128ull + word * CPW) * pitch_t + k2;
+                const bool inside = k2 < pitch_t;
+#pragma unroll
+                for (int h = 0; h < CPW / SPLIT; h++) {
+                    const int half = SPLIT > 1 ? h0 : h, col = word * CPW + half;
+                    uint32_t amax;
+                    if constexpr (CPW == 1) amax = magnitude<T, B>(raw);
+                    else amax = bits_of_half<T>(half ? m >> 16 : m & 0xFFFFu);
+                    float v[B];
+#pragma unroll
+                    for (int j = 0; j < B; j++) {
+                        if constexpr (CPW == 1) v[j] = __uint_as_float(raw[j]);
+                        else if constexpr (std::is_same_v<T, __nv_bfloat16>) v[j] = __uint_as_float(half ? raw[j] & 0xFFFF0000u : raw[j] << 16);
+                        else v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(half ? raw[j] >> 16 : raw[j])));
+                    }
+                    uint32_t c[B / 8];
+                    sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(moved)::value>(v, amax, scale, c));
+                    if (inside && col < cols_left) store_codes<B>(to + (half ? pitch_t : 0), c);
+                }
+            }
         }
-    } else if (COLS && threadIdx.x < 2 * VECS) {
-        if (c0 < K) {
-            const int tiles = scale_tiles_per_row(FMT, rows), i = threadIdx.x - VECS;
-            *reinterpret_cast<uint4*>(scales_t + (tc * tiles + tr * (NB / 4)) * TILE_BYTES + i * 16) = reinterpret_cast<const uint4*>(sc_t)[i];
+        __syncthreads();
+        // ---- whole scale tiles
+        constexpr int VECS = NB / 4 * 32;
+        if (threadIdx.x < VECS) {
+            if (rows_left > 0)
+                *reinterpret_cast<uint4*>(scales + (static_cast<size_t>(tr) * scale_tiles_per_row(FMT, K) + tc * (NB / 4)) * TILE_BYTES + threadIdx.x * 16) =
+                    reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+        } else if (COLS && threadIdx.x < 2 * VECS) {
+            const int i = threadIdx.x - VECS;
+            if (cols_left > 0)
+                *reinterpret_cast<uint4*>(scales_t + (static_cast<size_t>(tc) * scale_tiles_per_row(FMT, rows) + tr * (NB / 4)) * TILE_BYTES + i * 16) =
+                    reinterpret_cast<const uint4*>(sc_t)[i];
         }
     }
+    };
+    if (FMT == RDB_FP4_NVFP4 && scale.move != 1.0f) body(std::true_type());
+    else body(std::false_type());
 }
 
 // Eight codes -> eight halves (exact).
@@ -604,10 +665,10 @@ __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __r
 }
 
 // Every kernel of this file waits for its predecessor before it touches memory: the early start only hides the launch.
-static int launch(const void* kernel, dim3 grid, int smem, void** args, cudaStream_t stream) {
+static int launch(const void* kernel, dim3 grid, int threads, int smem, void** args, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -626,7 +687,7 @@ static dim3 octet_grid(int rows, long long columns) {
 }
 
 template <class T, int FMT, bool COLS>
-static int launch_tiles(int rows, int K, void** args, unsigned* tiles_x, cudaStream_t stream) {
+static int launch_tiles(int rows, int K, void** args, unsigned* tiles_x, unsigned* tiles_all, int sm_count, cudaStream_t stream) {
     using C = TileCfg<T, FMT>;
     static bool attr_set[kMaxDevices] = {};
     int dev = 0;
@@ -641,7 +702,9 @@ static int launch_tiles(int rows, int K, void** args, unsigned* tiles_x, cudaStr
     const long long y = COLS ? (static_cast<long long>(rows) + 255) / 256 * 2 : (static_cast<long long>(rows) + 127) / 128;
     if (x * y > 0x7FFFFFFFll) return RDB_SIZE_ABOVE_LIMIT;
     *tiles_x = static_cast<unsigned>(x);
-    return launch(reinterpret_cast<const void*>(kernel), dim3(static_cast<unsigned>(x * y)), C::SMEM, args, stream);
+    *tiles_all = static_cast<unsigned>(x * y);
+    const unsigned grid = static_cast<unsigned>(sm_count * C::PER_SM);
+    return launch(reinterpret_cast<const void*>(kernel), dim3(*tiles_all < grid ? *tiles_all : grid), kTileThreads, C::SMEM, args, stream);
 }
 
 template <class T, int FMT>
@@ -659,19 +722,19 @@ static int quantize(const void* x_, long long ldx, int rows, int K, float* tscal
         partials = static_cast<int>(blocks < kAmaxBlocks ? blocks : kAmaxBlocks);
         if (partials > info->sm_count * 6) partials = info->sm_count * 6;
         void* args[] = {&x, &ldx, &rows, &K, &partial};
-        const int r = launch(reinterpret_cast<const void*>(amax_kernel<T>), dim3(partials), 0, args, stream);
+        const int r = launch(reinterpret_cast<const void*>(amax_kernel<T>), dim3(partials), kThreads, 0, args, stream);
         if (r != RDB_SUCCESS) return r;
     }
     if (!codes_t && by16 && K % B == 0) {
         void* args[] = {&x, &ldx, &rows, &K, &tscale, &partial, &partials, &codes, &scales};
         const dim3 grid = octet_grid(rows, (4ll * scale_tiles_per_row(FMT, K) + 31) / 32);
         return launch(by32 ? reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT, 32>) : reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT, 16>),
-                      grid, 0, args, stream);
+                      grid, kThreads, 0, args, stream);
     }
     int vec = by16;
-    unsigned tiles_x = 0;
-    void* args[] = {&x, &ldx, &rows, &K, &vec, &tiles_x, &tscale, &partial, &partials, &codes, &scales, &codes_t, &scales_t};
-    return codes_t ? launch_tiles<T, FMT, true>(rows, K, args, &tiles_x, stream) : launch_tiles<T, FMT, false>(rows, K, args, &tiles_x, stream);
+    unsigned tiles_x = 0, tiles_all = 0;
+    void* args[] = {&x, &ldx, &rows, &K, &vec, &tiles_x, &tiles_all, &tscale, &partial, &partials, &codes, &scales, &codes_t, &scales_t};
+    return codes_t ? launch_tiles<T, FMT, true>(rows, K, args, &tiles_x, &tiles_all, info->sm_count, stream) : launch_tiles<T, FMT, false>(rows, K, args, &tiles_x, &tiles_all, info->sm_count, stream);
 }
 
 template <class T>
@@ -680,7 +743,7 @@ static int dequantize(const uint8_t* codes, const uint8_t* scales, const float* 
     int vec = aligned16(out) && K * sizeof(T) % 16 == 0 && K % 8 == 0;
     void* args[] = {&codes, &scales, &tscale, &rows, &K, &vec, &out};
     return launch(format == RDB_FP4_NVFP4 ? reinterpret_cast<const void*>(dequantize_kernel<T, RDB_FP4_NVFP4>) : reinterpret_cast<const void*>(dequantize_kernel<T, RDB_FP4_MXFP4>),
-                  octet_grid(rows, (static_cast<long long>(K) + 255) / 256), 0, args, stream);
+                  octet_grid(rows, (static_cast<long long>(K) + 255) / 256), kThreads, 0, args, stream);
 }
 
 static int check(int type, int rows, int K, int format) {

@@ -289,6 +289,22 @@ def test_quantize_extreme_tensors(cuda_device, form, fill):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t", [1.1754944e-38, 1e-30, 3e-19, 1e-3, 7.0, 2e18, 1e30])
+@pytest.mark.parametrize("size", [1e-36, 1e-20, 1.0, 1e19, 1e37])
+def test_given_tensor_scales_far_from_the_values(cuda_device, dtype, t, size):
+    """Saturated blocks where t is too small, zeros where it is too large."""
+    import rocm_dev_b200 as R
+    g = torch.Generator().manual_seed(4)
+    x = (torch.randn((48, 160), generator=g) * size).to(dtype)
+    x[3], x[:, 7] = 0.0, -0.0
+    ts = torch.tensor([t], dtype=torch.float32)
+    r, c = R.quantize_fp4_both(x.to(cuda_device), "nvfp4", ts.to(cuda_device))
+    check_quantized(r, x.float().numpy(), "nvfp4", ts.item())
+    check_quantized(c, x.float().numpy().T.copy(), "nvfp4", ts.item())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("form", FORMATS)
 @pytest.mark.parametrize("rows,K", [(1, 1), (3, 33), (130, 512), (65, 1001), (16, 4096)])
 def test_dequantize(cuda_device, form, rows, K):
