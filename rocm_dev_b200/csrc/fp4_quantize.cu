@@ -60,13 +60,21 @@ __device__ __forceinline__ void unpack(const uint32_t* w, float* v) {
 }
 
 // Largest magnitude of elements held in words, as fp32 bits: non-negative floats order like integers, infinities and NaNs
-// above every number.  16-bit types are compared two at a time: the halves of the result are the maxima of the halves.
-template <int WORDS>
+// above every number.  16-bit types are compared two at a time: the halves of the result are the maxima of the halves
+// (a NaN wins and stays one).
+template <class T, int WORDS>
 __device__ __forceinline__ uint32_t halves_magnitude(const uint32_t* w) {
-    uint32_t m = w[0] & 0x7FFF7FFFu;
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(w));
 #pragma unroll
-    for (int i = 1; i < WORDS; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
-    return m;
+        for (int i = 1; i < WORDS; i++) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(w + i)));
+        return *reinterpret_cast<const uint32_t*>(&m) & 0x7FFF7FFFu;
+    } else {
+        __half2 m = __habs2(*reinterpret_cast<const __half2*>(w));
+#pragma unroll
+        for (int i = 1; i < WORDS; i++) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(w + i)));
+        return *reinterpret_cast<const uint32_t*>(&m) & 0x7FFF7FFFu;
+    }
 }
 template <class T>
 __device__ __forceinline__ uint32_t bits_of_half(uint32_t h) {
@@ -81,7 +89,7 @@ __device__ __forceinline__ uint32_t magnitude(const uint32_t* w) {
         for (int i = 0; i < N; i++) m = max(m, w[i] & 0x7FFFFFFFu);
         return m;
     } else {
-        const uint32_t m = halves_magnitude<N / 2>(w);
+        const uint32_t m = halves_magnitude<T, N / 2>(w);
         return bits_of_half<T>(max(m & 0xFFFFu, m >> 16));
     }
 }
@@ -157,8 +165,9 @@ __device__ __forceinline__ float neg_reciprocal(float d) {
 template <class T>
 constexpr int kSteps = sizeof(T) == 4 ? 2 : 1;
 
-// One block: v[BLOCK] -> BLOCK / 8 words of codes, returns the scale byte.  MOVED: sc.move is not 1.
-template <class T, int FMT, bool MOVED>
+// One block: v[BLOCK] -> BLOCK / 8 words of codes, returns the scale byte.  CAREFUL: sc.move is not 1, or the tensor scale
+// was given and quotients may overflow.
+template <class T, int FMT, bool CAREFUL>
 __device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, const Scale& sc, uint32_t* codes) {
     constexpr int B = Format<FMT>::BLOCK;
     if constexpr (FMT == RDB_FP4_MXFP4) {
@@ -176,13 +185,14 @@ __device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, const 
         return amax >= kInf ? 0xFF : byte;
     } else {
         float a = __uint_as_float(amax);
-        if constexpr (MOVED) a *= sc.move;
-        const float top = 1024.0f * sc.t6;                           // beyond it everything saturates (given scales only)
-        if (!(a <= top)) {
-            a = top;
-            const float most = MOVED ? top / sc.move : top;
+        if constexpr (CAREFUL) {
+            a *= sc.move;
+            const float top = 1024.0f * sc.t6, most = top / sc.move;     // beyond it everything saturates
+            if (!(a <= top)) {
+                a = top;
 #pragma unroll
-            for (int i = 0; i < B; i++) v[i] = fminf(fmaxf(v[i], -most), most);
+                for (int i = 0; i < B; i++) v[i] = fminf(fmaxf(v[i], -most), most);
+            }
         }
         float n = a * sc.n6;
 #pragma unroll
@@ -193,22 +203,23 @@ __device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, const 
         asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(e));
         const uint32_t byte = e;
         float d = __half2float(__ushort_as_half(static_cast<unsigned short>(h2))) * sc.t;
-        if constexpr (MOVED) d *= sc.move;
+        if constexpr (CAREFUL) d *= sc.move;
         const float ninv = neg_reciprocal<T>(d);
         const Pair d2 = pair(d, d), n2 = pair(ninv, ninv);
+        const uint32_t keep = byte != 0 ? ~0u : 0u;                  // a scale of zero: zeros
 #pragma unroll
         for (int g = 0; g < B / 8; g++) {
             float q[8];
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 Pair x = pair(v[8 * g + i], v[8 * g + i + 1]);
-                if constexpr (MOVED) x = mul2(x, pair(sc.move, sc.move));
+                if constexpr (CAREFUL) x = mul2(x, pair(sc.move, sc.move));
                 Pair y = mul2(x, n2);
 #pragma unroll
                 for (int k = 0; k < kSteps<T>; k++) y = fma2(fma2(y, d2, x), n2, y);
                 split(y, q[i], q[i + 1]);
             }
-            codes[g] = byte != 0 ? pack8(q) ^ 0x88888888u : 0u;      // a scale of zero: zeros
+            codes[g] = (pack8(q) ^ 0x88888888u) & keep;
         }
         return amax >= kInf ? 0x7F : byte;
     }
@@ -314,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     const int tiles = scale_tiles_per_row(FMT, K);
     const int lane = threadIdx.x & 31, b = blockIdx.x * 32 + lane, blocks = K / B;
     const int octets = static_cast<int>((rows + 127ll) / 128 * 4);
-    auto body = [&](auto moved) {
+    auto body = [&](auto careful) {
         for (int o = blockIdx.y; o < octets; o += gridDim.y) {
             const int r0 = (o >> 2) * 128 + (o & 3) * 8 + (threadIdx.x >> 5);
             if (r0 >= rows) continue;
@@ -346,7 +357,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
                     float v[B];
                     unpack<T, B>(w[j], v);
                     uint32_t c[B / 8];
-                    byte[h + j] = encode_block<T, FMT, decltype(moved)::value>(v, magnitude<T, B>(w[j]), scale, c);
+                    byte[h + j] = encode_block<T, FMT, decltype(careful)::value>(v, magnitude<T, B>(w[j]), scale, c);
                     if (static_cast<size_t>(b) * (B / 2) < pitch) store_codes<B>(codes + r * pitch + static_cast<size_t>(b) * (B / 2), c);
                 }
             }
@@ -361,7 +372,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
                 *reinterpret_cast<uint4*>(scales + scale_word(r0, b >> 2, tiles)) = make_uint4(word[0], word[1], word[2], word[3]);
         }
     };
-    if (FMT == RDB_FP4_NVFP4 && scale.move != 1.0f) body(std::true_type());
+    if (FMT == RDB_FP4_NVFP4 && (scale.move != 1.0f || !partial)) body(std::true_type());
     else body(std::false_type());
 }
 
@@ -471,7 +482,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
     int ntr = tr, ntc = tc, turn = 0;
     fetch(tr, tc, buffers);
     const Scale scale = fetch_scale<T, FMT, kTileThreads>(tscale, partial, partials);
-    auto body = [&](auto moved) {
+    auto body = [&](auto careful) {
     for (unsigned n = blockIdx.x; n < tiles_all; n += gridDim.x, turn ^= 1, tr = ntr, tc = ntc) {
         if (n + gridDim.x < tiles_all) {
             advance(ntr, ntc);
@@ -500,7 +511,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
                 float v[B];
                 unpack<T, B>(w, v);
                 uint32_t c[B / 8];
-                sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(moved)::value>(v, magnitude<T, B>(w), scale, c));
+                sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(careful)::value>(v, magnitude<T, B>(w), scale, c));
                 if (inside && r < rows_left) store_codes<B>(to + static_cast<size_t>(j * (kTileThreads / NB)) * pitch, c);
             }
         }
@@ -518,7 +529,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
 #pragma unroll
                 for (int j = 0; j < B; j++) raw[j] = from[j * W];
                 uint32_t m = 0;                                     // a word holds two columns: their maxima together
-                if constexpr (CPW == 2) m = halves_magnitude<B>(raw);
+                if constexpr (CPW == 2) m = halves_magnitude<T, B>(raw);
                 const size_t k2 = tr * 64ull + rb * (B / 2);
                 uint8_t* to = codes_t + (tc * 128ull + word * CPW) * pitch_t + k2;
                 const bool inside = k2 < pitch_t;
@@ -536,7 +547,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
                         else v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(half ? raw[j] >> 16 : raw[j])));
                     }
                     uint32_t c[B / 8];
-                    sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(moved)::value>(v, amax, scale, c));
+                    sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(careful)::value>(v, amax, scale, c));
                     if (inside && col < cols_left) store_codes<B>(to + (half ? pitch_t : 0), c);
                 }
             }
@@ -556,7 +567,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
         }
     }
     };
-    if (FMT == RDB_FP4_NVFP4 && scale.move != 1.0f) body(std::true_type());
+    if (FMT == RDB_FP4_NVFP4 && (scale.move != 1.0f || !partial)) body(std::true_type());
     else body(std::false_type());
 }
 
@@ -727,7 +738,12 @@ static int quantize(const void* x_, long long ldx, int rows, int K, float* tscal
     }
     if (!codes_t && by16 && K % B == 0) {
         void* args[] = {&x, &ldx, &rows, &K, &tscale, &partial, &partials, &codes, &scales};
-        const dim3 grid = octet_grid(rows, (4ll * scale_tiles_per_row(FMT, K) + 31) / 32);
+        dim3 grid = octet_grid(rows, (4ll * scale_tiles_per_row(FMT, K) + 31) / 32);
+        // what a block does once (the partial maxima) is shared by several octets where there are blocks enough: 16 per SM
+        if (partial) {
+            const unsigned enough = (16u * info->sm_count + grid.x - 1) / grid.x;
+            if (grid.y > 2 * enough) grid.y = enough;
+        }
         return launch(by32 ? reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT, 32>) : reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT, 16>),
                       grid, kThreads, 0, args, stream);
     }
