@@ -12,8 +12,6 @@ along the rows and ``c`` the one along the columns
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
-
 import torch
 
 from ._lib import check, lib
@@ -23,30 +21,10 @@ BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 WORKSPACE_FLOATS = 1024
 
-
-class Fp4Tensor(NamedTuple):
-    """A held tensor [rows, K]: ``codes`` uint8 [rows, ceil(K / 32) * 16], ``scales`` uint8 in tiles (flat),
-    ``tensor_scale`` fp32[1] (``nvfp4``) or None."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    tensor_scale: Optional[torch.Tensor]
-    format: str
-    rows: int
-    K: int
-
-
-def _format(name: str) -> int:
-    try:
-        return FORMATS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"format must be one of {sorted(FORMATS)}, got {name!r}") from None
-
-
-def _type(dtype: torch.dtype) -> int:
-    try:
-        return _TYPES[dtype]
-    except KeyError:
-        raise TypeError(f"bfloat16, float16 or float32 expected, got {dtype}") from None
+# A step's calls are short: what a call costs on the host shows.  These two are the cheap forms of
+# torch.cuda.current_device() and torch.cuda.current_stream(dev).cuda_stream (0.1 us each instead of 0.2 and 2.2).
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def scale_bytes(format: str, rows: int, K: int) -> int:
@@ -55,122 +33,190 @@ def scale_bytes(format: str, rows: int, K: int) -> int:
 
 
 def row_bytes(K: int) -> int:
+    """Bytes of a row of codes."""
     return (K + 31) // 32 * 16
 
 
-class _on:
-    """``with torch.cuda.device(dev)``, at no cost where it is the current device already."""
-    __slots__ = ("dev", "prev")
-
-    def __init__(self, dev):
-        self.dev = dev.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.prev)
+def _format(name: str) -> int:
+    fmt = FORMATS.get(name) if isinstance(name, str) else None
+    if fmt is None:
+        raise ValueError(f"format must be one of {sorted(FORMATS)}, got {name!r}")
+    return fmt
 
 
-def _empty(format: str, rows: int, K: int, tensor_scale, dev) -> Fp4Tensor:
-    return Fp4Tensor(torch.empty((rows, row_bytes(K)), dtype=torch.uint8, device=dev),
-                     torch.empty(scale_bytes(format, rows, K), dtype=torch.uint8, device=dev), tensor_scale, format, rows, K)
+def _type(dtype: torch.dtype) -> int:
+    typ = _TYPES.get(dtype)
+    if typ is None:
+        raise TypeError(f"bfloat16, float16 or float32 expected, got {dtype}")
+    return typ
 
 
-def _quantize(x: torch.Tensor, format: str, tensor_scale, along_rows: bool, along_columns: bool):
+class Fp4Tensor:
+    """A held tensor [rows, K]: ``codes`` uint8 [rows, row_bytes(K)], ``scales`` uint8 in tiles (flat, scale_bytes(format,
+    rows, K)), ``tensor_scale`` fp32[1] (``nvfp4``) or None, all on ``device``."""
+    __slots__ = ("format", "rows", "K", "device", "_fmt", "_args", "_parts", "_buffer")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, tensor_scale, format: str, rows: int, K: int):
+        fmt = _format(format)
+        dev = codes.device
+        if not (codes.dtype is torch.uint8 and codes.shape == (rows, (K + 31) // 32 * 16) and codes.is_contiguous()):
+            raise ValueError(f"codes must be contiguous uint8 [{rows}, {row_bytes(K)}]")
+        if not (scales.dtype is torch.uint8 and scales.numel() == scale_bytes(format, rows, K) and scales.is_contiguous()
+                and scales.device == dev):
+            raise ValueError(f"scales must be {scale_bytes(format, rows, K)} contiguous bytes on {dev}")
+        if fmt == 0:
+            if tensor_scale is not None:
+                raise ValueError("mxfp4 has no tensor scale")
+            self._args = (codes.data_ptr(), scales.data_ptr(), None)
+        else:
+            if not (tensor_scale is not None and tensor_scale.dtype is torch.float32 and tensor_scale.numel() == 1
+                    and tensor_scale.device == dev):
+                raise ValueError(f"nvfp4 needs a tensor scale: one fp32 on {dev}")
+            self._args = (codes.data_ptr(), scales.data_ptr(), tensor_scale.data_ptr())
+        self._parts = (codes, scales, tensor_scale)
+        self.format, self.rows, self.K, self.device, self._fmt = format, rows, K, dev, fmt
+
+    def _views(self):
+        # a quantiser's result is one allocation (codes, scales, tensor scale at the addresses in _args); its tensors are
+        # made when they are asked for
+        if self._parts is None:
+            buf, given = self._buffer
+            base = buf.data_ptr()
+            codes, scales, ts = self._args
+            rb, sb = row_bytes(self.K), scale_bytes(self.format, self.rows, self.K)
+            part = lambda at, n: buf[at - base:at - base + n]  # noqa: E731
+            self._parts = (part(codes, self.rows * rb).view(self.rows, rb), part(scales, sb),
+                           given if ts is None or given is not None else part(ts, 4).view(torch.float32))
+        return self._parts
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._views()[0]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._views()[1]
+
+    @property
+    def tensor_scale(self):
+        return self._views()[2]
+
+    def to(self, device) -> "Fp4Tensor":
+        """The same tensor on another device (or on the host, to be stored)."""
+        move = lambda t: None if t is None else t.to(device)  # noqa: E731
+        return Fp4Tensor(move(self.codes), move(self.scales), move(self.tensor_scale), self.format, self.rows, self.K)
+
+    def __repr__(self) -> str:
+        return f"Fp4Tensor({self.format}, [{self.rows}, {self.K}], {self.device})"
+
+
+def _device(dev: torch.device) -> int:
+    if dev.type != "cuda":
+        raise ValueError(f"device tensors required, got one on {dev} (there is no CPU path)")
+    return dev.index
+
+
+def _call(fn, where: str, dev: int, *args) -> None:
+    """fn(*args, the current stream of device dev), with dev as the current device."""
+    prev = _current_device()
+    if prev == dev:
+        code = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, _raw_stream(dev))
+    if code:
+        check(code, where)
+
+
+def _held(form: str, fmt: int, rows: int, K: int, dev, buffer, at: int, scales: int, scale_ptr) -> Fp4Tensor:
+    t = Fp4Tensor.__new__(Fp4Tensor)
+    t.format, t.rows, t.K, t.device, t._fmt = form, rows, K, dev, fmt
+    t._args, t._parts, t._buffer = (at, scales, scale_ptr), None, buffer
+    return t
+
+
+def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
     fmt, typ = _format(format), _type(x.dtype)
-    assert x.is_cuda and x.dim() == 2, "a 2-D device tensor is required (there is no CPU path)"
+    dev = x.device
+    index = _device(dev)
+    if x.dim() != 2:
+        raise ValueError(f"a 2-D tensor is required, got {tuple(x.shape)}")
     rows, K = x.shape
     if rows < 1 or K < 1:
         raise ValueError(f"an empty tensor cannot be quantised: {tuple(x.shape)}")
-    if x.stride(1) != 1 and K > 1 or x.stride(0) < K and rows > 1:
+    ldx, unit = x.stride()
+    if unit != 1 and K > 1 or ldx < K and rows > 1:
         x = x.contiguous()                        # transposed or overlapping views
-    ldx = x.stride(0) if rows > 1 else K
-    dev = x.device
+        ldx = K
+    elif rows == 1:
+        ldx = K
     given = tensor_scale is not None
-    work = None
-    if fmt == 0:
-        assert not given, "mxfp4 has no tensor scale"
-    elif given:
-        assert tensor_scale.device == dev and tensor_scale.dtype == torch.float32 and tensor_scale.numel() == 1
-    else:
-        tensor_scale = torch.empty(1, dtype=torch.float32, device=dev)
-        work = torch.empty(WORKSPACE_FLOATS, dtype=torch.float32, device=dev)
-    r = _empty(format, rows, K, tensor_scale, dev) if along_rows else None
-    c = _empty(format, K, rows, tensor_scale, dev) if along_columns else None
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with _on(dev):
-        check(lib().rdb_quantize_fp4(x.data_ptr(), typ, ldx, rows, K, fmt, p(tensor_scale), given, p(r and r.codes),
-                                     p(r and r.scales), p(c and c.codes), p(c and c.scales), p(work),
-                                     torch.cuda.current_stream(dev).cuda_stream), "rdb_quantize_fp4")
-    return r, c
+    if given:
+        if fmt == 0:
+            raise ValueError("mxfp4 has no tensor scale")
+        if not (tensor_scale.dtype is torch.float32 and tensor_scale.numel() == 1 and tensor_scale.device == dev):
+            raise ValueError(f"the tensor scale must be one fp32 on {dev}")
+    # one allocation (every part a multiple of 16 bytes): codes and scales of either direction, the tensor scale, and the
+    # scratch that the call alone uses
+    codes, scales = rows * ((K + 31) // 32 * 16), scale_bytes(format, rows, K)
+    codes_t, scales_t = (K * ((rows + 31) // 32 * 16), scale_bytes(format, K, rows)) if both else (0, 0)
+    own_scale = fmt == 1 and not given
+    buffer = torch.empty(codes + scales + codes_t + scales_t + (16 + 4 * WORKSPACE_FLOATS if own_scale else 0), dtype=torch.uint8, device=dev)
+    at = buffer.data_ptr()
+    at_s, at_ct = at + codes, at + codes + scales
+    at_st, end = at_ct + codes_t, at_ct + codes_t + scales_t
+    scale_ptr = end if own_scale else tensor_scale.data_ptr() if given else None
+    _call(lib().rdb_quantize_fp4, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, scale_ptr, given, at, at_s,
+          at_ct if both else None, at_st if both else None, end + 16 if own_scale else None)
+    held = (buffer, tensor_scale)
+    return (_held(format, fmt, rows, K, dev, held, at, at_s, scale_ptr),
+            _held(format, fmt, K, rows, dev, held, at_ct, at_st, scale_ptr) if both else None)
 
 
 def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None) -> Fp4Tensor:
     """x [rows, K] (bf16, fp16 or fp32; rows may be a pitch apart) -> held form, blocks along the rows.
     ``tensor_scale`` (``nvfp4``): a positive fp32[1] to use in place of max|x| / 2688 - a calibrated one, for which x is
     read once instead of twice."""
-    return _quantize(x, format, tensor_scale, True, False)[0]
+    return _quantize(x, format, tensor_scale, False)[0]
 
 
 def quantize_fp4_both(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None):
     """(held form of x, held form of its transpose [K, rows] with blocks along x's columns), one tensor scale for both."""
-    return _quantize(x, format, tensor_scale, True, True)
-
-
-def _checked(t: Fp4Tensor) -> int:
-    fmt = _format(t.format)
-    codes, scales, ts = t.codes, t.scales, t.tensor_scale
-    assert codes.is_cuda and codes.dtype == torch.uint8 and codes.shape == (t.rows, row_bytes(t.K)) and codes.is_contiguous()
-    assert scales.device == codes.device and scales.dtype == torch.uint8 and scales.is_contiguous() and \
-        scales.numel() == scale_bytes(t.format, t.rows, t.K)
-    if fmt == 0:
-        assert ts is None, "mxfp4 has no tensor scale"
-    else:
-        assert ts is not None and ts.device == codes.device and ts.dtype == torch.float32 and ts.numel() == 1
-    return fmt
+    return _quantize(x, format, tensor_scale, True)
 
 
 def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that codes and scales stand for, [rows, K] of ``dtype``."""
-    fmt, typ = _checked(t), _type(dtype)
-    dev = t.codes.device
-    out = torch.empty((t.rows, t.K), dtype=dtype, device=dev)
-    with _on(dev):
-        check(lib().rdb_dequantize_fp4(t.codes.data_ptr(), t.scales.data_ptr(), t.tensor_scale.data_ptr() if fmt else None, fmt,
-                                       t.rows, t.K, out.data_ptr(), typ, torch.cuda.current_stream(dev).cuda_stream),
-              "rdb_dequantize_fp4")
+    typ, index = _type(dtype), _device(t.device)
+    out = torch.empty(t.rows, t.K, dtype=dtype, device=t.device)
+    codes, scales, ts = t._args
+    _call(lib().rdb_dequantize_fp4, "rdb_dequantize_fp4", index, codes, scales, ts, t._fmt, t.rows, t.K, out.data_ptr(), typ)
     return out
 
 
 def _product(A: Fp4Tensor, B: Fp4Tensor, out, out_dtype):
-    fmt = _checked(A)
-    if B.format != A.format or B.K != A.K:
-        raise ValueError(f"operands of one format and depth are required: {A.format} K={A.K}, {B.format} K={B.K}")
-    _checked(B)
-    dev = A.codes.device
-    assert B.codes.device == dev
+    dev = A.device
+    index = _device(dev)
+    if B._fmt != A._fmt or B.K != A.K:
+        raise ValueError(f"operands of one format and depth are required: {A!r}, {B!r}")
+    if B.device != dev:
+        raise ValueError(f"operands on one device are required: {A!r}, {B!r}")
     if out is None:
         typ = _type(out_dtype)
-        out = torch.empty((A.rows, B.rows), dtype=out_dtype, device=dev)
+        out = torch.empty(A.rows, B.rows, dtype=out_dtype, device=dev)
     else:
         typ = _type(out.dtype)
-        assert out.device == dev and out.is_contiguous() and out.shape == (A.rows, B.rows)
-    return (A.codes.data_ptr(), A.scales.data_ptr(), A.tensor_scale.data_ptr() if fmt else None, B.codes.data_ptr(),
-            B.scales.data_ptr(), B.tensor_scale.data_ptr() if fmt else None, out.data_ptr(), typ, A.rows, B.rows, A.K, fmt), out, dev
+        if not (out.device == dev and out.is_contiguous() and out.shape == (A.rows, B.rows)):
+            raise ValueError(f"out must be contiguous [{A.rows}, {B.rows}] on {dev}")
+    return (*A._args, *B._args, out.data_ptr(), typ, A.rows, B.rows, A.K, A._fmt), out, index
 
 
 def dense_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
                    out_dtype: torch.dtype = torch.bfloat16, tiling: int = 0, max_ctas: int = 0) -> torch.Tensor:
     """D[M,N] = A . B^T over the values of A [M,K] and B [N,K], any sizes; fp32 accumulation, rounded once to
     ``out_dtype`` (``out``'s type where it is given).  ``tiling``, ``max_ctas``: the tuner's knobs, 0 = automatic."""
-    args, out, dev = _product(A, B, out, out_dtype)
-    with _on(dev):
-        check(lib().rdb_dense_gemm_fp4_tuned(*args, tiling, max_ctas, torch.cuda.current_stream(dev).cuda_stream),
-              "rdb_dense_gemm_fp4")
+    args, out, index = _product(A, B, out, out_dtype)
+    _call(lib().rdb_dense_gemm_fp4_tuned, "rdb_dense_gemm_fp4", index, *args, tiling, max_ctas)
     return out
 
 
@@ -178,9 +224,8 @@ def skinny_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
                     flags: int = 0) -> torch.Tensor:
     """The same product for at most 32 rows of A (decode): a stream over B.  ``flags``: 0 or ``OVERLAP_PRIOR_KERNEL`` (the
     launch may request B while the preceding kernel of the stream drains; that kernel must not write B)."""
-    args, out, dev = _product(A, B, out, out_dtype)
-    with _on(dev):
-        check(lib().rdb_skinny_gemm_fp4(*args, flags, torch.cuda.current_stream(dev).cuda_stream), "rdb_skinny_gemm_fp4")
+    args, out, index = _product(A, B, out, out_dtype)
+    _call(lib().rdb_skinny_gemm_fp4, "rdb_skinny_gemm_fp4", index, *args, flags)
     return out
 
 

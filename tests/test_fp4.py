@@ -146,8 +146,11 @@ def test_scale_tiles_round_trip():
     import rocm_dev_b200 as R
     for f, rows, K in [("mxfp4", 130, 700), ("nvfp4", 1, 16), ("nvfp4", 300, 1030)]:
         s = torch.randint(0, 255, (rows, -(-K // BLOCK[f])), dtype=torch.uint8)
-        t = R.Fp4Tensor(None, R.pack_fp4_scales(s, f, K), None, f, rows, K)
+        codes, ts = torch.zeros((rows, -(-K // 32) * 16), dtype=torch.uint8), None if f == "mxfp4" else torch.ones(1)
+        t = R.Fp4Tensor(codes, R.pack_fp4_scales(s, f, K), ts, f, rows, K)
         assert torch.equal(R.unpack_fp4_scales(t), s)
+        back = t.to("cpu")
+        assert (back.format, back.rows, back.K) == (f, rows, K) and torch.equal(back.scales, t.scales)
 
 
 def test_refusals_before_anything_is_launched():
@@ -184,8 +187,19 @@ def test_refusals_of_the_python_face():
         R.quantize_fp4(x, "fp4")
     with pytest.raises(TypeError):
         R.quantize_fp4(x.double())
-    with pytest.raises(AssertionError):
-        R.quantize_fp4(x)                                            # there is no CPU path
+    for bad in (x, x[0], torch.zeros(0, 4)):
+        with pytest.raises(ValueError):
+            R.quantize_fp4(bad)                                      # there is no CPU path
+    codes, scales, one = torch.zeros((4, 32), dtype=torch.uint8), torch.zeros(2048, dtype=torch.uint8), torch.ones(1)
+    t = R.Fp4Tensor(codes, scales, one, "nvfp4", 4, 64)
+    for bad in [(codes, scales, None, "nvfp4", 4, 64), (codes, scales, one, "mxfp4", 4, 64), (codes, scales[:-1], one, "nvfp4", 4, 64),
+                (codes, scales, one.double(), "nvfp4", 4, 64), (codes, scales, one, "nvfp4", 4, 65), (codes, scales, one, "nvfp4", 5, 64),
+                (codes.int(), scales, one, "nvfp4", 4, 64), (codes.t(), scales, one, "nvfp4", 32, 8), (codes, scales, one, "e2m1", 4, 64)]:
+        with pytest.raises(ValueError):
+            R.Fp4Tensor(*bad)
+    for call in (lambda: R.dequantize_fp4(t), lambda: R.dense_gemm_fp4(t, t), lambda: R.skinny_gemm_fp4(t, t)):
+        with pytest.raises(ValueError):
+            call()
 
 
 # ------------------------------------------------------------------ quantisers
