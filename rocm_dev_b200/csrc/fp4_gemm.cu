@@ -493,28 +493,47 @@ static SplitPlan split_plan(int format, int M, int N, int K, int sm_count, int r
     SplitPlan best = {};
     best.mbox = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const int rows = M < 128 ? M : 128;
-    double best_cost = 1e30;
-    for (int R = 64; R <= 256; R += 64) {
-        if (r_hint > 0 && R != r_hint) continue;
-        const int b_tiles = (R + 127) / 128;
-        const double stage = (best.mbox + R) * 128.0 + tiles * TILE_BYTES * (1 + b_tiles);
-        for (int S = 1; S <= 8; S++) {
-            if ((s_hint > 0 && S != (s_hint < num_kb ? s_hint : num_kb)) || (S > 1 && S > num_kb)) continue;
-            const long long clusters = static_cast<long long>((N + R - 1) / R) * m_tiles;
-            int fit = resident[S] * sm_count / 148;
-            if (fit < 1) fit = 1;
-            const long long waves = (clusters + fit - 1) / fit;
-            const int kb = (num_kb + S - 1) / S;
-            // one SM takes ~60 GB/s through TMA, a stage of four MMAs and its hand-over ~360 ns, the chip ~6.3 TB/s;
-            // the epilogue ~25 ps a value (shared-memory round trip), a split ~0.7 us
-            const double t_load = kb * (stage / 60e9 > 360e-9 ? stage / 60e9 : 360e-9);
-            const double t_chip = static_cast<double>(clusters) * S * kb * stage / 6.3e12 / waves;
-            const double c = waves * ((t_load > t_chip ? t_load : t_chip) + 1.5e-6 + 25e-12 * rows * R / S + (S > 1 ? 0.7e-6 : 0.0));
-            if (c < best_cost) { best_cost = c; best.R = R; best.S = S; }
+    int stage_cap = MAX_STAGES;
+    if (M <= 32 && r_hint == 0 && s_hint == 0) {
+        // A stream over B.  128 columns and four stages leave room for a second CTA on every SM, which may belong to the
+        // next launch: 28672 x 4096 at M = 16 takes 14.6 us, with one CTA of 256 columns 15.6.  K is cut as often as the
+        // clusters are all resident two to an SM: 8192 x 8192 takes 18.5 us uncut, 9.5 cut in four (64 clusters of at
+        // most 66), 15.9 cut in five.  A long K may overflow that a little (4096 x 14336: 9.4 us cut in seven, 10.3 in
+        // six); a short one is not cut below two stages a CTA (2048 x 2048: 4.5 us in four, 4.9 in eight).
+        best.R = N <= 64 ? 64 : 128;
+        best.S = 1;
+        stage_cap = 4;
+        const int n_tiles = (N + best.R - 1) / best.R;
+        for (int S = 2; S <= 8 && S <= (num_kb < 8 ? 4 : num_kb / 2) && S <= num_kb; S++) {
+            int fit = 2 * resident[S] * sm_count / 148;
+            if (num_kb >= 6 * S) fit += fit / 14;
+            if (n_tiles <= fit) best.S = S;
+        }
+    } else {
+        double best_cost = 1e30;
+        for (int R = 64; R <= 256; R += 64) {
+            if (r_hint > 0 && R != r_hint) continue;
+            const int b_tiles = (R + 127) / 128;
+            const double stage = (best.mbox + R) * 128.0 + tiles * TILE_BYTES * (1 + b_tiles);
+            for (int S = 1; S <= 8; S++) {
+                if ((s_hint > 0 && S != (s_hint < num_kb ? s_hint : num_kb)) || (S > 1 && S > num_kb)) continue;
+                const long long clusters = static_cast<long long>((N + R - 1) / R) * m_tiles;
+                int fit = resident[S] * sm_count / 148;
+                if (fit < 1) fit = 1;
+                const long long waves = (clusters + fit - 1) / fit;
+                const int kb = (num_kb + S - 1) / S;
+                // one SM takes ~60 GB/s through TMA, a stage of four MMAs and its hand-over ~360 ns, the chip ~6.3 TB/s;
+                // the epilogue ~25 ps a value (shared-memory round trip), a split ~0.7 us
+                const double t_load = kb * (stage / 60e9 > 360e-9 ? stage / 60e9 : 360e-9);
+                const double t_chip = static_cast<double>(clusters) * S * kb * stage / 6.3e12 / waves;
+                const double c = waves * ((t_load > t_chip ? t_load : t_chip) + 1.5e-6 + 25e-12 * rows * R / S + (S > 1 ? 0.7e-6 : 0.0));
+                if (c < best_cost) { best_cost = c; best.R = R; best.S = S; }
+            }
         }
     }
     best.b_tiles = (best.R + 127) / 128;
     best.stages = ring_limit(format, best.mbox, best.R, best.b_tiles);
+    if (best.stages > stage_cap) best.stages = stage_cap;
     if (stages_hint > 0 && stages_hint < best.stages) best.stages = stages_hint;
     const int kb = (num_kb + best.S - 1) / best.S;
     if (best.stages > kb) best.stages = kb;
