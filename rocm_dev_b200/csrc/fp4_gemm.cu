@@ -24,7 +24,7 @@ namespace fp4 {
 
 constexpr int SMEM_LIMIT = 232448;         // 227 KiB opt-in maximum per CTA
 constexpr int MAX_STAGES = 8;
-constexpr int SPLIT_THREADS = 192;
+constexpr int SPLIT_THREADS = 256;
 constexpr int A_OPERAND_SPAN = 128 * 128;  // bytes the MMA reads for its 128-row A operand, whatever was loaded
 
 struct SplitParams {
@@ -161,7 +161,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     }
 
     // ---- the accumulator goes to shared memory, stg[row][R], over the drained ring.  A warp reads the TMEM lane quadrant
-    // warp % 4 (32 rows); warps 4 and 5 share quadrants 0 and 1 with warps 0 and 1.
+    // warp % 4 (32 rows), every second 32 columns of it.
     float* stg = reinterpret_cast<float*>(smem);
     const int pitch = R + 4;
     const int quad = warp & 3;
@@ -172,9 +172,8 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         if (ok && *abort_flag == 0) {
             float* row = stg + (quad * 32 + lane) * pitch;
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
-            const int step = quad < 2 ? 64 : 32;
 #pragma unroll 1
-            for (int c0 = warp >= 4 ? 32 : 0; c0 < R; c0 += step) {
+            for (int c0 = warp >= 4 ? 32 : 0; c0 < R; c0 += 64) {
                 float v[32];
                 tmem_ld32(taddr + c0, v);
 #pragma unroll
@@ -199,17 +198,22 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             if (n0 + c < p.N) {
                 const float* mine = stg + m * pitch + c;
                 if (S == 1) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) v[j] = mine[j];
+                    const float4 x = *reinterpret_cast<const float4*>(mine);
+                    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
                 } else {
                     const uint32_t at = smem_u32(mine);
-                    for (int src = 0; src < S; src++) {
-                        float x[4];
-                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(mapa_smem(at, src)) : "memory");
+                    float x[8][4];                           // all ranks' loads in flight together, then summed in order
 #pragma unroll
-                        for (int j = 0; j < 4; j++) v[j] += x[j];
-                    }
+                    for (int src = 0; src < 8; src++)
+                        if (src < S)
+                            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(x[src][0]), "=f"(x[src][1]), "=f"(x[src][2]), "=f"(x[src][3]) : "r"(mapa_smem(at, src)) : "memory");
+#pragma unroll
+                    for (int src = 0; src < 8; src++)
+                        if (src < S) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) v[j] += x[src][j];
+                        }
                 }
 #pragma unroll
                 for (int j = 0; j < 4; j++) v[j] *= alpha;
@@ -395,8 +399,17 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         // row, no bank conflicts), then one copy out.  A thread holds a row: its own stores would touch 32 lines each.
         auto put = [&](int m0, int n, const float* v) {
             if (m0 >= p.M || n >= p.N) return;
-            if (!p.tma_out) {
-                if (m0 + lane < p.M) store32(p.D, p.out_type, p.N, m0 + lane, n, v, alpha);
+            if (!p.tma_out) {                            // rows of D off 16 bytes: neighbouring lanes store neighbouring columns
+                float* mine = reinterpret_cast<float*>(out) + lane * 33;
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 32; j++) mine[j] = v[j] * alpha;
+                __syncwarp();
+                const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
+                if (n + lane < static_cast<int>(p.N)) {
+#pragma unroll 8
+                    for (int r = 0; r < rows; r++) store1(p.D, p.out_type, static_cast<size_t>(m0 + r) * p.N + n + lane, reinterpret_cast<float*>(out)[r * 33 + lane]);
+                }
                 return;
             }
             uint8_t* buf = out + (turn & 1) * pairs::OUT_BYTES;

@@ -96,23 +96,10 @@ __device__ __forceinline__ uint32_t pack2(int type, float x, float y) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 32 consecutive outputs of row m from column n on, element by element.
-__device__ __forceinline__ void store32(void* D, int type, size_t N, int m, int n, const float* v, float alpha) {
-    const size_t at = static_cast<size_t>(m) * N + n;
-    if (type == RDB_TYPE_FP32) {
-        float* p = reinterpret_cast<float*>(D) + at;
-#pragma unroll
-        for (int j = 0; j < 32; j++)
-            if (n + j < N) p[j] = v[j] * alpha;
-    } else {
-        uint16_t* p = reinterpret_cast<uint16_t*>(D) + at;
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-            const uint32_t w = pack2(type, v[j] * alpha, v[j + 1] * alpha);
-            if (n + j < N) p[j] = static_cast<uint16_t>(w);
-            if (n + j + 1 < N) p[j + 1] = static_cast<uint16_t>(w >> 16);
-        }
-    }
+__device__ __forceinline__ void store1(void* D, int type, size_t at, float v) {
+    if (type == RDB_TYPE_FP32) reinterpret_cast<float*>(D)[at] = v;
+    else if (type == RDB_TYPE_BF16) reinterpret_cast<__nv_bfloat16*>(D)[at] = __float2bfloat16_rn(v);
+    else reinterpret_cast<__half*>(D)[at] = __float2half_rn(v);
 }
 
 // Four consecutive outputs of row m at column n, rounded once; vec: 4 outputs can be stored at once.
