@@ -497,7 +497,7 @@ static int ring_limit(int format, int mbox, int R, int b_tiles) {
     return st < MAX_STAGES ? st : MAX_STAGES;
 }
 
-// Tile width and K split of the least estimated time; 0 hints mean free choice.
+// Tile width and K split; 0 hints mean free choice.  Times are device times on 148 SMs, weights from HBM.
 static SplitPlan split_plan(int format, int M, int N, int K, int sm_count, int r_hint, int s_hint, int stages_hint) {
     // clusters of 1..8 CTAs that are resident at once on 148 SMs (measured)
     static const int resident[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
@@ -506,43 +506,38 @@ static SplitPlan split_plan(int format, int M, int N, int K, int sm_count, int r
     SplitPlan best = {};
     best.mbox = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
     const int rows = M < 128 ? M : 128;
+    auto tiles_of = [&](int R) { return static_cast<long long>((N + R - 1) / R) * m_tiles; };
     int stage_cap = MAX_STAGES;
-    if (M <= 32 && r_hint == 0 && s_hint == 0) {
+    best.R = 128;
+    best.S = 1;
+    if (r_hint > 0 || s_hint > 0) {
+        if (r_hint > 0) best.R = r_hint;
+        if (s_hint > 0) best.S = s_hint < num_kb ? s_hint : num_kb;
+    } else if (M <= 32) {
         // A stream over B.  128 columns and four stages leave room for a second CTA on every SM, which may belong to the
         // next launch: 28672 x 4096 at M = 16 takes 14.6 us, with one CTA of 256 columns 15.6.  K is cut as often as the
         // clusters are all resident two to an SM: 8192 x 8192 takes 18.5 us uncut, 9.5 cut in four (64 clusters of at
         // most 66), 15.9 cut in five.  A long K may overflow that a little (4096 x 14336: 9.4 us cut in seven, 10.3 in
         // six); a short one is not cut below two stages a CTA (2048 x 2048: 4.5 us in four, 4.9 in eight).
-        best.R = N <= 64 ? 64 : 128;
-        best.S = 1;
+        if (N <= 64) best.R = 64;
         stage_cap = 4;
-        const int n_tiles = (N + best.R - 1) / best.R;
         for (int S = 2; S <= 8 && S <= (num_kb < 8 ? 4 : num_kb / 2) && S <= num_kb; S++) {
             int fit = 2 * resident[S] * sm_count / 148;
             if (num_kb >= 6 * S) fit += fit / 14;
-            if (n_tiles <= fit) best.S = S;
+            if (tiles_of(best.R) <= fit) best.S = S;
+        }
+    } else if (tiles_of(128) <= sm_count) {
+        // One CTA to an SM: K is cut to fill the SMs, down to four stages a CTA (128 x 4096 x 4096: 8.5 us in four, 9.2 in
+        // two); a short K is not cut, tiles are narrower instead (1024^3: 5.5 us with 64 columns, 6.5 with 128).
+        best.S = static_cast<int>(sm_count / tiles_of(128));
+        if (best.S > num_kb / 4) best.S = num_kb / 4;
+        if (best.S > 8) best.S = 8;
+        if (best.S <= 1) {
+            best.S = 1;
+            if (num_kb <= 8 && tiles_of(64) <= sm_count) best.R = 64;
         }
     } else {
-        double best_cost = 1e30;
-        for (int R = 64; R <= 256; R += 64) {
-            if (r_hint > 0 && R != r_hint) continue;
-            const int b_tiles = (R + 127) / 128;
-            const double stage = (best.mbox + R) * 128.0 + tiles * TILE_BYTES * (1 + b_tiles);
-            for (int S = 1; S <= 8; S++) {
-                if ((s_hint > 0 && S != (s_hint < num_kb ? s_hint : num_kb)) || (S > 1 && S > num_kb)) continue;
-                const long long clusters = static_cast<long long>((N + R - 1) / R) * m_tiles;
-                int fit = resident[S] * sm_count / 148;
-                if (fit < 1) fit = 1;
-                const long long waves = (clusters + fit - 1) / fit;
-                const int kb = (num_kb + S - 1) / S;
-                // one SM takes ~60 GB/s through TMA, a stage of four MMAs and its hand-over ~360 ns, the chip ~6.3 TB/s;
-                // the epilogue ~25 ps a value (shared-memory round trip), a split ~0.7 us
-                const double t_load = kb * (stage / 60e9 > 360e-9 ? stage / 60e9 : 360e-9);
-                const double t_chip = static_cast<double>(clusters) * S * kb * stage / 6.3e12 / waves;
-                const double c = waves * ((t_load > t_chip ? t_load : t_chip) + 1.5e-6 + 25e-12 * rows * R / S + (S > 1 ? 0.7e-6 : 0.0));
-                if (c < best_cost) { best_cost = c; best.R = R; best.S = S; }
-            }
-        }
+        best.R = 256;       // 128 x 28672 x 4096: 19.4 us, with 128 columns in two waves 26
     }
     best.b_tiles = (best.R + 127) / 128;
     best.stages = ring_limit(format, best.mbox, best.R, best.b_tiles);
@@ -714,7 +709,14 @@ int rdb_dense_gemm_fp4_tuned(const uint8_t* A, const uint8_t* scales_a, const fl
     auto st = static_cast<cudaStream_t>(stream);
     const long long tiles = static_cast<long long>((M + 255ll) / 256) * ((N + 255ll) / 256);
     if (tiles > (1ll << 30)) return RDB_SIZE_ABOVE_LIMIT;
-    if (tiling == 0) tiling = tiles >= 32 || M > 2048 ? 2 : 1;
+    if (tiling == 0) {
+        // Pairs where their 256 x 256 tiles are enough for half of the machine and K is long, or there are more 128-row
+        // tiles than SMs: 512 x 4096 x 4096 takes 11.0 us (12.3 with 128-row tiles), 256 x 4096 x 4096 10.9 (9.9), 1024^3
+        // 6.8 (5.5).  Up to 128 rows a pair would multiply padding: 48 x 28672 x 4096 takes 20.9 us, 15.5 with 128 rows.
+        const long long t128 = static_cast<long long>((M + 127ll) / 128) * ((N + 127ll) / 128);
+        const bool pairs = M > 128 && (t128 > info->sm_count || (2 * t128 > info->sm_count && K > 8 * rdb::fp4::STAGE_K));
+        tiling = pairs ? 2 : 1;
+    }
     if (tiling == 2)
         return format == RDB_FP4_NVFP4 ? rdb::fp4::launch_pair<RDB_FP4_NVFP4>(q, max_ctas, info, st)
                                        : rdb::fp4::launch_pair<RDB_FP4_MXFP4>(q, max_ctas, info, st);
