@@ -415,3 +415,289 @@ def test_dense_product(cuda_device, form, M, N, K, dtype):
     torch.cuda.synchronize()
     assert R.lib().rdb_device_status() == 0
     check_product(got, A, B)
+
+
+# ------------------------------------------------------------------ what else the documentation allows
+def _product(A, B, **k):
+    import rocm_dev_b200 as R
+    return (R.skinny_gemm_fp4 if A.rows <= 32 and not k.get("tiling") else R.dense_gemm_fp4)(A, B, **k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("M,tiling", [(5, 0), (200, 1), (300, 2)])
+def test_what_is_no_number_stays_in_its_row_and_column(cuda_device, form, M, tiling):
+    import rocm_dev_b200 as R
+    N, K = 260, 700
+    a, b = draw(M, K, 1), draw(N, K, 2)
+    a[1, 3], b[7, 699] = float("nan"), float("inf")
+    A, B = held(a, form, cuda_device), held(b, form, cuda_device)
+    got = _product(A, B, out_dtype=torch.float32, **({"tiling": tiling} if tiling else {}))
+    bad = torch.isnan(got).cpu()
+    want = torch.zeros(M, N, dtype=torch.bool)
+    want[1], want[:, 7] = True, True
+    assert torch.equal(bad, want) and not torch.isinf(got).any()
+    (ca, sa, ta), (cb, sb, tb) = plain(A), plain(B)
+    x, y = values(ca, sa, form, K), values(cb, sb, form, K)
+    alpha = 1.0 if ta is None else float(ta) * float(tb)
+    fine = ~want.numpy()
+    exact, mag = np.nan_to_num(x) @ np.nan_to_num(y).T * alpha, np.abs(np.nan_to_num(x)) @ np.abs(np.nan_to_num(y)).T * alpha
+    err = np.abs(got.double().cpu().numpy() - exact)
+    assert (err[fine] <= (2.0 ** -24 * np.abs(exact) + (4 * np.sqrt(K) + 3) * 2.0 ** -24 * mag)[fine]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("M,N,K,tiling", [(7, 70, 300, 0), (100, 130, 600, 1), (270, 300, 520, 2)])
+@pytest.mark.parametrize("shift", [1, 2, 4, 5])
+def test_outputs_at_any_address_and_nothing_around_them(cuda_device, form, M, N, K, tiling, shift):
+    import rocm_dev_b200 as R
+    A, B = held(draw(M, K, 1), form, cuda_device), held(draw(N, K, 2), form, cuda_device)
+    for dtype in (torch.bfloat16, torch.float32):
+        wide = torch.full((M * N + 64,), 7.0, dtype=dtype, device=cuda_device)
+        out = wide[shift:shift + M * N].view(M, N)
+        got = R.dense_gemm_fp4(A, B, out=out, tiling=tiling) if tiling else R.skinny_gemm_fp4(A, B, out=out)
+        assert got.data_ptr() == out.data_ptr()
+        check_product(got, A, B)
+        assert (wide[:shift] == 7).all() and (wide[shift + M * N:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_bytes_behind_the_last_row_do_not_matter(cuda_device, form):
+    """Scale bytes of rows past the last (whole tiles of 128 rows are held) may be anything, a NaN included."""
+    import rocm_dev_b200 as R
+    for M, N, tiling in ((3, 200, 0), (130, 200, 1), (300, 200, 2)):
+        A, B = held(draw(M, 520, 1), form, cuda_device), held(draw(N, 520, 2), form, cuda_device)
+        want = R.dense_gemm_fp4(A, B, tiling=tiling) if tiling else R.skinny_gemm_fp4(A, B)
+        for t in (A, B):
+            tiles = t.scales.view(-(-t.rows // 128), -1, 32, 4, 4)
+            r = torch.arange(t.rows, -(-t.rows // 128) * 128, device=cuda_device)
+            tiles[r // 128, :, r % 32, r % 128 // 32, :] = 0xFF
+        got = R.dense_gemm_fp4(A, B, tiling=tiling) if tiling else R.skinny_gemm_fp4(A, B)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_same_bits_call_after_call(cuda_device, form):
+    import rocm_dev_b200 as R
+    for M, N, K, tiling in ((8, 4096, 4096, 0), (96, 512, 4096, 1), (600, 1100, 2048, 2)):
+        A, B = held(draw(M, K, 1), form, cuda_device), held(draw(N, K, 2), form, cuda_device)
+        runs = [R.dense_gemm_fp4(A, B, tiling=tiling, out_dtype=torch.float32) if tiling else R.skinny_gemm_fp4(A, B, out_dtype=torch.float32)
+                for _ in range(4)]
+        assert all(torch.equal(r, runs[0]) for r in runs)
+
+
+@pytest.mark.gpu
+def test_launches_that_overlap_their_predecessor(cuda_device):
+    """A chain of products in which each launch may request its weights while the one before it runs; the activations are
+    quantised from the product before."""
+    import rocm_dev_b200 as R
+    W = [held(draw(1024, 1024, s, std=0.02), "nvfp4", cuda_device) for s in range(4)]
+    x = draw(16, 1024, 9).to(cuda_device)
+
+    def chain(flags):
+        y = x
+        for _ in range(3):
+            for w in W:
+                y = R.skinny_gemm_fp4(R.quantize_fp4(y), w, flags=flags)
+        return y
+
+    want = chain(0)
+    for _ in range(5):
+        assert torch.equal(chain(R.OVERLAP_PRIOR_KERNEL), want)
+    assert R.lib().rdb_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_two_captured_graphs_and_eager_calls_at_once(cuda_device, form):
+    """Two graphs of quantiser and products replayed on two streams while eager calls run on a third: nothing is shared."""
+    import rocm_dev_b200 as R
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(3)]
+    W = held(draw(2048, 1024, 1, std=0.02), form, cuda_device)
+    xs = [draw(m, 1024, 5 + m).to(cuda_device) for m in (16, 300, 64)]
+
+    def step(x):
+        r, c = R.quantize_fp4_both(x, form)
+        y = _product(r, W)
+        z = R.dense_gemm_fp4(c, c, out_dtype=torch.float32)
+        return y, z, R.dequantize_fp4(r)
+
+    want = [step(x) for x in xs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x, s in zip(xs[:2], streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(step(x))
+        graphs.append(g)
+    for o in outs:
+        for t in o:
+            t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = step(xs[2])
+    torch.cuda.synchronize()
+    assert R.lib().rdb_device_status() == 0
+    for o, w in zip([*outs, eager], want):
+        assert all(torch.equal(a, b) for a, b in zip(o, w))
+
+
+@pytest.mark.gpu
+def test_new_values_in_the_same_buffers_are_seen(cuda_device):
+    """Nothing is kept by an address: operands overwritten in place, a replayed graph included."""
+    import rocm_dev_b200 as R
+    x = draw(8, 512, 1).to(cuda_device)
+    W = held(draw(256, 512, 2), "nvfp4", cuda_device)
+    s = torch.cuda.Stream(cuda_device)
+    with torch.cuda.stream(s):
+        R.skinny_gemm_fp4(R.quantize_fp4(x), W)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        y = R.skinny_gemm_fp4(R.quantize_fp4(x), W)
+    for seed in (3, 4):
+        x.copy_(draw(8, 512, seed))
+        new = held(draw(256, 512, seed + 9), "nvfp4", cuda_device)
+        W.codes.copy_(new.codes), W.scales.copy_(new.scales), W.tensor_scale.copy_(new.tensor_scale)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, R.skinny_gemm_fp4(R.quantize_fp4(x), new))
+
+
+@pytest.mark.gpu
+def test_another_device_than_the_current_one(cuda_device):
+    import rocm_dev_b200 as R
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    other = torch.device("cuda:1")
+    x = draw(8, 512, 1)
+    a, b = held(x, "nvfp4", other), held(x, "nvfp4", cuda_device)
+    assert torch.equal(R.skinny_gemm_fp4(a, a).cpu(), R.skinny_gemm_fp4(b, b).cpu()) and torch.cuda.current_device() == 0
+    with pytest.raises(ValueError):
+        R.skinny_gemm_fp4(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_gradients_of_a_linear_layer(cuda_device, form):
+    """y = x w^T with operands that the format holds exactly along either direction: the three products of a training step
+    against the 64-bit formula, and the gradients against differences of the loss sum(dy * y), which is linear in each."""
+    import rocm_dev_b200 as R
+    M, N, K = 70, 130, 200
+    g = torch.Generator().manual_seed(7)
+    grid = torch.tensor([0.5, 1, 1.5, 2, 3, 4, 6, -0.5, -1, -1.5, -2, -3, -4, -6])
+    pick = lambda *s: grid[torch.randint(0, 14, s, generator=g)]  # noqa: E731
+    x, w, dy = pick(M, K), pick(N, K), pick(M, N)
+    one = None if form == "mxfp4" else torch.ones(1, device=cuda_device)
+    for t in (x, w, dy):
+        t[::32], t[:, ::32] = 6.0, 6.0
+        r, c = R.quantize_fp4_both(t.to(cuda_device), form, one)
+        check_quantized(r, t.numpy(), form, 1.0)
+        check_quantized(c, t.numpy().T.copy(), form, 1.0)
+        # a 6 in every block, whose scale is 1 then, whichever way the blocks lie.  (Every 32nd alone leaves blocks of 16
+        # without one: with 4 as the largest magnitude their scale is e4m3(4 / 6) = 0.6875, and 4 is held as 4.125.)
+        t[::16], t[:, ::16] = 6.0, 6.0
+    both = [R.quantize_fp4_both(t.to(cuda_device), form, one) for t in (x, w, dy)]
+    for t, (r, c) in zip((x, w, dy), both):
+        assert torch.equal(R.dequantize_fp4(r, torch.float32).cpu(), t) and torch.equal(R.dequantize_fp4(c, torch.float32).cpu(), t.t())
+    (xr, xc), (wr, wc), (gr, gc) = both
+    y, dx, dw = (R.dense_gemm_fp4(a, b, out_dtype=torch.float32).double().cpu() for a, b in ((xr, wr), (gr, wc), (gc, xc)))
+    x, w, dy = x.double(), w.double(), dy.double()
+    # multiples of 1/4 below 2^24 / 4: every sum is exact in fp32
+    assert torch.equal(y, x @ w.t()) and torch.equal(dx, dy @ w) and torch.equal(dw, dy.t() @ x)
+    loss = lambda x, w: (dy * (x @ w.t())).sum()  # noqa: E731
+    for i, j in ((0, 0), (33, 199), (69, 64)):
+        d = torch.zeros_like(x)
+        d[i, j] = 0.25
+        assert ((loss(x + d, w) - loss(x - d, w)) / 0.5 - dx[i, j]).abs() < 1e-6
+    for i, j in ((0, 199), (129, 0), (64, 77)):
+        d = torch.zeros_like(w)
+        d[i, j] = 0.25
+        assert ((loss(x, w + d) - loss(x, w - d)) / 0.5 - dw[i, j]).abs() < 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("M", [4, 150])
+def test_a_layer_run_as_it_is_served(cuda_device, form, M):
+    """Quantise, project up, quantise, project down: each product against the 64-bit product of what its operands hold, and
+    the whole against the same steps in plain form."""
+    import rocm_dev_b200 as R
+    x = draw(M, 512, 1)
+    up, down = draw(1000, 512, 2, std=0.02), draw(512, 1000, 3, std=0.02)
+    U, D = held(up, form, cuda_device), held(down, form, cuda_device)
+    X = held(x, form, cuda_device)
+    h = _product(X, U)
+    check_product(h, X, U)
+    H = R.quantize_fp4(h, form)
+    check_quantized(H, h.float().cpu().numpy(), form)
+    y = _product(H, D, out_dtype=torch.float32)
+    check_product(y, H, D)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda_device):
+    """x of 2.3e9 elements (4.6 GB of bf16, codes of 1.15 GB, values of 4.6 GB): the last rows as in a tensor of their own; and
+    a product whose output passes 2^32 bytes."""
+    import rocm_dev_b200 as R
+    rows, K = 140_001, 16_384
+    free, _ = torch.cuda.mem_get_info(cuda_device)
+    if free < 40e9:
+        pytest.skip("too little memory")
+    x = torch.empty((rows, K), dtype=torch.bfloat16, device=cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    for i in range(0, rows, 20_000):
+        x[i:i + 20_000] = torch.randn((min(20_000, rows - i), K), generator=g, device=cuda_device).bfloat16()
+    for form in FORMATS:
+        r, c = R.quantize_fp4_both(x, form)
+        one = R.quantize_fp4(x, form)
+        tail = slice(rows - 97, rows)
+        t = R.quantize_fp4(x[tail], form, r.tensor_scale)
+        assert torch.equal(r.codes, one.codes) and torch.equal(r.codes[tail], t.codes)
+        assert torch.equal(R.unpack_fp4_scales(r)[tail], R.unpack_fp4_scales(t))
+        tc = R.quantize_fp4(x[:, -3:].t().contiguous(), form, r.tensor_scale)
+        assert torch.equal(c.codes[-3:], tc.codes) and torch.equal(R.unpack_fp4_scales(c)[-3:], R.unpack_fp4_scales(tc))
+        v = R.dequantize_fp4(one)
+        assert torch.equal(v[tail], R.dequantize_fp4(t))
+        del r, c, one, v
+    del x
+    M, N = 70_000, 32_776
+    A, B = held(draw(M, 64, 1), "nvfp4", cuda_device), held(draw(N, 64, 2), "nvfp4", cuda_device)
+    d = R.dense_gemm_fp4(A, B)
+    rows = slice(M - 140, M)
+    cut = R.Fp4Tensor(A.codes[rows].contiguous(), R.pack_fp4_scales(R.unpack_fp4_scales(A)[rows], "nvfp4", 64), A.tensor_scale, "nvfp4", 140, 64)
+    assert torch.equal(d[rows], R.dense_gemm_fp4(cut, B))
+    torch.cuda.synchronize()
+    assert R.lib().rdb_device_status() == 0
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device(cuda_device):
+    import rocm_dev_b200 as R
+    A, B = held(draw(40, 64, 1), "nvfp4", cuda_device), held(draw(8, 64, 2), "nvfp4", cuda_device)
+    with pytest.raises(R.RdbError) as e:
+        R.skinny_gemm_fp4(A, B)
+    assert e.value.code == 1
+    for bad in (held(draw(8, 96, 2), "nvfp4", cuda_device), held(draw(8, 64, 2), "mxfp4", cuda_device), B.to("cpu")):
+        with pytest.raises(ValueError):
+            R.dense_gemm_fp4(A, bad)
+    for out in (torch.empty(40, 9, device=cuda_device), torch.empty(8, 40, device=cuda_device).t(), torch.empty(40, 8)):
+        with pytest.raises(ValueError):
+            R.dense_gemm_fp4(A, B, out=out)
+    with pytest.raises(TypeError):
+        R.dense_gemm_fp4(A, B, out_dtype=torch.float64)
+    x = draw(4, 64, 1).to(cuda_device)
+    with pytest.raises(ValueError):
+        R.quantize_fp4(x, "mxfp4", torch.ones(1, device=cuda_device))
+    with pytest.raises(ValueError):
+        R.quantize_fp4(x, "nvfp4", torch.ones(1))
+    with pytest.raises(ValueError):
+        R.quantize_fp4(x[:, :0])
