@@ -9,10 +9,12 @@ from __future__ import annotations
 import glob
 import os
 import subprocess
+import sysconfig
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "librocm_dev_b200.so")
+FAST_PATH = os.path.join(_HERE, "_fastcall.so")     # optional: see csrc/fastcall.c
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -30,7 +32,7 @@ def _stale() -> bool:
     if not os.path.exists(LIB_PATH):
         return True
     t = os.path.getmtime(LIB_PATH)
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h"))
+    deps = sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.c"))
     deps.append(os.path.join(_HERE, "..", "include", "rocm_dev_b200.h"))
     return any(os.path.getmtime(d) > t for d in deps)
 
@@ -45,7 +47,18 @@ def build(force: bool = False, verbose: bool = False) -> str:
         cmd += ["-Xptxas", "-v"]
     cmd += ["-o", LIB_PATH, *sources()]
     subprocess.check_call(cmd)
+    _build_fastcall()
     return LIB_PATH
+
+
+def _build_fastcall() -> None:
+    """The C entry of the short calls, where the Python headers are there; without it ctypes does the same."""
+    include = sysconfig.get_paths()["include"]
+    if os.path.exists(FAST_PATH):
+        os.remove(FAST_PATH)
+    if os.path.exists(os.path.join(include, "Python.h")):
+        subprocess.check_call([os.environ.get("CC", "gcc"), "-O2", "-shared", "-fPIC", "-I", include, "-o", FAST_PATH,
+                               os.path.join(CSRC, "fastcall.c")])
 
 
 if __name__ == "__main__":

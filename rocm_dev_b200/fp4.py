@@ -12,6 +12,8 @@ along the rows and ``c`` the one along the columns
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
 from ._lib import check, lib
@@ -20,6 +22,7 @@ FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 WORKSPACE_FLOATS = 1024
+_BYTE = torch.uint8
 
 # A step's calls are short: what a call costs on the host shows.  These two are the cheap forms of
 # torch.cuda.current_device() and torch.cuda.current_stream(dev).cuda_stream (0.1 us each instead of 0.2 and 2.2).
@@ -58,23 +61,24 @@ class Fp4Tensor:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, tensor_scale, format: str, rows: int, K: int):
         fmt = _format(format)
-        dev = codes.device
-        if not (codes.dtype is torch.uint8 and codes.shape == (rows, (K + 31) // 32 * 16) and codes.is_contiguous()):
-            raise ValueError(f"codes must be contiguous uint8 [{rows}, {row_bytes(K)}]")
-        if not (scales.dtype is torch.uint8 and scales.numel() == scale_bytes(format, rows, K) and scales.is_contiguous()
-                and scales.device == dev):
-            raise ValueError(f"scales must be {scale_bytes(format, rows, K)} contiguous bytes on {dev}")
+        index = codes.get_device()
+        if (codes.dtype is not _BYTE or codes.shape != (rows, (K + 31) // 32 * 16) or not codes.is_contiguous()
+                or scales.dtype is not _BYTE or scales.numel() != (rows + 127) // 128 * ((K + 255) // 256) * (2048 if fmt else 1024)
+                or not scales.is_contiguous() or scales.get_device() != index):
+            raise ValueError(f"codes must be contiguous uint8 [{rows}, {row_bytes(K)}] and scales {scale_bytes(format, rows, K)} "
+                             "contiguous bytes on one device")
         if fmt == 0:
             if tensor_scale is not None:
                 raise ValueError("mxfp4 has no tensor scale")
-            self._args = (codes.data_ptr(), scales.data_ptr(), None)
+            scale_ptr = None
+        elif (tensor_scale is None or tensor_scale.dtype is not torch.float32 or tensor_scale.numel() != 1
+              or tensor_scale.get_device() != index):
+            raise ValueError("nvfp4 needs a tensor scale: one fp32 on the device of the codes")
         else:
-            if not (tensor_scale is not None and tensor_scale.dtype is torch.float32 and tensor_scale.numel() == 1
-                    and tensor_scale.device == dev):
-                raise ValueError(f"nvfp4 needs a tensor scale: one fp32 on {dev}")
-            self._args = (codes.data_ptr(), scales.data_ptr(), tensor_scale.data_ptr())
+            scale_ptr = tensor_scale.data_ptr()
+        self._args = (codes.data_ptr(), scales.data_ptr(), scale_ptr)
         self._parts = (codes, scales, tensor_scale)
-        self.format, self.rows, self.K, self.device, self._fmt = format, rows, K, dev, fmt
+        self.format, self.rows, self.K, self.device, self._fmt = format, rows, K, codes.device, fmt
 
     def _views(self):
         # a quantiser's result is one allocation (codes, scales, tensor scale at the addresses in _args); its tensors are
@@ -116,16 +120,37 @@ def _device(dev: torch.device) -> int:
     return dev.index
 
 
-def _call(fn, where: str, dev: int, *args) -> None:
-    """fn(*args, the current stream of device dev), with dev as the current device."""
-    prev = _current_device()
-    if prev == dev:
+class _Entries:
+    """The library's functions, through csrc/fastcall.c where it was built, else through ctypes."""
+
+    def __init__(self):
+        L = lib()
+        names = ("rdb_quantize_fp4", "rdb_dequantize_fp4", "rdb_dense_gemm_fp4_tuned", "rdb_skinny_gemm_fp4")
+        try:
+            from . import _fastcall as fast
+            fast.bind(*(C.cast(getattr(L, n), C.c_void_p).value for n in names))
+            found = (fast.quantize, fast.dequantize, fast.dense, fast.skinny)
+        except ImportError:
+            found = tuple(getattr(L, n) for n in names)
+        self.quantize, self.dequantize, self.dense, self.skinny = found
+
+
+_entries = None
+
+
+def _call(name: str, dev: int, *args) -> None:
+    """The entry `name` with args and the current stream of device dev, dev being made the current device."""
+    global _entries
+    if _entries is None:
+        _entries = _Entries()
+    fn = getattr(_entries, name)
+    if _current_device() == dev:
         code = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
             code = fn(*args, _raw_stream(dev))
     if code:
-        check(code, where)
+        check(code, f"{name} (4-bit)")
 
 
 def _held(form: str, fmt: int, rows: int, K: int, dev, buffer, at: int, scales: int, scale_ptr) -> Fp4Tensor:
@@ -166,7 +191,7 @@ def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
     at_s, at_ct = at + codes, at + codes + scales
     at_st, end = at_ct + codes_t, at_ct + codes_t + scales_t
     scale_ptr = end if own_scale else tensor_scale.data_ptr() if given else None
-    _call(lib().rdb_quantize_fp4, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, scale_ptr, given, at, at_s,
+    _call("quantize", index, x.data_ptr(), typ, ldx, rows, K, fmt, scale_ptr, given, at, at_s,
           at_ct if both else None, at_st if both else None, end + 16 if own_scale else None)
     held = (buffer, tensor_scale)
     return (_held(format, fmt, rows, K, dev, held, at, at_s, scale_ptr),
@@ -190,7 +215,7 @@ def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.T
     typ, index = _type(dtype), _device(t.device)
     out = torch.empty(t.rows, t.K, dtype=dtype, device=t.device)
     codes, scales, ts = t._args
-    _call(lib().rdb_dequantize_fp4, "rdb_dequantize_fp4", index, codes, scales, ts, t._fmt, t.rows, t.K, out.data_ptr(), typ)
+    _call("dequantize", index, codes, scales, ts, t._fmt, t.rows, t.K, out.data_ptr(), typ)
     return out
 
 
@@ -216,7 +241,7 @@ def dense_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
     """D[M,N] = A . B^T over the values of A [M,K] and B [N,K], any sizes; fp32 accumulation, rounded once to
     ``out_dtype`` (``out``'s type where it is given).  ``tiling``, ``max_ctas``: the tuner's knobs, 0 = automatic."""
     args, out, index = _product(A, B, out, out_dtype)
-    _call(lib().rdb_dense_gemm_fp4_tuned, "rdb_dense_gemm_fp4", index, *args, tiling, max_ctas)
+    _call("dense", index, *args, tiling, max_ctas)
     return out
 
 
@@ -225,7 +250,7 @@ def skinny_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
     """The same product for at most 32 rows of A (decode): a stream over B.  ``flags``: 0 or ``OVERLAP_PRIOR_KERNEL`` (the
     launch may request B while the preceding kernel of the stream drains; that kernel must not write B)."""
     args, out, index = _product(A, B, out, out_dtype)
-    _call(lib().rdb_skinny_gemm_fp4, "rdb_skinny_gemm_fp4", index, *args, flags)
+    _call("skinny", index, *args, flags)
     return out
 
 
