@@ -16,6 +16,8 @@
 #include "host_util.h"
 #include "ptx.cuh"
 
+RDB_DEFINE_WAIT_BUDGET_SETTER()
+
 namespace rdb {
 namespace fp4 {
 
@@ -114,6 +116,17 @@ __device__ __forceinline__ uint32_t finite_magnitude(const uint32_t* w) {
         }
     }
     return m;
+}
+
+// The same of N floats, two a step (sm_100's three-operand maximum; a NaN wins).
+template <int N>
+__device__ __forceinline__ uint32_t magnitude(const float* v) {
+    float m;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(v[0]), "f"(v[1]), "f"(v[2]));
+#pragma unroll
+    for (int i = 3; i < N - 1; i += 2) asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i]), "f"(v[i + 1]));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[N - 1]), "f"(0.0f));
+    return __float_as_uint(m) & 0x7FFFFFFFu;
 }
 
 // 8 floats -> 8 e2m1 codes.
@@ -373,7 +386,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
                     float v[B];
                     unpack<T, B>(w[j], v);
                     uint32_t c[B / 8];
-                    byte[h + j] = encode_block<T, FMT, decltype(careful)::value>(v, magnitude<T, B>(w[j]), scale, c);
+                    const uint32_t amax = FMT == RDB_FP4_MXFP4 ? magnitude<T, B>(w[j]) : magnitude<B>(v);     // each the faster one here
+                    byte[h + j] = encode_block<T, FMT, decltype(careful)::value>(v, amax, scale, c);
                     if (static_cast<size_t>(b) * (B / 2) < pitch) store_codes<B>(codes + r * pitch + static_cast<size_t>(b) * (B / 2), c);
                 }
             }
@@ -600,7 +614,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
                 float v[B];
                 unpack<T, B>(w, v);
                 uint32_t c[B / 8];
-                sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(careful)::value>(v, magnitude<T, B>(w), scale, c));
+                sc[(b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, c));
                 if (inside && r < rows_left) store_codes<B>(to + static_cast<size_t>(j * (kTileThreads / NB)) * pitch, c);
             }
         }
@@ -617,17 +631,12 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
                 const uint32_t* from = tile + at(rb * B, word);
 #pragma unroll
                 for (int j = 0; j < B; j++) raw[j] = from[j * W];
-                [[maybe_unused]] uint32_t m = 0;                    // a word holds two columns: their maxima together
-                if constexpr (CPW == 2) m = halves_magnitude<T, B>(raw);
                 const size_t k2 = tr * 64ull + rb * (B / 2);
                 uint8_t* to = codes_t + (tc * 128ull + word * CPW) * pitch_t + k2;
                 const bool inside = k2 < pitch_t;
 #pragma unroll
                 for (int h = 0; h < CPW / SPLIT; h++) {
                     const int half = SPLIT > 1 ? h0 : h, col = word * CPW + half;
-                    uint32_t amax;
-                    if constexpr (CPW == 1) amax = magnitude<T, B>(raw);
-                    else amax = bits_of_half<T>(half ? m >> 16 : m & 0xFFFFu);
                     float v[B];
 #pragma unroll
                     for (int j = 0; j < B; j++) {
@@ -636,7 +645,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
                         else v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(half ? raw[j] >> 16 : raw[j])));
                     }
                     uint32_t c[B / 8];
-                    sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(careful)::value>(v, amax, scale, c));
+                    sc_t[(rb >> 2) * 512 + (col & 31) * 16 + (col >> 5) * 4 + (rb & 3)] = static_cast<uint8_t>(encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, c));
                     if (inside && col < cols_left) store_codes<B>(to + (half ? pitch_t : 0), c);
                 }
             }
@@ -655,6 +664,175 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
                     reinterpret_cast<const uint4*>(sc_t)[i];
         }
     }
+    };
+    if (FMT == RDB_FP4_NVFP4 && (scale.move != 1.0f || !partial)) body(std::true_type());
+    else body(std::false_type());
+}
+
+// Both directions for x on 16-byte boundaries.  Persistent blocks; a producer thread fills a ring of tiles - 128 rows of
+// four blocks - with TMA boxes of 128 bytes x 128 rows (SWIZZLE_128B: 16-byte chunk c of row r at c ^ r % 8), two groups of
+// four warps take alternate tiles, and nothing but the ring's barriers holds them together.  A thread makes the four
+// blocks of one row, or of the one or two columns in a word: their scale bytes are a whole scale word, their codes whole
+// 16-byte stores, and no data passes between threads.  Bank conflicts: along a row the 8 lanes of a 16-byte phase hold 8
+// rows, whose chunks the swizzle spreads; along the columns the 32 lanes read the 32 words of one row.
+template <class T, int FMT>
+struct BothCfg {
+    static constexpr int B = Format<FMT>::BLOCK, BW = B * sizeof(T) / 4, CPW = 4 / sizeof(T);
+    static constexpr int COLS = 4 * B;                              // columns of a tile
+    static constexpr int BOXES = COLS * sizeof(T) / 128, BOX_BYTES = 128 * 128;
+    static constexpr int GROUPS = 128 / COLS;                       // scale words of a column in a tile: 2 or 1
+    static constexpr int STAGE = BOXES * BOX_BYTES;
+    // an even ring: the groups take alternate tiles, and only with a slot of its own does a group wait for consecutive
+    // completions of a barrier (a parity wait cannot tell completion n from n + 2)
+    static constexpr int STAGES = STAGE == 16384 ? 4 : 2;
+    static constexpr int PER_SM = STAGE == 65536 ? 1 : 2;
+    static constexpr int SMEM = 1024 + STAGES * STAGE;
+};
+constexpr int kBothThreads = 288;      // warps 0-3 and 4-7: the two groups, warp 8: the producer
+
+template <class T, int FMT>
+__global__ void __launch_bounds__(kBothThreads, BothCfg<T, FMT>::PER_SM)
+quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, unsigned tiles_x, unsigned tiles_all, float* tscale, const uint32_t* partial,
+                     int partials, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint8_t* __restrict__ codes_t,
+                     uint8_t* __restrict__ scales_t, int* status) {
+    using C = BothCfg<T, FMT>;
+    constexpr int B = C::B, BW = C::BW, CPW = C::CPW, COLS = C::COLS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t bars[2 * C::STAGES];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + C::STAGES);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::STAGES; i++) {
+            mbar_init(full0 + 8 * i, 1);
+            mbar_init(empty0 + 8 * i, 4);
+        }
+        fence_barrier_init();
+    }
+    if (threadIdx.x == 256) prefetch_tensormap(&tm);
+    pdl_launch_dependents();
+    __syncthreads();
+    pdl_wait_prior();
+    // tiles n = blockIdx.x, + gridDim.x, ... counted from the last one (the maximum's pass read those last)
+    if (warp == 8 && lane == 0) {
+        const uint64_t pol = l2_policy_evict_first();
+        int i = 0;
+        for (unsigned n = blockIdx.x; n < tiles_all && i < C::STAGES; n += gridDim.x, i++) {      // the first ring-full: before the scale is known
+            const unsigned id = tiles_all - 1 - n, tr = id / tiles_x, tc = id - tr * tiles_x;
+            mbar_arrive_expect_tx(full0 + 8 * i, C::STAGE);
+#pragma unroll
+            for (int b = 0; b < C::BOXES; b++)
+                tma_load_2d(smem_u32(smem) + i * C::STAGE + b * C::BOX_BYTES, &tm, tc * COLS + b * (128 / static_cast<int>(sizeof(T))), tr * 128, full0 + 8 * i, pol);
+        }
+    }
+    const Scale scale = fetch_scale<T, FMT, kBothThreads>(tscale, partial, partials);
+
+    if (warp == 8) {
+        if (lane == 0) {
+            const uint64_t pol = l2_policy_evict_first();
+            unsigned n = blockIdx.x + C::STAGES * gridDim.x;
+            for (int i = C::STAGES; n < tiles_all && n >= gridDim.x; n += gridDim.x, i++) {
+                const int s = i % C::STAGES;
+                if (!mbar_wait(empty0 + 8 * s, ((i / C::STAGES) & 1) ^ 1)) { report_timeout(status); break; }
+                const unsigned id = tiles_all - 1 - n, tr = id / tiles_x, tc = id - tr * tiles_x;
+                mbar_arrive_expect_tx(full0 + 8 * s, C::STAGE);
+#pragma unroll
+                for (int b = 0; b < C::BOXES; b++)
+                    tma_load_2d(smem_u32(smem) + s * C::STAGE + b * C::BOX_BYTES, &tm, tc * COLS + b * (128 / static_cast<int>(sizeof(T))), tr * 128, full0 + 8 * s, pol);
+            }
+        }
+        return;          // (every tile that was requested is waited for by a group below)
+    }
+
+    const size_t pitch = row_bytes(K), pitch_t = row_bytes(rows);
+    const int tiles_k = scale_tiles_per_row(FMT, K), tiles_r = scale_tiles_per_row(FMT, rows);
+    const int group = warp >> 2, q = warp & 3;
+    auto body = [&](auto careful) {
+        // four blocks of row r of the tile
+        auto along_row = [&](const uint8_t* tile, unsigned tr, unsigned tc, int r) {
+            const long long row = tr * 128ll + r;
+            const uint8_t* line = tile + r * 128;
+            const uint32_t turn = (r & 7) << 4;
+            uint8_t* to = codes + row * pitch + tc * (COLS / 2ull);
+            const bool exists = row < rows;
+            uint32_t word = 0, c[B / 8 * 2];
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                uint32_t w[BW];
+#pragma unroll
+                for (int i = 0; i < BW; i += 4) {
+                    const int at = (b * BW + i) * 4;
+                    *reinterpret_cast<uint4*>(w + i) = *reinterpret_cast<const uint4*>(line + at / 128 * C::BOX_BYTES + ((at % 128) ^ turn));
+                }
+                float v[B];
+                unpack<T, B>(w, v);
+                uint32_t* out = B == 16 ? c + (b & 1) * 2 : c;
+                word |= encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, out) << (8 * b);
+                // 16 bytes: two blocks of 16, or one of 32
+                if (B == 32 || (b & 1)) {
+                    const size_t k2 = B == 32 ? b * 16 : b / 2 * 16;
+                    if (exists && tc * (COLS / 2ull) + k2 < pitch) *reinterpret_cast<uint4*>(to + k2) = make_uint4(c[0], c[1], c[2], c[3]);
+                }
+            }
+            if (exists) *reinterpret_cast<uint32_t*>(scales + scale_word(row, tc, tiles_k)) = word;
+        };
+        // four blocks of each column in word `lane` of a box; g: which 4 B rows
+        auto along_columns = [&](const uint8_t* tile, unsigned tr, unsigned tc, int box, int g) {
+            const uint8_t* from = tile + box * C::BOX_BYTES + g * (COLS * 128);
+            const long long col = tc * static_cast<long long>(COLS) + box * (128 / static_cast<int>(sizeof(T))) + lane * CPW;
+            const size_t k0 = tr * 64ull + g * (COLS / 2);
+            uint8_t* to = codes_t + col * pitch_t + k0;
+            uint32_t word[CPW], c[CPW][B / 8 * 2];
+#pragma unroll
+            for (int h = 0; h < CPW; h++) word[h] = 0;
+#pragma unroll 2
+            for (int b = 0; b < 4; b++) {
+                uint32_t raw[B];
+#pragma unroll
+                for (int j = 0; j < B; j++) raw[j] = *reinterpret_cast<const uint32_t*>(from + (b * B + j) * 128 + ((lane * 4) ^ ((j & 7) << 4)));
+#pragma unroll
+                for (int h = 0; h < CPW; h++) {
+                    float v[B];
+#pragma unroll
+                    for (int j = 0; j < B; j++) {
+                        if constexpr (CPW == 1) v[j] = __uint_as_float(raw[j]);
+                        else if constexpr (std::is_same_v<T, __nv_bfloat16>) v[j] = __uint_as_float(h ? raw[j] & 0xFFFF0000u : raw[j] << 16);
+                        else v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(h ? raw[j] >> 16 : raw[j])));
+                    }
+                    uint32_t* out = B == 16 ? c[h] + (b & 1) * 2 : c[h];
+                    word[h] |= encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, out) << (8 * b);
+                    if (B == 32 || (b & 1)) {
+                        const size_t k2 = B == 32 ? b * 16 : b / 2 * 16;
+                        if (col + h < K && k0 + k2 < pitch_t) *reinterpret_cast<uint4*>(to + h * pitch_t + k2) = make_uint4(c[h][0], c[h][1], c[h][2], c[h][3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < CPW; h++)
+                if (col + h < K) *reinterpret_cast<uint32_t*>(scales_t + scale_word(col + h, tr * C::GROUPS + g, tiles_r)) = word[h];
+        };
+
+        int i = 0;
+        for (unsigned n = blockIdx.x; n < tiles_all; n += gridDim.x, i++) {
+            if ((i & 1) != group) continue;
+            const int s = i % C::STAGES;
+            if (!mbar_wait(full0 + 8 * s, (i / C::STAGES) & 1)) { report_timeout(status); break; }
+            const unsigned id = tiles_all - 1 - n, tr = id / tiles_x, tc = id - tr * tiles_x;
+            const uint8_t* tile = smem + s * C::STAGE;
+            if constexpr (CPW == 2) {                               // two warps take the rows, two the columns
+                if (q < 2) {
+                    along_row(tile, tr, tc, q * 64 + lane);
+                    along_row(tile, tr, tc, q * 64 + 32 + lane);
+                } else {
+                    along_columns(tile, tr, tc, C::BOXES == 2 ? q - 2 : 0, C::BOXES == 2 ? 0 : q - 2);
+                }
+            } else {                                                // each warp a quarter of either
+                along_row(tile, tr, tc, q * 32 + lane);
+                along_columns(tile, tr, tc, C::BOXES == 4 ? q : q & 1, C::BOXES == 4 ? 0 : q >> 1);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty0 + 8 * s);
+        }
     };
     if (FMT == RDB_FP4_NVFP4 && (scale.move != 1.0f || !partial)) body(std::true_type());
     else body(std::false_type());
@@ -811,6 +989,32 @@ static int launch_tiles(int rows, int K, void** args, unsigned* tiles_x, unsigne
 }
 
 template <class T, int FMT>
+static int launch_both(const T* x, long long ldx, int rows, int K, float* tscale, uint32_t* partial, int partials, uint8_t* codes, uint8_t* scales,
+                       uint8_t* codes_t, uint8_t* scales_t, const DeviceInfo* info, cudaStream_t stream) {
+    using C = BothCfg<T, FMT>;
+    static bool attr_set[kMaxDevices] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return RDB_CUDA_ERROR;
+    auto kernel = quantize_both_kernel<T, FMT>;
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return RDB_CUDA_ERROR;
+        attr_set[dev] = true;
+    }
+    // scales are filled up to 256 elements along either direction
+    const long long tx = (static_cast<long long>(K) + 255) / 256 * (256 / C::COLS), all = tx * ((static_cast<long long>(rows) + 255) / 256 * 2);
+    if (all > 0x7FFFFFFFll) return RDB_SIZE_ABOVE_LIMIT;
+    CUtensorMap tm;
+    const int r = make_tmap_2d(&tm, x, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, sizeof(T), rows, K,
+                               static_cast<uint64_t>(ldx) * sizeof(T), 128 / sizeof(T), 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r != RDB_SUCCESS) return r;
+    unsigned tiles_x = static_cast<unsigned>(tx), tiles_all = static_cast<unsigned>(all);
+    int* status = info->status_dev;
+    void* args[] = {&tm, &rows, &K, &tiles_x, &tiles_all, &tscale, &partial, &partials, &codes, &scales, &codes_t, &scales_t, &status};
+    const unsigned grid = static_cast<unsigned>(info->sm_count * C::PER_SM);
+    return launch(reinterpret_cast<const void*>(kernel), dim3(tiles_all < grid ? tiles_all : grid), kBothThreads, C::SMEM, args, stream);
+}
+
+template <class T, int FMT>
 static int quantize(const void* x_, long long ldx, int rows, int K, float* tscale, bool given, uint8_t* codes, uint8_t* scales,
                     uint8_t* codes_t, uint8_t* scales_t, float* workspace, const DeviceInfo* info, cudaStream_t stream) {
     constexpr int B = Format<FMT>::BLOCK;
@@ -850,6 +1054,8 @@ static int quantize(const void* x_, long long ldx, int rows, int K, float* tscal
         return launch(by32 ? reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT, 32>) : reinterpret_cast<const void*>(quantize_rows_kernel<T, FMT, 16>),
                       grid, kThreads, 0, args, stream);
     }
+    if (codes_t && by16 && static_cast<unsigned long long>(row) < (1ull << 40))
+        return launch_both<T, FMT>(x, ldx, rows, K, tscale, partial, partials, codes, scales, codes_t, scales_t, info, stream);
     int vec = by16;
     unsigned tiles_x = 0, tiles_all = 0;
     void* args[] = {&x, &ldx, &rows, &K, &vec, &tiles_x, &tiles_all, &tscale, &partial, &partials, &codes, &scales, &codes_t, &scales_t};
