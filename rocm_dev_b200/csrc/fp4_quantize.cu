@@ -72,10 +72,10 @@ __device__ __forceinline__ void unpack(const uint32_t* w, float* v) {
 template <class T, int WORDS>
 __device__ __forceinline__ uint32_t halves_magnitude(const uint32_t* w) {
     if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-        __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(w));
+        uint32_t m = w[0] & 0x7FFF7FFFu;
 #pragma unroll
-        for (int i = 1; i < WORDS; i++) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(w + i)));
-        return *reinterpret_cast<const uint32_t*>(&m) & 0x7FFF7FFFu;
+        for (int i = 1; i < WORDS; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+        return m;
     } else {
         __half2 m = __habs2(*reinterpret_cast<const __half2*>(w));
 #pragma unroll
@@ -118,15 +118,22 @@ __device__ __forceinline__ uint32_t finite_magnitude(const uint32_t* w) {
     return m;
 }
 
-// The same of N floats, two a step (sm_100's three-operand maximum; a NaN wins).
+// The same of 16 or 32 floats: a tree of sm_100's three-operand maxima (a NaN wins).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float m;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
 template <int N>
 __device__ __forceinline__ uint32_t magnitude(const float* v) {
-    float m;
-    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(v[0]), "f"(v[1]), "f"(v[2]));
+    float m[N / 16];
 #pragma unroll
-    for (int i = 3; i < N - 1; i += 2) asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[i]), "f"(v[i + 1]));
-    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(v[N - 1]), "f"(0.0f));
-    return __float_as_uint(m) & 0x7FFFFFFFu;
+    for (int h = 0; h < N / 16; h++) {
+        const float* u = v + 16 * h;
+        m[h] = max3(max3(max3(u[0], u[1], u[2]), max3(u[3], u[4], u[5]), max3(u[6], u[7], u[8])),
+                    max3(max3(u[9], u[10], u[11]), max3(u[12], u[13], u[14]), u[15]), 0.0f);
+    }
+    return __float_as_uint(N == 16 ? m[0] : max3(m[0], m[N / 16 - 1], 0.0f)) & 0x7FFFFFFFu;
 }
 
 // 8 floats -> 8 e2m1 codes.
@@ -355,7 +362,9 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
     const int lane = threadIdx.x & 31, b = blockIdx.x * 32 + lane, blocks = K / B;
     const int octets = static_cast<int>((rows + 127ll) / 128 * 4);
     auto body = [&](auto careful) {
-        for (int o = blockIdx.y; o < octets; o += gridDim.y) {
+        // after the maximum's pass the last rows first: it read them last, and they may still be in L2
+        for (int n = blockIdx.y; n < octets; n += gridDim.y) {
+            const int o = partial ? octets - 1 - n : n;
             const int r0 = (o >> 2) * 128 + (o & 3) * 8 + (threadIdx.x >> 5);
             if (r0 >= rows) continue;
             uint32_t byte[4] = {0, 0, 0, 0};
@@ -669,9 +678,10 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
     else body(std::false_type());
 }
 
-// Both directions for x on 16-byte boundaries.  Persistent blocks; a producer thread fills a ring of tiles - 128 rows of
-// four blocks - with TMA boxes of 128 bytes x 128 rows (SWIZZLE_128B: 16-byte chunk c of row r at c ^ r % 8), two groups of
-// four warps take alternate tiles, and nothing but the ring's barriers holds them together.  A thread makes the four
+// Both directions for x on 16-byte boundaries.  Persistent blocks with a ring of tiles - 128 rows of four blocks - that TMA
+// boxes of 128 bytes x 128 rows fill (SWIZZLE_128B: 16-byte chunk c of row r at c ^ r % 8).  Two groups of four warps take
+// alternate tiles; the warp that is last to finish one requests the next into its place, and nothing else holds the warps
+// together (a ninth warp that only requested tiles cost the others a quarter of their registers).  A thread makes the four
 // blocks of one row, or of the one or two columns in a word: their scale bytes are a whole scale word, their codes whole
 // 16-byte stores, and no data passes between threads.  Bank conflicts: along a row the 8 lanes of a 16-byte phase hold 8
 // rows, whose chunks the swizzle spreads; along the columns the 32 lanes read the 32 words of one row.
@@ -688,7 +698,7 @@ struct BothCfg {
     static constexpr int PER_SM = STAGE == 65536 ? 1 : 2;
     static constexpr int SMEM = 1024 + STAGES * STAGE;
 };
-constexpr int kBothThreads = 288;      // warps 0-3 and 4-7: the two groups, warp 8: the producer
+constexpr int kBothThreads = 256;
 
 template <class T, int FMT>
 __global__ void __launch_bounds__(kBothThreads, BothCfg<T, FMT>::PER_SM)
@@ -699,50 +709,33 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
     constexpr int B = C::B, BW = C::BW, CPW = C::CPW, COLS = C::COLS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t bars[2 * C::STAGES];
+    __shared__ uint64_t bars[C::STAGES];
+    __shared__ unsigned finished[C::STAGES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + C::STAGES);
+    const uint32_t full0 = smem_u32(bars);
+    // tiles n = blockIdx.x, + gridDim.x, ... counted from the last one (the maximum's pass read those last)
+    auto request = [&](unsigned n, int s) {
+        const unsigned id = tiles_all - 1 - n, tr = id / tiles_x, tc = id - tr * tiles_x;
+        const uint64_t pol = l2_policy_evict_first();
+        mbar_arrive_expect_tx(full0 + 8 * s, C::STAGE);
+#pragma unroll
+        for (int b = 0; b < C::BOXES; b++)
+            tma_load_2d(smem_u32(smem) + s * C::STAGE + b * C::BOX_BYTES, &tm, tc * COLS + b * (128 / static_cast<int>(sizeof(T))), tr * 128, full0 + 8 * s, pol);
+    };
+    pdl_launch_dependents();
     if (threadIdx.x == 0) {
+        prefetch_tensormap(&tm);
         for (int i = 0; i < C::STAGES; i++) {
             mbar_init(full0 + 8 * i, 1);
-            mbar_init(empty0 + 8 * i, 4);
+            finished[i] = 0;
         }
         fence_barrier_init();
+        pdl_wait_prior();
+        for (int i = 0; i < C::STAGES && blockIdx.x + i * gridDim.x < tiles_all; i++) request(blockIdx.x + i * gridDim.x, i);
     }
-    if (threadIdx.x == 256) prefetch_tensormap(&tm);
-    pdl_launch_dependents();
     __syncthreads();
     pdl_wait_prior();
-    // tiles n = blockIdx.x, + gridDim.x, ... counted from the last one (the maximum's pass read those last)
-    if (warp == 8 && lane == 0) {
-        const uint64_t pol = l2_policy_evict_first();
-        int i = 0;
-        for (unsigned n = blockIdx.x; n < tiles_all && i < C::STAGES; n += gridDim.x, i++) {      // the first ring-full: before the scale is known
-            const unsigned id = tiles_all - 1 - n, tr = id / tiles_x, tc = id - tr * tiles_x;
-            mbar_arrive_expect_tx(full0 + 8 * i, C::STAGE);
-#pragma unroll
-            for (int b = 0; b < C::BOXES; b++)
-                tma_load_2d(smem_u32(smem) + i * C::STAGE + b * C::BOX_BYTES, &tm, tc * COLS + b * (128 / static_cast<int>(sizeof(T))), tr * 128, full0 + 8 * i, pol);
-        }
-    }
     const Scale scale = fetch_scale<T, FMT, kBothThreads>(tscale, partial, partials);
-
-    if (warp == 8) {
-        if (lane == 0) {
-            const uint64_t pol = l2_policy_evict_first();
-            unsigned n = blockIdx.x + C::STAGES * gridDim.x;
-            for (int i = C::STAGES; n < tiles_all && n >= gridDim.x; n += gridDim.x, i++) {
-                const int s = i % C::STAGES;
-                if (!mbar_wait(empty0 + 8 * s, ((i / C::STAGES) & 1) ^ 1)) { report_timeout(status); break; }
-                const unsigned id = tiles_all - 1 - n, tr = id / tiles_x, tc = id - tr * tiles_x;
-                mbar_arrive_expect_tx(full0 + 8 * s, C::STAGE);
-#pragma unroll
-                for (int b = 0; b < C::BOXES; b++)
-                    tma_load_2d(smem_u32(smem) + s * C::STAGE + b * C::BOX_BYTES, &tm, tc * COLS + b * (128 / static_cast<int>(sizeof(T))), tr * 128, full0 + 8 * s, pol);
-            }
-        }
-        return;          // (every tile that was requested is waited for by a group below)
-    }
 
     const size_t pitch = row_bytes(K), pitch_t = row_bytes(rows);
     const int tiles_k = scale_tiles_per_row(FMT, K), tiles_r = scale_tiles_per_row(FMT, rows);
@@ -755,24 +748,24 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
             const uint32_t turn = (r & 7) << 4;
             uint8_t* to = codes + row * pitch + tc * (COLS / 2ull);
             const bool exists = row < rows;
-            uint32_t word = 0, c[B / 8 * 2];
+            uint32_t word = 0;
+#pragma unroll 1
+            for (int k2 = 0; k2 < COLS / 2; k2 += 16) {             // 16 bytes of codes: two blocks of 16, or one of 32
+                uint32_t c[4];
 #pragma unroll
-            for (int b = 0; b < 4; b++) {
-                uint32_t w[BW];
+                for (int b = 0; b < 32 / B; b++) {
+                    uint32_t w[BW];
 #pragma unroll
-                for (int i = 0; i < BW; i += 4) {
-                    const int at = (b * BW + i) * 4;
-                    *reinterpret_cast<uint4*>(w + i) = *reinterpret_cast<const uint4*>(line + at / 128 * C::BOX_BYTES + ((at % 128) ^ turn));
+                    for (int i = 0; i < BW; i += 4) {
+                        const int at = k2 * 2 * static_cast<int>(sizeof(T)) + (b * BW + i) * 4;
+                        *reinterpret_cast<uint4*>(w + i) = *reinterpret_cast<const uint4*>(line + at / 128 * C::BOX_BYTES + ((at % 128) ^ turn));
+                    }
+                    float v[B];
+                    unpack<T, B>(w, v);
+                    // the four scale bytes come in from the top
+                    word = word >> 8 | encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, c + b * (B / 8)) << 24;
                 }
-                float v[B];
-                unpack<T, B>(w, v);
-                uint32_t* out = B == 16 ? c + (b & 1) * 2 : c;
-                word |= encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, out) << (8 * b);
-                // 16 bytes: two blocks of 16, or one of 32
-                if (B == 32 || (b & 1)) {
-                    const size_t k2 = B == 32 ? b * 16 : b / 2 * 16;
-                    if (exists && tc * (COLS / 2ull) + k2 < pitch) *reinterpret_cast<uint4*>(to + k2) = make_uint4(c[0], c[1], c[2], c[3]);
-                }
+                if (exists && tc * (COLS / 2ull) + k2 < pitch) *reinterpret_cast<uint4*>(to + k2) = make_uint4(c[0], c[1], c[2], c[3]);
             }
             if (exists) *reinterpret_cast<uint32_t*>(scales + scale_word(row, tc, tiles_k)) = word;
         };
@@ -782,30 +775,32 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
             const long long col = tc * static_cast<long long>(COLS) + box * (128 / static_cast<int>(sizeof(T))) + lane * CPW;
             const size_t k0 = tr * 64ull + g * (COLS / 2);
             uint8_t* to = codes_t + col * pitch_t + k0;
-            uint32_t word[CPW], c[CPW][B / 8 * 2];
+            uint32_t word[CPW];
 #pragma unroll
             for (int h = 0; h < CPW; h++) word[h] = 0;
-#pragma unroll 2
-            for (int b = 0; b < 4; b++) {
-                uint32_t raw[B];
+#pragma unroll 1
+            for (int k2 = 0; k2 < COLS / 2; k2 += 16) {
+                uint32_t c[CPW][4];
 #pragma unroll
-                for (int j = 0; j < B; j++) raw[j] = *reinterpret_cast<const uint32_t*>(from + (b * B + j) * 128 + ((lane * 4) ^ ((j & 7) << 4)));
+                for (int b = 0; b < 32 / B; b++) {
+                    uint32_t raw[B];
 #pragma unroll
-                for (int h = 0; h < CPW; h++) {
-                    float v[B];
+                    for (int j = 0; j < B; j++) raw[j] = *reinterpret_cast<const uint32_t*>(from + (2 * k2 + b * B + j) * 128 + ((lane * 4) ^ ((j & 7) << 4)));
 #pragma unroll
-                    for (int j = 0; j < B; j++) {
-                        if constexpr (CPW == 1) v[j] = __uint_as_float(raw[j]);
-                        else if constexpr (std::is_same_v<T, __nv_bfloat16>) v[j] = __uint_as_float(h ? raw[j] & 0xFFFF0000u : raw[j] << 16);
-                        else v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(h ? raw[j] >> 16 : raw[j])));
-                    }
-                    uint32_t* out = B == 16 ? c[h] + (b & 1) * 2 : c[h];
-                    word[h] |= encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, out) << (8 * b);
-                    if (B == 32 || (b & 1)) {
-                        const size_t k2 = B == 32 ? b * 16 : b / 2 * 16;
-                        if (col + h < K && k0 + k2 < pitch_t) *reinterpret_cast<uint4*>(to + h * pitch_t + k2) = make_uint4(c[h][0], c[h][1], c[h][2], c[h][3]);
+                    for (int h = 0; h < CPW; h++) {
+                        float v[B];
+#pragma unroll
+                        for (int j = 0; j < B; j++) {
+                            if constexpr (CPW == 1) v[j] = __uint_as_float(raw[j]);
+                            else if constexpr (std::is_same_v<T, __nv_bfloat16>) v[j] = __uint_as_float(h ? raw[j] & 0xFFFF0000u : raw[j] << 16);
+                            else v[j] = __half2float(__ushort_as_half(static_cast<unsigned short>(h ? raw[j] >> 16 : raw[j])));
+                        }
+                        word[h] = word[h] >> 8 | encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, c[h] + b * (B / 8)) << 24;
                     }
                 }
+#pragma unroll
+                for (int h = 0; h < CPW; h++)
+                    if (col + h < K && k0 + k2 < pitch_t) *reinterpret_cast<uint4*>(to + h * pitch_t + k2) = make_uint4(c[h][0], c[h][1], c[h][2], c[h][3]);
             }
 #pragma unroll
             for (int h = 0; h < CPW; h++)
@@ -831,7 +826,14 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
                 along_columns(tile, tr, tc, C::BOXES == 4 ? q : q & 1, C::BOXES == 4 ? 0 : q >> 1);
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(empty0 + 8 * s);
+            if (lane == 0) {
+                __threadfence_block();
+                if ((atomicAdd(finished + s, 1u) & 3u) == 3u) {     // all four warps have read the tile
+                    __threadfence_block();
+                    if (tiles_all - n > C::STAGES * gridDim.x) request(n + C::STAGES * gridDim.x, s);
+                }
+            }
+            __syncwarp();
         }
     };
     if (FMT == RDB_FP4_NVFP4 && (scale.move != 1.0f || !partial)) body(std::true_type());
