@@ -871,6 +871,51 @@ def suite_quant(torch, R, quant, dev, stream, T=16384):
                       "per_tensor": {"us": round(us_t, 1), "gbs": round(by_t / us_t / 1e3, 1), "frac": round(by_t / us_t / 1e3 / peak_hbm, 3)}}}
 
 
+def suite_fp4(torch, R, dev, stream):
+    """The 4-bit path on the shapes of the other suites: quantisers on [16384, 8192] bf16 (and both directions at
+    4096 x 14336), the dense product at 4096^3 / 8192^3, the skinny product on the decode sweep's (N, K) at M = 1 and 16
+    (weights rotate past L2)."""
+    peak_hbm, _ = measured_peak()
+    cases = {}
+    T = 16384
+    xs = [torch.randn(T, 8192, device=dev).bfloat16() for _ in range(2)]
+    ts = (xs[0].abs().max().float() / 2688).reshape(1)
+    n = T * 8192
+    for form, block in (("mxfp4", 32), ("nvfp4", 16)):
+        us = _graph_time(torch, stream, lambda i: R.quantize_fp4(xs[i % 2], form, ts if form == "nvfp4" else None), 6)
+        by = n * 2 + n // 2 + n // block
+        cases[f"quantize_{form}"] = {"us": round(us, 1), "gbs": round(by / us / 1e3, 1), "frac": round(by / us / 1e3 / peak_hbm, 3)}
+    del xs
+    xs = [torch.randn(4096, 14336, device=dev).bfloat16() for _ in range(3)]
+    n = xs[0].numel()
+    for form, block in (("mxfp4", 32), ("nvfp4", 16)):
+        us = _graph_time(torch, stream, lambda i: R.quantize_fp4_both(xs[i % 3], form), 6)
+        by = n * 2 * (2 if form == "nvfp4" else 1) + 2 * (n // 2 + n // block)     # nvfp4: the maximum reads x first
+        cases[f"quantize_both_{form}"] = {"us": round(us, 1), "gbs": round(by / us / 1e3, 1), "frac": round(by / us / 1e3 / peak_hbm, 3)}
+    del xs
+    hold = lambda r, k, form: R.quantize_fp4(torch.randn(r, k, device=dev).bfloat16(), form)  # noqa: E731
+    for m in (4096, 8192):
+        for form in ("mxfp4", "nvfp4"):
+            A, B = hold(m, m, form), hold(m, m, form)
+            D = torch.empty(m, m, dtype=torch.bfloat16, device=dev)
+            us = _graph_time(torch, stream, lambda i: R.dense_gemm_fp4(A, B, out=D), 10)
+            cases[f"dense_{form}_{m}"] = {"us": round(us, 1), "tflops": round(2.0 * m ** 3 / us / 1e6, 1)}
+    for name, N, K in SHAPES:
+        copies = max(2, int(2.4e8 / (N * K * 0.5625)))
+        Ws = [hold(N, K, "nvfp4") for _ in range(copies)]
+        for M in (1, 16):
+            A = hold(M, K, "nvfp4")
+            D = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
+            us = _graph_time(torch, stream, lambda i: R.skinny_gemm_fp4(A, Ws[i % copies], out=D), 2 * copies)
+            ov = _graph_time(torch, stream, lambda i: R.skinny_gemm_fp4(A, Ws[i % copies], out=D, flags=R.OVERLAP_PRIOR_KERNEL), 2 * copies)
+            by = (N + M) * K * 0.5625 + 2 * M * N
+            cases[f"skinny_{name}_M{M}"] = {"us": round(us, 2), "gbs": round(by / us / 1e3, 1), "frac": round(by / us / 1e3 / peak_hbm, 3),
+                                            "overlapped_us": round(ov, 2)}
+        del Ws
+    return {"metric": "4-bit quantisers and products, device time", "unit": "us",
+            "roofline": {"bound": "hbm (quantisers, skinny), tensor (dense)", "peak": peak_hbm, "unit": "GB/s"}, "cases": cases}
+
+
 def run_suites_compact(torch, dist, R, quant, dev, rank, world, stream):
     """The other kernels of the scope table in a few hundred milliseconds, for
     the headline line's `suites` key: dense 8192^3 (rows sharded over the ranks
@@ -890,7 +935,7 @@ def run_suites_compact(torch, dist, R, quant, dev, rank, world, stream):
 def run_suite(args):
     """Measured lines for the other paths of the scope table (one JSON line per
     invocation): dense GEMM (config 2, row-sharded over the ranks), 2:4 sparse
-    GEMM (config 3), tiled_sum_reduce, the quantisers, the allreduce.  Not the
+    GEMM (config 3), tiled_sum_reduce, the quantisers, the 4-bit path, the allreduce.  Not the
     headline metric."""
     import torch
     import torch.distributed as dist
@@ -917,6 +962,8 @@ def run_suite(args):
         out.update(suite_reduce(torch, R, dev, stream))
     elif args.suite == "quant":
         out.update(suite_quant(torch, R, quant, dev, stream))
+    elif args.suite == "fp4":
+        out.update(suite_fp4(torch, R, dev, stream))
     elif args.suite == "allreduce":
         if world < 2:
             raise SystemExit("--suite allreduce needs torchrun with at least 2 ranks")
@@ -948,7 +995,7 @@ def main():
     ap.add_argument("--no-suites", action="store_true", help="skip the compact dense / sparse / reduce / quantiser block")
     ap.add_argument("--mode", default="grouped", choices=["grouped", "layer", "single"],
                     help="launch shape of the headline sweep (the other two are reported beside it in `modes`)")
-    ap.add_argument("--suite", default="", choices=["", "dense", "sparse", "reduce", "quant", "allreduce"],
+    ap.add_argument("--suite", default="", choices=["", "dense", "sparse", "reduce", "quant", "fp4", "allreduce"],
                     help="measure one of the other paths instead of the headline sweep")
     args = ap.parse_args()
     if args.impl == "reference":
