@@ -266,7 +266,9 @@ int rdb_dequantize_fp4(const uint8_t *codes, const uint8_t *scales, const float 
  * format, fp32 accumulation of exact products, D row-major, OVERWRITTEN.  The tensor scales are NULL for MXFP4.
  * rdb_skinny_gemm_fp4: the same for M <= 32, tuned for streaming B; flags as for rdb_skinny_gemm_fp8_tuned
  * (RDB_SKINNY_OVERLAP_PRIOR_KERNEL: B's codes and scales are requested before the preceding kernel of the stream has
- * finished, which must not write them).  No workspace: calls on different streams may overlap. */
+ * finished, which must not write them; nor may the one before that where the preceding one was launched with this flag by
+ * an fp8 entry, whose kernels let their successors start at once).  No workspace: calls on different streams may overlap.
+ * Make one call on each device before a stream capture (it sets up the device's status word). */
 int rdb_dense_gemm_fp4(const uint8_t *A, const uint8_t *scales_a, const float *tensor_scale_a, const uint8_t *B,
                        const uint8_t *scales_b, const float *tensor_scale_b, void *D, int out_type, int M, int N, int K,
                        int format, void *stream);

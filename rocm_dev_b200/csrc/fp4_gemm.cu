@@ -88,7 +88,6 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = tmem_slot;
-    pdl_launch_dependents();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -112,6 +111,9 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
             if (!p.early_b) pdl_wait_prior();
             for (int i = 0; i < pre; i++) load_b(i, stage0 + i * STAGE, full0 + 8 * i);
             if (p.early_b) pdl_wait_prior();
+            // the next kernel may start now that this one's predecessor has finished: one that fetches its weights early
+            // then overlaps this kernel alone, never one further back that may have written them
+            pdl_launch_dependents();
             for (int i = 0; i < pre; i++) load_a(i, stage0 + i * STAGE, full0 + 8 * i);
             for (int i = pre; i < nkb; i++) {
                 const int s = i % nstages;
@@ -314,8 +316,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     tc_fence_after_sync();
     const uint32_t tmem_base = tmem_slot;
     const int num_tiles = p.tiles_m * p.tiles_n;
-    pdl_launch_dependents();
     pdl_wait_prior();
+    pdl_launch_dependents();
 
     if (warp == 0 || warp == 6) {
         if (lane == 0) {

@@ -25,6 +25,13 @@ constexpr int kThreads = 256;
 constexpr int kAmaxBlocks = RDB_FP4_WORKSPACE_FLOATS;    // upper bound of the first pass's grid: one partial maximum each
 constexpr uint32_t kInf = 0x7F800000u;
 
+// The next kernel may start once this one's predecessor has finished, not before: a launch that fetches its weights early
+// then overlaps this kernel alone, never one further back that may have written them.
+__device__ __forceinline__ void start_after_prior() {
+    pdl_wait_prior();
+    pdl_launch_dependents();
+}
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -294,8 +301,7 @@ constexpr int kAmaxStretch = 1024;
 template <class T>
 __global__ void __launch_bounds__(kThreads) amax_kernel(const T* __restrict__ x, long long ldx, int rows, int K, uint32_t* __restrict__ partial) {
     __shared__ uint32_t warp_max[kThreads / 32];
-    pdl_launch_dependents();
-    pdl_wait_prior();
+    start_after_prior();
     constexpr int N = 16 / sizeof(T);
     const int lane = threadIdx.x & 31;
     const int per_row = (K - 1) / kAmaxStretch + 1;
@@ -354,8 +360,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
                                                                  const uint32_t* partial, int partials, uint8_t* __restrict__ codes,
                                                                  uint8_t* __restrict__ scales) {
     constexpr int B = Format<FMT>::BLOCK, WORDS = B * sizeof(T) / 4, HELD = WORDS > 16 ? 2 : 4;
-    pdl_launch_dependents();
-    pdl_wait_prior();
+    start_after_prior();
     const Scale scale = fetch_scale<T, FMT, kThreads>(tscale, partial, partials);
     const size_t pitch = row_bytes(K);
     const int tiles = scale_tiles_per_row(FMT, K);
@@ -424,8 +429,7 @@ __global__ void __launch_bounds__(kSmallThreads) quantize_small_kernel(const T* 
                                                                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     constexpr int B = 16, WORDS = B * sizeof(T) / 4, FMT = RDB_FP4_NVFP4;
     __shared__ uint32_t warp_max[kSmallThreads / 32], cta_max;
-    pdl_launch_dependents();
-    pdl_wait_prior();
+    start_after_prior();
     const size_t pitch = row_bytes(K);
     const int tiles = scale_tiles_per_row(FMT, K), per_row = 4 * tiles, total = rows * per_row, blocks = K / B;
     const int first = blockIdx.x * kSmallThreads + threadIdx.x, step = gridDim.x * kSmallThreads;
@@ -548,8 +552,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
     extern __shared__ __align__(16) uint32_t buffers[];
     uint8_t* sc = reinterpret_cast<uint8_t*>(buffers + C::BUFFERS * C::TILE_WORDS);     // [NB / 4][512] along the rows
     uint8_t* sc_t = sc + NB * 128;                                                      // the same along the columns
-    pdl_launch_dependents();
-    pdl_wait_prior();
+    start_after_prior();
     auto at = [](int r, int w) { return r * W + (w ^ (((r / B) & 3) << 3)); };
     const size_t pitch = row_bytes(K), pitch_t = row_bytes(rows);
     constexpr int V = W / 4, VE = 16 / sizeof(T), STEP = kTileThreads / V;     // vectors of a row, elements of a vector, rows a pass
@@ -722,7 +725,6 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
         for (int b = 0; b < C::BOXES; b++)
             tma_load_2d(smem_u32(smem) + s * C::STAGE + b * C::BOX_BYTES, &tm, tc * COLS + b * (128 / static_cast<int>(sizeof(T))), tr * 128, full0 + 8 * s, pol);
     };
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         prefetch_tensormap(&tm);
         for (int i = 0; i < C::STAGES; i++) {
@@ -734,7 +736,7 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
         for (int i = 0; i < C::STAGES && blockIdx.x + i * gridDim.x < tiles_all; i++) request(blockIdx.x + i * gridDim.x, i);
     }
     __syncthreads();
-    pdl_wait_prior();
+    start_after_prior();
     const Scale scale = fetch_scale<T, FMT, kBothThreads>(tscale, partial, partials);
 
     const size_t pitch = row_bytes(K), pitch_t = row_bytes(rows);
@@ -887,8 +889,7 @@ template <class T, int FMT>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                               const float* tscale, int rows, int K, int vec, T* __restrict__ out) {
     constexpr int B = Format<FMT>::BLOCK;
-    pdl_launch_dependents();
-    pdl_wait_prior();
+    start_after_prior();
     __shared__ __align__(16) T stage[kThreads / 32][256];
     const float t = FMT == RDB_FP4_NVFP4 ? *tscale : 1.0f;
     const size_t pitch = row_bytes(K);

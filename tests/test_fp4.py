@@ -701,3 +701,27 @@ def test_refusals_on_the_device(cuda_device):
         R.quantize_fp4(x, "nvfp4", torch.ones(1))
     with pytest.raises(ValueError):
         R.quantize_fp4(x[:, :0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_weights_written_two_launches_before_an_overlapping_one(cuda_device, form):
+    """The flag allows B to be requested while the PRECEDING kernel runs: what the one before that wrote has to be there,
+    however long it took."""
+    import rocm_dev_b200 as R
+    x = draw(4, 4096, 1).to(cuda_device)
+    scale = None if form == "mxfp4" else torch.full((1,), 1e-3, device=cuda_device)
+    ws = [(torch.randn((2048, 4096), generator=torch.Generator(cuda_device).manual_seed(s), device=cuda_device) * 0.1).bfloat16() for s in range(2)]
+    want = [R.skinny_gemm_fp4(R.quantize_fp4(x, form), R.quantize_fp4(w, form, scale)) for w in ws]
+    torch.cuda.synchronize()
+    s, w = torch.cuda.Stream(cuda_device), ws[0].clone()
+    g = torch.cuda.CUDAGraph()                              # launches follow one another faster than from Python
+    with torch.cuda.graph(g, stream=s):
+        W = R.quantize_fp4(w, form, scale)
+        got = R.skinny_gemm_fp4(R.quantize_fp4(x, form), W, flags=R.OVERLAP_PRIOR_KERNEL)
+    for i in range(20):
+        w.copy_(ws[i % 2])
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want[i % 2]), i
