@@ -686,7 +686,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
 // alternate tiles; the warp that is last to finish one requests the next into its place, and nothing else holds the warps
 // together (a ninth warp that only requested tiles cost the others a quarter of their registers).  A thread makes the four
 // blocks of one row, or of the one or two columns in a word: their scale bytes are a whole scale word, their codes whole
-// 16-byte stores, and no data passes between threads.  Bank conflicts: along a row the 8 lanes of a 16-byte phase hold 8
+// 32-byte stores, and no data passes between threads.  Bank conflicts: along a row the 8 lanes of a 16-byte phase hold 8
 // rows, whose chunks the swizzle spreads; along the columns the 32 lanes read the 32 words of one row.
 template <class T, int FMT>
 struct BothCfg {
@@ -702,6 +702,17 @@ struct BothCfg {
     static constexpr int SMEM = 1024 + STAGES * STAGE;
 };
 constexpr int kBothThreads = 256;
+
+// 32 bytes of codes at byte `at` of a row of `pitch` bytes (a multiple of 16), as far as they lie in it.  wide: rows start
+// on 32-byte boundaries.
+__device__ __forceinline__ void store32(uint8_t* p, const uint32_t* c, size_t at, size_t pitch, bool wide) {
+    if (wide) {
+        if (at < pitch) stg32(p, c);
+    } else {
+        if (at < pitch) *reinterpret_cast<uint4*>(p) = make_uint4(c[0], c[1], c[2], c[3]);
+        if (at + 16 < pitch) *reinterpret_cast<uint4*>(p + 16) = make_uint4(c[4], c[5], c[6], c[7]);
+    }
+}
 
 template <class T, int FMT>
 __global__ void __launch_bounds__(kBothThreads, BothCfg<T, FMT>::PER_SM)
@@ -740,6 +751,7 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
     const Scale scale = fetch_scale<T, FMT, kBothThreads>(tscale, partial, partials);
 
     const size_t pitch = row_bytes(K), pitch_t = row_bytes(rows);
+    const bool wide = ((reinterpret_cast<uintptr_t>(codes) | pitch) & 31) == 0, wide_t = ((reinterpret_cast<uintptr_t>(codes_t) | pitch_t) & 31) == 0;
     const int tiles_k = scale_tiles_per_row(FMT, K), tiles_r = scale_tiles_per_row(FMT, rows);
     const int group = warp >> 2, q = warp & 3;
     auto body = [&](auto careful) {
@@ -752,10 +764,10 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
             const bool exists = row < rows;
             uint32_t word = 0;
 #pragma unroll 1
-            for (int k2 = 0; k2 < COLS / 2; k2 += 16) {             // 16 bytes of codes: two blocks of 16, or one of 32
-                uint32_t c[4];
+            for (int k2 = 0; k2 < COLS / 2; k2 += 32) {             // 32 bytes of codes: four blocks of 16, or two of 32
+                uint32_t c[8];
 #pragma unroll
-                for (int b = 0; b < 32 / B; b++) {
+                for (int b = 0; b < 64 / B; b++) {
                     uint32_t w[BW];
 #pragma unroll
                     for (int i = 0; i < BW; i += 4) {
@@ -767,7 +779,7 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
                     // the four scale bytes come in from the top
                     word = word >> 8 | encode_block<T, FMT, decltype(careful)::value>(v, magnitude<B>(v), scale, c + b * (B / 8)) << 24;
                 }
-                if (exists && tc * (COLS / 2ull) + k2 < pitch) *reinterpret_cast<uint4*>(to + k2) = make_uint4(c[0], c[1], c[2], c[3]);
+                if (exists) store32(to + k2, c, tc * (COLS / 2ull) + k2, pitch, wide);
             }
             if (exists) *reinterpret_cast<uint32_t*>(scales + scale_word(row, tc, tiles_k)) = word;
         };
@@ -781,10 +793,10 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
 #pragma unroll
             for (int h = 0; h < CPW; h++) word[h] = 0;
 #pragma unroll 1
-            for (int k2 = 0; k2 < COLS / 2; k2 += 16) {
-                uint32_t c[CPW][4];
+            for (int k2 = 0; k2 < COLS / 2; k2 += 32) {
+                uint32_t c[CPW][8];
 #pragma unroll
-                for (int b = 0; b < 32 / B; b++) {
+                for (int b = 0; b < 64 / B; b++) {
                     uint32_t raw[B];
 #pragma unroll
                     for (int j = 0; j < B; j++) raw[j] = *reinterpret_cast<const uint32_t*>(from + (2 * k2 + b * B + j) * 128 + ((lane * 4) ^ ((j & 7) << 4)));
@@ -802,7 +814,7 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
                 }
 #pragma unroll
                 for (int h = 0; h < CPW; h++)
-                    if (col + h < K && k0 + k2 < pitch_t) *reinterpret_cast<uint4*>(to + h * pitch_t + k2) = make_uint4(c[h][0], c[h][1], c[h][2], c[h][3]);
+                    if (col + h < K) store32(to + h * pitch_t + k2, c[h], k0 + k2, pitch_t, wide_t);
             }
 #pragma unroll
             for (int h = 0; h < CPW; h++)

@@ -153,9 +153,29 @@ def test_scale_tiles_round_trip():
         assert (back.format, back.rows, back.K) == (f, rows, K) and torch.equal(back.scales, t.scales)
 
 
-def test_refusals_before_anything_is_launched():
+def _entries(through):
+    """The library's functions through ctypes, or through csrc/fastcall.c, which has to hand on every argument in its place."""
+    import types
+
     import rocm_dev_b200 as R
     L = R.lib()
+    if through == "ctypes":
+        return L
+    fast = pytest.importorskip("rocm_dev_b200._fastcall")
+    names = ("rdb_quantize_fp4", "rdb_dequantize_fp4", "rdb_dense_gemm_fp4_tuned", "rdb_skinny_gemm_fp4")
+    fast.bind(*(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names))
+    for f, n in ((fast.quantize, 14), (fast.dequantize, 9), (fast.dense, 15), (fast.skinny, 14)):
+        for bad in ([0] * (n - 1), [0] * (n + 1), ["x"] + [0] * (n - 1), [0] * (n - 1) + [1.5]):
+            with pytest.raises(TypeError):
+                f(*bad)
+    dense = lambda *a: fast.dense(*a[:12], 0, 0, a[12])  # noqa: E731
+    return types.SimpleNamespace(rdb_quantize_fp4=fast.quantize, rdb_dequantize_fp4=fast.dequantize, rdb_dense_gemm_fp4_tuned=fast.dense,
+                                 rdb_skinny_gemm_fp4=fast.skinny, rdb_dense_gemm_fp4=dense, rdb_skinny_gemm_fp4_tuned=L.rdb_skinny_gemm_fp4_tuned)
+
+
+@pytest.mark.parametrize("through", ["ctypes", "c"])
+def test_refusals_before_anything_is_launched(through):
+    L = _entries(through)
     buf = ctypes.create_string_buffer(4096)
     p = (ctypes.addressof(buf) + 255) // 256 * 256
     Q = lambda **k: L.rdb_quantize_fp4(*{**dict(x=p, typ=0, ldx=64, rows=4, K=64, fmt=1, ts=p, given=0, codes=p, scales=p, ct=None, st=None, ws=p, stream=None), **k}.values())  # noqa: E731
@@ -725,3 +745,33 @@ def test_weights_written_two_launches_before_an_overlapping_one(cuda_device, for
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want[i % 2]), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("shift", [0, 16, 32, 48])
+def test_quantized_buffers_at_any_16_bytes(cuda_device, form, shift):
+    """Codes and scales that start on 16 bytes but no more, and nothing written around them."""
+    import rocm_dev_b200 as R
+    from rocm_dev_b200 import fp4
+    rows, K = 96, 320
+    x = draw(rows, K, 1).to(cuda_device)
+    want_r, want_c = R.quantize_fp4_both(x, form)
+    sizes = [rows * fp4.row_bytes(K), fp4.scale_bytes(form, rows, K), K * fp4.row_bytes(rows), fp4.scale_bytes(form, K, rows)]
+    for both in (False, True):
+        bufs = [torch.full((n + 160,), 0xAB, dtype=torch.uint8, device=cuda_device) for n in sizes]
+        at = [b.data_ptr() + 16 + shift for b in bufs]
+        ts, ws = torch.empty(1, device=cuda_device), torch.empty(fp4.WORKSPACE_FLOATS, device=cuda_device)
+        code = R.lib().rdb_quantize_fp4(x.data_ptr(), 0, K, rows, K, fp4.FORMATS[form], ts.data_ptr(), 0, at[0], at[1], at[2] if both else None,
+                                        at[3] if both else None, ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert code == 0
+        parts = [b[16 + shift:16 + shift + n] for b, n in zip(bufs, sizes)]
+        if form == "nvfp4":
+            assert torch.equal(ts, want_r.tensor_scale)
+        for i, t in enumerate((want_r, want_c) if both else (want_r,)):
+            assert torch.equal(parts[2 * i].view(t.rows, -1), t.codes)
+            got = R.Fp4Tensor(parts[2 * i].clone().view(t.rows, -1), parts[2 * i + 1].clone(), None if form == "mxfp4" else ts, form, t.rows, t.K)
+            assert torch.equal(R.unpack_fp4_scales(got), R.unpack_fp4_scales(t))
+        for b, n, used in zip(bufs, sizes, (1, 1, both, both)):
+            assert (b[:16 + shift] == 0xAB).all() and (b[16 + shift + n:] == 0xAB).all()
+            assert used or (b == 0xAB).all()
