@@ -251,11 +251,12 @@ size_t rdb_fp4_scale_bytes(int format, int rows, int K);     /* 0 for an unsuppo
 
 /* Quantises x [rows, K] (row pitch ldx elements, x_type one of rdb_type), with blocks along the rows into codes / scales
  * and, where codes_t is not NULL, with blocks along the columns into codes_t / scales_t, the held form of the TRANSPOSED
- * tensor [K, rows] (what the gradients' products read); x is read once for both.  Both directions share the tensor scale, which is
- * written to tensor_scale[0], or read from it where scale_given is non-zero.  workspace: RDB_FP4_WORKSPACE_FLOATS floats
- * of scratch for an RDB_FP4_NVFP4 call that computes its scale (else may be NULL); nothing in it outlives the call. */
+ * tensor [K, rows] (what the gradients' products read); x is read once for both.  RDB_FP4_NVFP4: both directions share
+ * the tensor scale, which is taken from given_scale[0] or, where that is NULL, computed, and written to tensor_scale[0]
+ * either way; workspace: RDB_FP4_WORKSPACE_FLOATS floats of scratch for a call that computes its scale (else may be
+ * NULL), of which nothing outlives the call.  RDB_FP4_MXFP4: tensor_scale and given_scale are NULL. */
 int rdb_quantize_fp4(const void *x, int x_type, long long ldx, int rows, int K, int format, float *tensor_scale,
-                     int scale_given, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
+                     const float *given_scale, uint8_t *codes, uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t,
                      float *workspace, void *stream);
 
 /* out [rows, K] (contiguous, out_type) = element * scale * tensor scale, the last product in fp32, then rounded once. */

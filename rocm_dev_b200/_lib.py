@@ -53,7 +53,7 @@ _SIGNATURES = {
     "rdb_sparse_file_read": (i, [C.c_char_p, vp, C.c_size_t, vp, C.c_size_t]),
     "rdb_fp4_row_bytes": (C.c_size_t, [i]),
     "rdb_fp4_scale_bytes": (C.c_size_t, [i, i, i]),
-    "rdb_quantize_fp4": (i, [vp, i, C.c_longlong, i, i, i, vp, i, vp, vp, vp, vp, vp, vp]),
+    "rdb_quantize_fp4": (i, [vp, i, C.c_longlong, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp]),
     "rdb_dequantize_fp4": (i, [vp, vp, vp, i, i, i, vp, i, vp]),
     "rdb_dense_gemm_fp4": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, vp]),
     "rdb_dense_gemm_fp4_tuned": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, vp]),

@@ -48,7 +48,7 @@ static int numbers(PyObject *const *args, Py_ssize_t n, Py_ssize_t want, long lo
         return PyLong_FromLong(status);                                                  \
     }
 
-FUNCTION(quantize, 14, P(0), I(1), v[2], I(3), I(4), I(5), P(6), I(7), P(8), P(9), P(10), P(11), P(12), P(13))
+FUNCTION(quantize, 14, P(0), I(1), v[2], I(3), I(4), I(5), P(6), P(7), P(8), P(9), P(10), P(11), P(12), P(13))
 FUNCTION(dequantize, 9, P(0), P(1), P(2), I(3), I(4), I(5), P(6), I(7), P(8))
 FUNCTION(dense, 15, P(0), P(1), P(2), P(3), P(4), P(5), P(6), I(7), I(8), I(9), I(10), I(11), I(12), I(13), P(14))
 FUNCTION(skinny, 14, P(0), P(1), P(2), P(3), P(4), P(5), P(6), I(7), I(8), I(9), I(10), I(11), (unsigned)v[12], P(13))

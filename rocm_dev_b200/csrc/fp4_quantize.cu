@@ -274,7 +274,7 @@ __device__ __forceinline__ Scale scale_of_maximum(uint32_t m) {
 
 // The tensor scale (NVFP4: given, or from the first pass's partial maxima), for the whole block: every thread takes part.
 template <class T, int FMT, int THREADS>
-__device__ __forceinline__ Scale fetch_scale(float* tscale, const uint32_t* partial, int partials) {
+__device__ __forceinline__ Scale fetch_scale(float* tscale, const float* given, const uint32_t* partial, int partials) {
     Scale sc = {1.0f, 6.0f, 0.0f, 1.0f};
     if constexpr (FMT == RDB_FP4_NVFP4) {
         if (partial) {
@@ -287,10 +287,10 @@ __device__ __forceinline__ Scale fetch_scale(float* tscale, const uint32_t* part
 #pragma unroll
             for (int w = 0; w < THREADS / 32; w++) m = max(m, warp_max[w]);
             sc = scale_of_maximum<T>(m);
-            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *tscale = sc.t;
         } else {
-            sc = scale_of<T>(*tscale);
+            sc = scale_of<T>(*given);
         }
+        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *tscale = sc.t;
     }
     return sc;
 }
@@ -357,11 +357,11 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t* c) {
 // ALIGN: 32 or 16 bytes.
 template <class T, int FMT, int ALIGN>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int rows, int K, float* tscale,
-                                                                 const uint32_t* partial, int partials, uint8_t* __restrict__ codes,
+                                                                 const float* given, const uint32_t* partial, int partials, uint8_t* __restrict__ codes,
                                                                  uint8_t* __restrict__ scales) {
     constexpr int B = Format<FMT>::BLOCK, WORDS = B * sizeof(T) / 4, HELD = WORDS > 16 ? 2 : 4;
     start_after_prior();
-    const Scale scale = fetch_scale<T, FMT, kThreads>(tscale, partial, partials);
+    const Scale scale = fetch_scale<T, FMT, kThreads>(tscale, given, partial, partials);
     const size_t pitch = row_bytes(K);
     const int tiles = scale_tiles_per_row(FMT, K);
     const int lane = threadIdx.x & 31, b = blockIdx.x * 32 + lane, blocks = K / B;
@@ -545,7 +545,7 @@ __device__ __forceinline__ uint4 load_vector(const T* row, long long c, int K, b
 template <class T, int FMT, bool COLS>
 __global__ void __launch_bounds__(kTileThreads, TileCfg<T, FMT>::PER_SM)
 quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, int vec, unsigned tiles_x, unsigned tiles_all, float* tscale,
-                     const uint32_t* partial, int partials, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                     const float* given, const uint32_t* partial, int partials, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                      uint8_t* __restrict__ codes_t, uint8_t* __restrict__ scales_t) {
     using C = TileCfg<T, FMT>;
     constexpr int B = C::B, NB = C::NB, W = C::W, CPW = C::CPW, BW = B * sizeof(T) / 4;
@@ -596,7 +596,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
     int tr = static_cast<int>(tiles_y - 1 - blockIdx.x / tiles_x), tc = static_cast<int>(tiles_x - 1 - blockIdx.x % tiles_x);
     int ntr = tr, ntc = tc, turn = 0;
     fetch(tr, tc, buffers);
-    const Scale scale = fetch_scale<T, FMT, kTileThreads>(tscale, partial, partials);
+    const Scale scale = fetch_scale<T, FMT, kTileThreads>(tscale, given, partial, partials);
     auto body = [&](auto careful) {
     for (unsigned n = blockIdx.x; n < tiles_all; n += gridDim.x, turn ^= 1, tr = ntr, tc = ntc) {
         if (n + gridDim.x < tiles_all) {
@@ -716,7 +716,7 @@ __device__ __forceinline__ void store32(uint8_t* p, const uint32_t* c, size_t at
 
 template <class T, int FMT>
 __global__ void __launch_bounds__(kBothThreads, BothCfg<T, FMT>::PER_SM)
-quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, unsigned tiles_x, unsigned tiles_all, float* tscale, const uint32_t* partial,
+quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, unsigned tiles_x, unsigned tiles_all, float* tscale, const float* given, const uint32_t* partial,
                      int partials, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint8_t* __restrict__ codes_t,
                      uint8_t* __restrict__ scales_t, int* status) {
     using C = BothCfg<T, FMT>;
@@ -748,7 +748,7 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
     }
     __syncthreads();
     start_after_prior();
-    const Scale scale = fetch_scale<T, FMT, kBothThreads>(tscale, partial, partials);
+    const Scale scale = fetch_scale<T, FMT, kBothThreads>(tscale, given, partial, partials);
 
     const size_t pitch = row_bytes(K), pitch_t = row_bytes(rows);
     const bool wide = ((reinterpret_cast<uintptr_t>(codes) | pitch) & 31) == 0, wide_t = ((reinterpret_cast<uintptr_t>(codes_t) | pitch_t) & 31) == 0;
@@ -1004,7 +1004,7 @@ static int launch_tiles(int rows, int K, void** args, unsigned* tiles_x, unsigne
 }
 
 template <class T, int FMT>
-static int launch_both(const T* x, long long ldx, int rows, int K, float* tscale, uint32_t* partial, int partials, uint8_t* codes, uint8_t* scales,
+static int launch_both(const T* x, long long ldx, int rows, int K, float* tscale, const float* given, uint32_t* partial, int partials, uint8_t* codes, uint8_t* scales,
                        uint8_t* codes_t, uint8_t* scales_t, const DeviceInfo* info, cudaStream_t stream) {
     using C = BothCfg<T, FMT>;
     static bool attr_set[kMaxDevices] = {};
@@ -1024,13 +1024,13 @@ static int launch_both(const T* x, long long ldx, int rows, int K, float* tscale
     if (r != RDB_SUCCESS) return r;
     unsigned tiles_x = static_cast<unsigned>(tx), tiles_all = static_cast<unsigned>(all);
     int* status = info->status_dev;
-    void* args[] = {&tm, &rows, &K, &tiles_x, &tiles_all, &tscale, &partial, &partials, &codes, &scales, &codes_t, &scales_t, &status};
+    void* args[] = {&tm, &rows, &K, &tiles_x, &tiles_all, &tscale, &given, &partial, &partials, &codes, &scales, &codes_t, &scales_t, &status};
     const unsigned grid = static_cast<unsigned>(info->sm_count * C::PER_SM);
     return launch(reinterpret_cast<const void*>(kernel), dim3(tiles_all < grid ? tiles_all : grid), kBothThreads, C::SMEM, args, stream);
 }
 
 template <class T, int FMT>
-static int quantize(const void* x_, long long ldx, int rows, int K, float* tscale, bool given, uint8_t* codes, uint8_t* scales,
+static int quantize(const void* x_, long long ldx, int rows, int K, float* tscale, const float* given, uint8_t* codes, uint8_t* scales,
                     uint8_t* codes_t, uint8_t* scales_t, float* workspace, const DeviceInfo* info, cudaStream_t stream) {
     constexpr int B = Format<FMT>::BLOCK;
     const T* x = static_cast<const T*>(x_);
@@ -1059,7 +1059,7 @@ static int quantize(const void* x_, long long ldx, int rows, int K, float* tscal
         if (r != RDB_SUCCESS) return r;
     }
     if (direct) {
-        void* args[] = {&x, &ldx, &rows, &K, &tscale, &partial, &partials, &codes, &scales};
+        void* args[] = {&x, &ldx, &rows, &K, &tscale, &given, &partial, &partials, &codes, &scales};
         dim3 grid = octet_grid(rows, (4ll * scale_tiles_per_row(FMT, K) + 31) / 32);
         // what a block does once (the partial maxima) is shared by several octets where there are blocks enough: 16 per SM
         if (partial) {
@@ -1070,10 +1070,10 @@ static int quantize(const void* x_, long long ldx, int rows, int K, float* tscal
                       grid, kThreads, 0, args, stream);
     }
     if (codes_t && by16 && static_cast<unsigned long long>(row) < (1ull << 40))
-        return launch_both<T, FMT>(x, ldx, rows, K, tscale, partial, partials, codes, scales, codes_t, scales_t, info, stream);
+        return launch_both<T, FMT>(x, ldx, rows, K, tscale, given, partial, partials, codes, scales, codes_t, scales_t, info, stream);
     int vec = by16;
     unsigned tiles_x = 0, tiles_all = 0;
-    void* args[] = {&x, &ldx, &rows, &K, &vec, &tiles_x, &tiles_all, &tscale, &partial, &partials, &codes, &scales, &codes_t, &scales_t};
+    void* args[] = {&x, &ldx, &rows, &K, &vec, &tiles_x, &tiles_all, &tscale, &given, &partial, &partials, &codes, &scales, &codes_t, &scales_t};
     return codes_t ? launch_tiles<T, FMT, true>(rows, K, args, &tiles_x, &tiles_all, info->sm_count, stream) : launch_tiles<T, FMT, false>(rows, K, args, &tiles_x, &tiles_all, info->sm_count, stream);
 }
 
@@ -1105,23 +1105,23 @@ size_t rdb_fp4_scale_bytes(int format, int rows, int K) {
     return rdb::fp4::scale_bytes(format, rows, K);
 }
 
-int rdb_quantize_fp4(const void* x, int x_type, long long ldx, int rows, int K, int format, float* tensor_scale, int scale_given,
+int rdb_quantize_fp4(const void* x, int x_type, long long ldx, int rows, int K, int format, float* tensor_scale, const float* given_scale,
                      uint8_t* codes, uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t, float* workspace, void* stream) {
     using namespace rdb::fp4;
     const int ok = check(x_type, rows, K, format);
     if (ok != RDB_SUCCESS) return ok;
     if (ldx < K) return RDB_BAD_SHAPE;
     if (!x || !codes || !scales || (codes_t == nullptr) != (scales_t == nullptr)) return RDB_INVALID_CONFIG;
-    if (format == RDB_FP4_NVFP4 && (!tensor_scale || (!scale_given && !workspace))) return RDB_INVALID_CONFIG;
+    if (format == RDB_FP4_NVFP4 ? !tensor_scale || (!given_scale && !workspace) : tensor_scale || given_scale) return RDB_INVALID_CONFIG;
     const uintptr_t size = x_type == RDB_TYPE_FP32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(x) % size || !rdb::aligned16(codes) || !rdb::aligned16(scales) || !rdb::aligned16(codes_t) ||
-        !rdb::aligned16(scales_t) || (reinterpret_cast<uintptr_t>(tensor_scale) & 3u) || (reinterpret_cast<uintptr_t>(workspace) & 3u))
+        !rdb::aligned16(scales_t) || (reinterpret_cast<uintptr_t>(tensor_scale) & 3u) || (reinterpret_cast<uintptr_t>(given_scale) & 3u) || (reinterpret_cast<uintptr_t>(workspace) & 3u))
         return RDB_BAD_ALIGNMENT;
     int err = 0;
     rdb::DeviceInfo* info = rdb::device_info(&err);
     if (!info) return err;
     auto s = static_cast<cudaStream_t>(stream);
-#define RDB_QUANTIZE(T, F) quantize<T, F>(x, ldx, rows, K, tensor_scale, scale_given != 0, codes, scales, codes_t, scales_t, workspace, info, s)
+#define RDB_QUANTIZE(T, F) quantize<T, F>(x, ldx, rows, K, tensor_scale, given_scale, codes, scales, codes_t, scales_t, workspace, info, s)
     if (format == RDB_FP4_NVFP4)
         return x_type == RDB_TYPE_BF16 ? RDB_QUANTIZE(__nv_bfloat16, RDB_FP4_NVFP4) : x_type == RDB_TYPE_FP16 ? RDB_QUANTIZE(__half, RDB_FP4_NVFP4) : RDB_QUANTIZE(float, RDB_FP4_NVFP4);
     return x_type == RDB_TYPE_BF16 ? RDB_QUANTIZE(__nv_bfloat16, RDB_FP4_MXFP4) : x_type == RDB_TYPE_FP16 ? RDB_QUANTIZE(__half, RDB_FP4_MXFP4) : RDB_QUANTIZE(float, RDB_FP4_MXFP4);

@@ -57,40 +57,43 @@ def _type(dtype: torch.dtype) -> int:
 class Fp4Tensor:
     """A held tensor [rows, K]: ``codes`` uint8 [rows, row_bytes(K)], ``scales`` uint8 in tiles (flat, scale_bytes(format,
     rows, K)), ``tensor_scale`` fp32[1] (``nvfp4``) or None, all on ``device``."""
-    __slots__ = ("format", "rows", "K", "device", "_fmt", "_args", "_parts", "_buffer")
+    __slots__ = ("format", "rows", "K", "_fmt", "_parts", "_buffer", "_held")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, tensor_scale, format: str, rows: int, K: int):
         fmt = _format(format)
-        index = codes.get_device()
         if (codes.dtype is not _BYTE or codes.shape != (rows, (K + 31) // 32 * 16) or not codes.is_contiguous()
                 or scales.dtype is not _BYTE or scales.numel() != (rows + 127) // 128 * ((K + 255) // 256) * (2048 if fmt else 1024)
-                or not scales.is_contiguous() or scales.get_device() != index):
+                or not scales.is_contiguous()):
             raise ValueError(f"codes must be contiguous uint8 [{rows}, {row_bytes(K)}] and scales {scale_bytes(format, rows, K)} "
-                             "contiguous bytes on one device")
+                             "contiguous bytes")
         if fmt == 0:
             if tensor_scale is not None:
                 raise ValueError("mxfp4 has no tensor scale")
-            scale_ptr = None
-        elif (tensor_scale is None or tensor_scale.dtype is not torch.float32 or tensor_scale.numel() != 1
-              or tensor_scale.get_device() != index):
-            raise ValueError("nvfp4 needs a tensor scale: one fp32 on the device of the codes")
-        else:
-            scale_ptr = tensor_scale.data_ptr()
-        self._args = (codes.data_ptr(), scales.data_ptr(), scale_ptr)
-        self._parts = (codes, scales, tensor_scale)
-        self.format, self.rows, self.K, self.device, self._fmt = format, rows, K, codes.device, fmt
+        elif tensor_scale is None or tensor_scale.dtype is not torch.float32 or tensor_scale.numel() != 1:
+            raise ValueError("nvfp4 needs a tensor scale: one fp32")
+        self.format, self.rows, self.K, self._fmt = format, rows, K, fmt
+        self._parts, self._buffer, self._held = (codes, scales, tensor_scale), None, None
+        self._now()
+
+    def _now(self):
+        """(addresses of codes, scales and tensor scale, device): of a caller's tensors as they are at the call."""
+        held = self._held
+        if held is not None:
+            return held
+        codes, scales, ts = self._parts
+        dev = codes.device
+        if scales.device != dev or ts is not None and ts.device != dev:
+            raise ValueError("codes, scales and tensor scale must lie on one device")
+        return (codes.data_ptr(), scales.data_ptr(), None if ts is None else ts.data_ptr()), dev
 
     def _views(self):
-        # a quantiser's result is one allocation (codes, scales, tensor scale at the addresses in _args); its tensors are
-        # made when they are asked for
+        # a quantiser's result is one allocation, with the addresses in _held; its tensors are made when they are asked for
         if self._parts is None:
-            buf, given = self._buffer
-            base = buf.data_ptr()
-            codes, scales, ts = self._args
+            buf, base = self._buffer, self._buffer.data_ptr()
+            codes, scales, ts = (a if a is None else a - base for a in self._held[0])
             rb, sb = row_bytes(self.K), scale_bytes(self.format, self.rows, self.K)
-            part = lambda at, n: buf[at - base:at - base + n]  # noqa: E731
-            self._parts = (part(codes, self.rows * rb).view(self.rows, rb), part(scales, sb),
-                           given if ts is None or given is not None else part(ts, 4).view(torch.float32))
+            self._parts = (buf[codes:codes + self.rows * rb].view(self.rows, rb), buf[scales:scales + sb],
+                           None if ts is None else buf[ts:ts + 4].view(torch.float32))
         return self._parts
 
     @property
@@ -105,65 +108,69 @@ class Fp4Tensor:
     def tensor_scale(self):
         return self._views()[2]
 
+    @property
+    def device(self) -> torch.device:
+        return self._now()[1]
+
     def to(self, device) -> "Fp4Tensor":
         """The same tensor on another device (or on the host, to be stored)."""
         move = lambda t: None if t is None else t.to(device)  # noqa: E731
-        return Fp4Tensor(move(self.codes), move(self.scales), move(self.tensor_scale), self.format, self.rows, self.K)
+        return Fp4Tensor(*map(move, self._views()), self.format, self.rows, self.K)
+
+    def __reduce__(self):                        # copies and files hold the tensors, never an address
+        return Fp4Tensor, (*self._views(), self.format, self.rows, self.K)
 
     def __repr__(self) -> str:
         return f"Fp4Tensor({self.format}, [{self.rows}, {self.K}], {self.device})"
 
 
-def _device(dev: torch.device) -> int:
+def _index(dev: torch.device) -> int:
     if dev.type != "cuda":
         raise ValueError(f"device tensors required, got one on {dev} (there is no CPU path)")
     return dev.index
 
 
-class _Entries:
+def _bind():
     """The library's functions, through csrc/fastcall.c where it was built, else through ctypes."""
-
-    def __init__(self):
-        L = lib()
-        names = ("rdb_quantize_fp4", "rdb_dequantize_fp4", "rdb_dense_gemm_fp4_tuned", "rdb_skinny_gemm_fp4")
-        try:
-            from . import _fastcall as fast
-            fast.bind(*(C.cast(getattr(L, n), C.c_void_p).value for n in names))
-            found = (fast.quantize, fast.dequantize, fast.dense, fast.skinny)
-        except ImportError:
-            found = tuple(getattr(L, n) for n in names)
-        self.quantize, self.dequantize, self.dense, self.skinny = found
+    global _entries
+    L = lib()
+    names = ("rdb_quantize_fp4", "rdb_dequantize_fp4", "rdb_dense_gemm_fp4_tuned", "rdb_skinny_gemm_fp4")
+    try:
+        from . import _fastcall as fast
+        fast.bind(*(C.cast(getattr(L, n), C.c_void_p).value for n in names))
+        _entries = (fast.quantize, fast.dequantize, fast.dense, fast.skinny)
+    except ImportError:
+        _entries = tuple(getattr(L, n) for n in names)
+    return _entries
 
 
 _entries = None
+_QUANTIZE, _DEQUANTIZE, _DENSE, _SKINNY = range(4)
 
 
-def _call(name: str, dev: int, *args) -> None:
-    """The entry `name` with args and the current stream of device dev, dev being made the current device."""
-    global _entries
-    if _entries is None:
-        _entries = _Entries()
-    fn = getattr(_entries, name)
+def _call(which: int, where: str, dev: int, *args) -> None:
+    """Entry `which` with args and the current stream of device dev, dev being made the current device."""
+    fn = (_entries or _bind())[which]
     if _current_device() == dev:
         code = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
             code = fn(*args, _raw_stream(dev))
     if code:
-        check(code, f"{name} (4-bit)")
+        check(code, where)
 
 
-def _held(form: str, fmt: int, rows: int, K: int, dev, buffer, at: int, scales: int, scale_ptr) -> Fp4Tensor:
+def _result(form: str, fmt: int, rows: int, K: int, dev, buffer, addresses) -> Fp4Tensor:
     t = Fp4Tensor.__new__(Fp4Tensor)
-    t.format, t.rows, t.K, t.device, t._fmt = form, rows, K, dev, fmt
-    t._args, t._parts, t._buffer = (at, scales, scale_ptr), None, buffer
+    t.format, t.rows, t.K, t._fmt = form, rows, K, fmt
+    t._parts, t._buffer, t._held = None, buffer, (addresses, dev)
     return t
 
 
 def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
     fmt, typ = _format(format), _type(x.dtype)
     dev = x.device
-    index = _device(dev)
+    index = _index(dev)
     if x.dim() != 2:
         raise ValueError(f"a 2-D tensor is required, got {tuple(x.shape)}")
     rows, K = x.shape
@@ -175,34 +182,45 @@ def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
         ldx = K
     elif rows == 1:
         ldx = K
-    given = tensor_scale is not None
-    if given:
-        if fmt == 0:
+    # one allocation (every part a multiple of 16 bytes): codes and scales of either direction, then the tensor scale and
+    # the scratch that the call alone uses
+    per_word = 2048 if fmt else 1024              # scale bytes of 128 rows x 256 elements
+    at_s = rows * ((K + 31) // 32 * 16)
+    size = at_ct = at_s + (rows + 127) // 128 * ((K + 255) // 256) * per_word
+    if both:
+        at_st = at_ct + K * ((rows + 31) // 32 * 16)
+        size = at_st + (K + 127) // 128 * ((rows + 255) // 256) * per_word
+    given = scale = work = None
+    if fmt == 0:
+        if tensor_scale is not None:
             raise ValueError("mxfp4 has no tensor scale")
-        if not (tensor_scale.dtype is torch.float32 and tensor_scale.numel() == 1 and tensor_scale.device == dev):
-            raise ValueError(f"the tensor scale must be one fp32 on {dev}")
-    # one allocation (every part a multiple of 16 bytes): codes and scales of either direction, the tensor scale, and the
-    # scratch that the call alone uses
-    codes, scales = rows * ((K + 31) // 32 * 16), scale_bytes(format, rows, K)
-    codes_t, scales_t = (K * ((rows + 31) // 32 * 16), scale_bytes(format, K, rows)) if both else (0, 0)
-    own_scale = fmt == 1 and not given
-    buffer = torch.empty(codes + scales + codes_t + scales_t + (16 + 4 * WORKSPACE_FLOATS if own_scale else 0), dtype=torch.uint8, device=dev)
-    at = buffer.data_ptr()
-    at_s, at_ct = at + codes, at + codes + scales
-    at_st, end = at_ct + codes_t, at_ct + codes_t + scales_t
-    scale_ptr = end if own_scale else tensor_scale.data_ptr() if given else None
-    _call("quantize", index, x.data_ptr(), typ, ldx, rows, K, fmt, scale_ptr, given, at, at_s,
-          at_ct if both else None, at_st if both else None, end + 16 if own_scale else None)
-    held = (buffer, tensor_scale)
-    return (_held(format, fmt, rows, K, dev, held, at, at_s, scale_ptr),
-            _held(format, fmt, K, rows, dev, held, at_ct, at_st, scale_ptr) if both else None)
+        buffer = torch.empty(size, dtype=_BYTE, device=dev)
+        at = buffer.data_ptr()
+    else:
+        if tensor_scale is None:
+            buffer = torch.empty(size + 16 + 4 * WORKSPACE_FLOATS, dtype=_BYTE, device=dev)
+            at = buffer.data_ptr()
+            work = at + size + 16
+        else:
+            if not (tensor_scale.dtype is torch.float32 and tensor_scale.numel() == 1 and tensor_scale.device == dev):
+                raise ValueError(f"the tensor scale must be one fp32 on {dev}")
+            given = tensor_scale.data_ptr()
+            buffer = torch.empty(size + 16, dtype=_BYTE, device=dev)
+            at = buffer.data_ptr()
+        scale = at + size
+    if both:
+        _call(_QUANTIZE, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, scale, given, at, at + at_s, at + at_ct, at + at_st, work)
+        return (_result(format, fmt, rows, K, dev, buffer, (at, at + at_s, scale)),
+                _result(format, fmt, K, rows, dev, buffer, (at + at_ct, at + at_st, scale)))
+    _call(_QUANTIZE, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, scale, given, at, at + at_s, None, None, work)
+    return _result(format, fmt, rows, K, dev, buffer, (at, at + at_s, scale))
 
 
 def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None) -> Fp4Tensor:
     """x [rows, K] (bf16, fp16 or fp32; rows may be a pitch apart) -> held form, blocks along the rows.
     ``tensor_scale`` (``nvfp4``): a positive fp32[1] to use in place of max|x| / 2688 - a calibrated one, for which x is
-    read once instead of twice."""
-    return _quantize(x, format, tensor_scale, False)[0]
+    read once instead of twice.  Its value is copied: changing it later leaves the result as it is."""
+    return _quantize(x, format, tensor_scale, False)
 
 
 def quantize_fp4_both(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None):
@@ -212,20 +230,20 @@ def quantize_fp4_both(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torc
 
 def dequantize_fp4(t: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that codes and scales stand for, [rows, K] of ``dtype``."""
-    typ, index = _type(dtype), _device(t.device)
-    out = torch.empty(t.rows, t.K, dtype=dtype, device=t.device)
-    codes, scales, ts = t._args
-    _call("dequantize", index, codes, scales, ts, t._fmt, t.rows, t.K, out.data_ptr(), typ)
+    typ = _type(dtype)
+    (codes, scales, ts), dev = t._now()
+    index = _index(dev)
+    out = torch.empty(t.rows, t.K, dtype=dtype, device=dev)
+    _call(_DEQUANTIZE, "rdb_dequantize_fp4", index, codes, scales, ts, t._fmt, t.rows, t.K, out.data_ptr(), typ)
     return out
 
 
 def _product(A: Fp4Tensor, B: Fp4Tensor, out, out_dtype):
-    dev = A.device
-    index = _device(dev)
-    if B._fmt != A._fmt or B.K != A.K:
-        raise ValueError(f"operands of one format and depth are required: {A!r}, {B!r}")
-    if B.device != dev:
-        raise ValueError(f"operands on one device are required: {A!r}, {B!r}")
+    a, dev = A._now()
+    b, dev_b = B._now()
+    index = _index(dev)
+    if B._fmt != A._fmt or B.K != A.K or dev_b != dev:
+        raise ValueError(f"operands of one format and depth, on one device, are required: {A!r}, {B!r}")
     if out is None:
         typ = _type(out_dtype)
         out = torch.empty(A.rows, B.rows, dtype=out_dtype, device=dev)
@@ -233,7 +251,7 @@ def _product(A: Fp4Tensor, B: Fp4Tensor, out, out_dtype):
         typ = _type(out.dtype)
         if not (out.device == dev and out.is_contiguous() and out.shape == (A.rows, B.rows)):
             raise ValueError(f"out must be contiguous [{A.rows}, {B.rows}] on {dev}")
-    return (*A._args, *B._args, out.data_ptr(), typ, A.rows, B.rows, A.K, A._fmt), out, index
+    return (*a, *b, out.data_ptr(), typ, A.rows, B.rows, A.K, A._fmt), out, index
 
 
 def dense_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
@@ -241,7 +259,7 @@ def dense_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
     """D[M,N] = A . B^T over the values of A [M,K] and B [N,K], any sizes; fp32 accumulation, rounded once to
     ``out_dtype`` (``out``'s type where it is given).  ``tiling``, ``max_ctas``: the tuner's knobs, 0 = automatic."""
     args, out, index = _product(A, B, out, out_dtype)
-    _call("dense", index, *args, tiling, max_ctas)
+    _call(_DENSE, "rdb_dense_gemm_fp4", index, *args, tiling, max_ctas)
     return out
 
 
@@ -250,7 +268,7 @@ def skinny_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
     """The same product for at most 32 rows of A (decode): a stream over B.  ``flags``: 0 or ``OVERLAP_PRIOR_KERNEL`` (the
     launch may request B while the preceding kernel of the stream drains; that kernel must not write B)."""
     args, out, index = _product(A, B, out, out_dtype)
-    _call("skinny", index, *args, flags)
+    _call(_SKINNY, "rdb_skinny_gemm_fp4", index, *args, flags)
     return out
 
 

@@ -3,7 +3,9 @@
 Tolerance of a product, per element: half a step of the output type, 3 fp32 roundings for the tensor scales and their
 products, and the summation-order noise 4 sqrt(K) 2^-24 sum|a b| of an fp32 accumulation (as in the fp8 tests): the
 products themselves, and a block's scale times them, are exact."""
+import copy
 import ctypes
+import pickle
 
 import numpy as np
 import pytest
@@ -151,6 +153,9 @@ def test_scale_tiles_round_trip():
         assert torch.equal(R.unpack_fp4_scales(t), s)
         back = t.to("cpu")
         assert (back.format, back.rows, back.K) == (f, rows, K) and torch.equal(back.scales, t.scales)
+        for again in (copy.deepcopy(t), pickle.loads(pickle.dumps(t))):
+            assert torch.equal(again.codes, t.codes) and torch.equal(again.scales, t.scales) and repr(again) == repr(t)
+            assert again._now()[0][0] == again.codes.data_ptr() != t.codes.data_ptr()
 
 
 def _entries(through):
@@ -178,10 +183,10 @@ def test_refusals_before_anything_is_launched(through):
     L = _entries(through)
     buf = ctypes.create_string_buffer(4096)
     p = (ctypes.addressof(buf) + 255) // 256 * 256
-    Q = lambda **k: L.rdb_quantize_fp4(*{**dict(x=p, typ=0, ldx=64, rows=4, K=64, fmt=1, ts=p, given=0, codes=p, scales=p, ct=None, st=None, ws=p, stream=None), **k}.values())  # noqa: E731
+    Q = lambda **k: L.rdb_quantize_fp4(*{**dict(x=p, typ=0, ldx=64, rows=4, K=64, fmt=1, ts=p, given=None, codes=p, scales=p, ct=None, st=None, ws=p, stream=None), **k}.values())  # noqa: E731
     assert Q(rows=0) == 8 and Q(K=0) == 8 and Q(ldx=63) == 8
     assert Q(fmt=2) == 6 and Q(typ=3) == 6 and Q(x=None) == 6 and Q(codes=None) == 6 and Q(scales=None) == 6
-    assert Q(ts=None) == 6 and Q(ws=None) == 6 and Q(ct=p) == 6
+    assert Q(ts=None) == 6 and Q(ws=None) == 6 and Q(ct=p) == 6 and Q(fmt=0) == 6 and Q(fmt=0, ts=None, given=p) == 6 and Q(given=p + 2) == 7
     assert Q(x=p + 1) == 7 and Q(codes=p + 8) == 7 and Q(scales=p + 4) == 7 and Q(ts=p + 2) == 7 and Q(typ=2, x=p + 2) == 7
     D = lambda **k: L.rdb_dequantize_fp4(*{**dict(codes=p, scales=p, ts=p, fmt=1, rows=4, K=64, out=p, typ=0, stream=None), **k}.values())  # noqa: E731
     assert D(rows=0) == 8 and D(fmt=-1) == 6 and D(typ=9) == 6 and D(ts=None) == 6 and D(out=None) == 6 and D(out=p + 1) == 7
@@ -593,6 +598,30 @@ def test_new_values_in_the_same_buffers_are_seen(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_copies_and_moved_tensors(cuda_device, form):
+    """A held tensor that was copied, stored, or whose codes got other memory is read where it lies now."""
+    import rocm_dev_b200 as R
+    x = draw(33, 300, 1).to(cuda_device)
+    t, c = R.quantize_fp4_both(x, form)
+    for q, v in ((t, x), (c, x.t())):
+        want = R.dequantize_fp4(q)
+        for again in (copy.deepcopy(q), pickle.loads(pickle.dumps(q)), q.to("cpu").to(cuda_device)):
+            assert torch.equal(R.dequantize_fp4(again), want) and again.codes.data_ptr() != q.codes.data_ptr()
+    if form == "nvfp4":
+        one = torch.ones(1, device=cuda_device)
+        q = R.quantize_fp4(x, form, one)
+        want = R.dequantize_fp4(q)
+        one.fill_(2.0)                                       # a calibration that moves on
+        assert torch.equal(R.dequantize_fp4(q), want) and q.tensor_scale.item() == 1.0
+    del q, again
+    own = copy.deepcopy(t)
+    own.codes.data = torch.zeros_like(own.codes)             # what module.to() does to its parameters
+    torch.cuda.empty_cache()
+    assert not R.dequantize_fp4(own).any()
+
+
+@pytest.mark.gpu
 def test_another_device_than_the_current_one(cuda_device):
     import rocm_dev_b200 as R
     if torch.cuda.device_count() < 2:
@@ -762,7 +791,7 @@ def test_quantized_buffers_at_any_16_bytes(cuda_device, form, shift):
         bufs = [torch.full((n + 160,), 0xAB, dtype=torch.uint8, device=cuda_device) for n in sizes]
         at = [b.data_ptr() + 16 + shift for b in bufs]
         ts, ws = torch.empty(1, device=cuda_device), torch.empty(fp4.WORKSPACE_FLOATS, device=cuda_device)
-        code = R.lib().rdb_quantize_fp4(x.data_ptr(), 0, K, rows, K, fp4.FORMATS[form], ts.data_ptr(), 0, at[0], at[1], at[2] if both else None,
+        code = R.lib().rdb_quantize_fp4(x.data_ptr(), 0, K, rows, K, fp4.FORMATS[form], None if form == "mxfp4" else ts.data_ptr(), None, at[0], at[1], at[2] if both else None,
                                         at[3] if both else None, ws.data_ptr(), torch.cuda.current_stream().cuda_stream)
         assert code == 0
         parts = [b[16 + shift:16 + shift + n] for b, n in zip(bufs, sizes)]
