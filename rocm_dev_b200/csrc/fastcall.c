@@ -1,6 +1,6 @@
 /* CPython entry to the short calls of the library: the same functions that ctypes reaches, with their arguments converted
- * in C.  A 4-bit product of one token takes 6 us on the device; ctypes spends 1.3 us on the conversion of its 14
- * arguments, this 0.3.  Optional: without it (no Python headers) the package calls through ctypes.
+ * in C.  A 4-bit product of one token takes 6 us on the device; ctypes spends 1.2 us on a call with its 14
+ * arguments.  Optional: without it (no Python headers) the package calls through ctypes.
  *   bind(quantize, dequantize, dense, skinny)   addresses of the library's functions, once
  *   quantize(...), dequantize(...), dense(...), skinny(...)   their arguments in order, None for NULL; returns the status */
 #define PY_SSIZE_T_CLEAN

@@ -297,6 +297,8 @@ __device__ __forceinline__ Scale fetch_scale(float* tscale, const float* given, 
 
 // First pass of a call that computes the tensor scale: one partial maximum per CTA.  A warp takes stretches of 1024
 // elements of a row: single elements up to the first 16-byte boundary and behind the last, whole vectors between them.
+// Bound by HBM: 4096 x 14336 bf16 (117 MB) takes 24 us before the row quantiser, 15 to 17 before the two-way one, which
+// begins with the rows that were read last.
 constexpr int kAmaxStretch = 1024;
 template <class T>
 __global__ void __launch_bounds__(kThreads) amax_kernel(const T* __restrict__ x, long long ldx, int rows, int K, uint32_t* __restrict__ partial) {
@@ -354,7 +356,8 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t* c) {
 // Blocks along the rows, x on 16-byte boundaries and K a multiple of the block: a thread holds a whole block, so nothing
 // but the scale bytes passes between threads.  A warp takes 32 blocks of the rows r, r + 32, r + 64, r + 96 of a 128-row
 // tile: four loads in flight, and the four scale words of a lane quartet are 16 consecutive bytes of the scale tile.
-// ALIGN: 32 or 16 bytes.
+// ALIGN: 32 or 16 bytes.  Bound by HBM: 4096 x 14336 bf16 takes 24 us in MXFP4 and 25 in NVFP4 with a given scale (23 at
+// the copy rate), fp32 46 (42).
 template <class T, int FMT, int ALIGN>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int rows, int K, float* tscale,
                                                                  const float* given, const uint32_t* partial, int partials, uint8_t* __restrict__ codes,
@@ -542,6 +545,8 @@ __device__ __forceinline__ uint4 load_vector(const T* row, long long c, int K, b
     return *reinterpret_cast<const uint4*>(e);
 }
 
+// Bound by instructions (shifted loads, a transpose through shared memory): 4096 x 14336 bf16 off 16 bytes takes 60 us by
+// rows, both ways 74 in MXFP4 and 82 in NVFP4, where aligned rows take 24, 34 and 50.
 template <class T, int FMT, bool COLS>
 __global__ void __launch_bounds__(kTileThreads, TileCfg<T, FMT>::PER_SM)
 quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, int vec, unsigned tiles_x, unsigned tiles_all, float* tscale,
@@ -714,6 +719,9 @@ __device__ __forceinline__ void store32(uint8_t* p, const uint32_t* c, size_t at
     }
 }
 
+// 4096 x 14336 bf16 takes 34 us in MXFP4 and 48 to 50 in NVFP4 (28 at the copy rate).  NVFP4, with two scales in 32 elements
+// and a division for each, is bound by instructions: without loads and stores 43 us of 48 remain (MXFP4 26 of 37), issue
+// slots are 58 % busy.  Two CTAs of 127 registers per SM; three of 80 took 74 us where two took 50, both measured cold.
 template <class T, int FMT>
 __global__ void __launch_bounds__(kBothThreads, BothCfg<T, FMT>::PER_SM)
 quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, unsigned tiles_x, unsigned tiles_all, float* tscale, const float* given, const uint32_t* partial,
@@ -896,7 +904,7 @@ __device__ __forceinline__ void decode_block(uint32_t codes, uint32_t scale, flo
 // A warp takes 256 elements (8 per lane) of the rows r, r + 32, r + 64, r + 96 of a 128-row tile: their scale words are one
 // 16-byte load.  element * scale is exact in fp32, the tensor scale's product rounds, the output type rounds again.
 // vec: rows of the output start on boundaries of 8 elements; else the values pass through shared memory, so that neighbouring
-// lanes store neighbouring elements.
+// lanes store neighbouring elements.  Bound by HBM: 4096 x 14336 takes 25 us to bf16, 43 to fp32.
 template <class T, int FMT>
 __global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                               const float* tscale, int rows, int K, int vec, T* __restrict__ out) {
@@ -1038,13 +1046,14 @@ static int quantize(const void* x_, long long ldx, int rows, int K, float* tscal
     const bool by32 = (reinterpret_cast<uintptr_t>(x) & 31u) == 0 && row % 32 == 0, by16 = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && row % 16 == 0;
     const bool direct = !codes_t && by16 && K % B == 0;      // a thread can take whole blocks straight from memory
     const long long all_blocks = 4ll * scale_tiles_per_row(FMT, K) * rows;
-    // 4 blocks a thread, 8 CTAs: a launch and a pass over x less (8 x 4096 bf16: 2.4 us against 3.7)
-    if (FMT == RDB_FP4_NVFP4 && !given && direct && all_blocks <= 4ll * kSmallCluster * kSmallThreads) {
+    // Up to 2 blocks a thread of 8 CTAs: a launch and a pass over x less (bf16, 8 x 4096: 2.6 us against 3.4 in two
+    // launches, 32 x 4096: 3.2 against 3.5).  Beyond that one cluster is slower than all SMs: 32 x 8192 took 4.6 against 3.6.
+    if (FMT == RDB_FP4_NVFP4 && !given && direct && all_blocks <= 2ll * kSmallCluster * kSmallThreads) {
         void* args[] = {&x, &ldx, &rows, &K, &tscale, &codes, &scales};
         int ctas = 1;
         while (ctas < kSmallCluster && all_blocks > static_cast<long long>(ctas) * kSmallThreads) ctas *= 2;
         return launch(all_blocks <= static_cast<long long>(ctas) * kSmallThreads ? reinterpret_cast<const void*>(quantize_small_kernel<T, 1>)
-                                                                                 : reinterpret_cast<const void*>(quantize_small_kernel<T, 4>),
+                                                                                 : reinterpret_cast<const void*>(quantize_small_kernel<T, 2>),
                       dim3(ctas), kSmallThreads, 0, args, stream, ctas);
     }
     uint32_t* partial = nullptr;
