@@ -235,7 +235,7 @@ int rdb_dense_gemm_fp8_f32(const uint8_t *A, const uint8_t *B, float *D, int M, 
  *                  magnitude / (6 t)); element = e2m1(x / (t s)), zero where s is.  6 t, t s and both quotients are
  *                  rounded to fp32.  t must be a positive number.
  * A block that holds an infinity or a NaN gets the scale type's NaN, and what is computed from it is NaN.
- * A held tensor [rows, K], for any rows, K >= 1:
+ * A held tensor [rows, K], rows and K from 1 to 2^31 - 1025 (more: RDB_SIZE_ABOVE_LIMIT):
  *   codes   [rows, rdb_fp4_row_bytes(K)] bytes (ceil(K / 32) * 16), two codes to a byte, the even index in the low half,
  *           zero codes behind K;
  *   scales  rdb_fp4_scale_bytes(format, rows, K) bytes in tiles of 128 rows x 4 blocks (512 bytes): row r, block b of a

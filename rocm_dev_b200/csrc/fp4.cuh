@@ -19,6 +19,8 @@ namespace fp4 {
 
 constexpr int STAGE_K = 256;             // elements of K per pipeline stage and granularity of the scale tiles
 constexpr int TILE_BYTES = 512;          // 128 rows x 4 scale bytes
+// Most rows and columns of a tensor: indices rounded up to whole tiles and read-ahead within them stay below 2^31.
+constexpr int MAX_EXTENT = 2147483647 - 1024;
 
 template <int FMT>
 struct Format {

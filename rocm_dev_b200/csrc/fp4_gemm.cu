@@ -659,6 +659,7 @@ static int launch_pair(const Product& q, int max_ctas, const DeviceInfo* info, c
 static int check(const Product& q, int format) {
     if (q.M < 1 || q.N < 1 || q.K < 1) return RDB_BAD_SHAPE;
     if (format != RDB_FP4_MXFP4 && format != RDB_FP4_NVFP4) return RDB_INVALID_CONFIG;
+    if (q.M > MAX_EXTENT || q.N > MAX_EXTENT || q.K > MAX_EXTENT) return RDB_SIZE_ABOVE_LIMIT;
     if (q.out_type != RDB_TYPE_BF16 && q.out_type != RDB_TYPE_FP16 && q.out_type != RDB_TYPE_FP32) return RDB_INVALID_CONFIG;
     if (!q.A || !q.sa || !q.B || !q.sb || !q.D) return RDB_INVALID_CONFIG;
     if (format == RDB_FP4_NVFP4 ? !q.ta || !q.tb : q.ta || q.tb) return RDB_INVALID_CONFIG;

@@ -1099,6 +1099,7 @@ static int check(int type, int rows, int K, int format) {
     if (rows < 1 || K < 1) return RDB_BAD_SHAPE;
     if (format != RDB_FP4_MXFP4 && format != RDB_FP4_NVFP4) return RDB_INVALID_CONFIG;
     if (type != RDB_TYPE_BF16 && type != RDB_TYPE_FP16 && type != RDB_TYPE_FP32) return RDB_INVALID_CONFIG;
+    if (rows > MAX_EXTENT || K > MAX_EXTENT) return RDB_SIZE_ABOVE_LIMIT;
     return RDB_SUCCESS;
 }
 

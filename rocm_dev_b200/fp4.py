@@ -22,6 +22,7 @@ FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 WORKSPACE_FLOATS = 1024
+MAX_EXTENT = 2 ** 31 - 1025                   # rows and columns of a tensor
 _BYTE = torch.uint8
 
 # A step's calls are short: what a call costs on the host shows.  These two are the cheap forms of
@@ -61,6 +62,8 @@ class Fp4Tensor:
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, tensor_scale, format: str, rows: int, K: int):
         fmt = _format(format)
+        if rows > MAX_EXTENT or K > MAX_EXTENT:
+            raise ValueError(f"a held tensor has at most {MAX_EXTENT} rows and columns, got [{rows}, {K}]")
         if (codes.dtype is not _BYTE or codes.shape != (rows, (K + 31) // 32 * 16) or not codes.is_contiguous()
                 or scales.dtype is not _BYTE or scales.numel() != (rows + 127) // 128 * ((K + 255) // 256) * (2048 if fmt else 1024)
                 or not scales.is_contiguous()):
@@ -169,13 +172,15 @@ def _result(form: str, fmt: int, rows: int, K: int, dev, buffer, addresses) -> F
 
 def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
     fmt, typ = _format(format), _type(x.dtype)
-    dev = x.device
-    index = _index(dev)
     if x.dim() != 2:
         raise ValueError(f"a 2-D tensor is required, got {tuple(x.shape)}")
     rows, K = x.shape
     if rows < 1 or K < 1:
         raise ValueError(f"an empty tensor cannot be quantised: {tuple(x.shape)}")
+    if rows > MAX_EXTENT or K > MAX_EXTENT:
+        raise ValueError(f"at most {MAX_EXTENT} rows and columns can be quantised: {tuple(x.shape)}")
+    dev = x.device
+    index = _index(dev)
     ldx, unit = x.stride()
     if unit != 1 and K > 1 or ldx < K and rows > 1:
         x = x.contiguous()                        # transposed or overlapping views

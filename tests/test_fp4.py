@@ -227,6 +227,31 @@ def test_refusals_of_the_python_face():
             call()
 
 
+@pytest.mark.parametrize("through", ["ctypes", "c"])
+def test_extents_beyond_32_bit_indices_are_refused(through):
+    """Either entry hands on 32 bits of a size; beyond 2^31 - 1025 tile-rounded indices would overflow."""
+    import rocm_dev_b200 as R
+    L, most = _entries(through), 2 ** 31 - 1025
+    buf = ctypes.create_string_buffer(512)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    for rows, K in ((most + 1, 1), (1, most + 1), (2 ** 31 - 1, 2 ** 31 - 1)):
+        assert L.rdb_quantize_fp4(p, 0, 2 ** 40, rows, K, 1, p, None, p, p, None, None, p, None) == 11
+        assert L.rdb_dequantize_fp4(p, p, p, 1, rows, K, p, 0, None) == 11
+        for M, N, k in ((rows, 1, K), (1, rows, K), (rows, K, 1)):
+            assert L.rdb_dense_gemm_fp4(p, p, p, p, p, p, p, 0, M, N, k, 1, None) == 11
+            assert L.rdb_skinny_gemm_fp4(p, p, p, p, p, p, p, 0, M, N, k, 1, 0, None) == 11
+    for n in (most + 1, 2 ** 32 + 5):
+        for shape in ((n, 1), (1, n)):
+            wide = torch.zeros((1, 1), dtype=torch.bfloat16).expand(shape)
+            for call in (R.quantize_fp4, R.quantize_fp4_both):
+                with pytest.raises(ValueError, match=str(most)):
+                    call(wide)
+            codes = torch.empty((shape[0], (shape[1] + 31) // 32 * 16), dtype=torch.uint8, device="meta")
+            scales = torch.empty((shape[0] + 127) // 128 * ((shape[1] + 255) // 256) * 1024, dtype=torch.uint8, device="meta")
+            with pytest.raises(ValueError, match=str(most)):
+                R.Fp4Tensor(codes, scales, None, "mxfp4", *shape)
+
+
 # ------------------------------------------------------------------ quantisers
 SHAPES = [(1, 1), (1, 16), (2, 17), (3, 31), (5, 32), (8, 4096), (130, 257), (33, 1000), (257, 129), (700, 48)]
 
