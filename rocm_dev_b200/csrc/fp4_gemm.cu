@@ -187,13 +187,23 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         tc_fence_before_sync();
     }
     __syncthreads();
+    const bool aborted = *abort_flag != 0;                   // every wait that can set it lies behind
+    if (aborted) {
+        for (int i = 0; i < 64; i++) __nanosleep(2000);      // MMAs and copies in flight land before their memory is given back
+    }
+    // TMEM goes back before this CTA waits for its peers: more CTAs may share an SM than its 512 columns serve, and one of
+    // the peers may still wait for columns.  Two clusters that each held some and waited for the other's would hang.
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, p.tmem_cols);
+    }
     if (S > 1) {
         cluster_arrive_release();
         cluster_wait_acquire();                              // every rank's partial sums are in place
     }
     pdl_wait_prior();                                        // D may belong to the preceding kernel
     const float alpha = alpha_s;
-    if (*abort_flag == 0) {
+    if (!aborted) {
         // columns in granules of four; rank r sums and stores [G r / S, G (r + 1) / S)
         const int G = R / 4, g0 = G * rank / S, ng = G * (rank + 1) / S - g0;
         for (int item = threadIdx.x; item < rows * ng; item += SPLIT_THREADS) {
@@ -224,13 +234,9 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                 store4(p.D, p.out_type, p.N, m0 + m, n0 + c, v, p.vec);
             }
         }
-    } else {
-        for (int i = 0; i < 64; i++) __nanosleep(2000);      // copies in flight land before the memory is given back
     }
-    tc_fence_before_sync();
-    __syncthreads();
-    if (warp == 1) tmem_dealloc(tmem_base, p.tmem_cols);
     if (S > 1) {                                             // no rank leaves while another still reads its memory
+        __syncwarp();
         cluster_arrive_release();
         cluster_wait_acquire();
     }
