@@ -86,6 +86,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     return true;
 }
 
+// After a wait ran out: time for MMAs and copies in flight to land before their memory is given back.
+__device__ __forceinline__ void drain_after_abort() {
+#pragma unroll 1
+    for (int i = 0; i < 64; i++) __nanosleep(2000);
+}
+
+// Barrier `id` (1..15; 0 is __syncthreads) between `threads` threads of the CTA, some of which only arrive.
+__device__ __forceinline__ void named_barrier_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void named_barrier_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
 // Records a timed-out wait in the (host-mapped) status word.
 __device__ __forceinline__ void report_timeout(int* status) { *reinterpret_cast<volatile int*>(status) = 10; }
 

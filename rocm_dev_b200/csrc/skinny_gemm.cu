@@ -263,7 +263,18 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             }
         }
         if (warp == TMEM_WARP && lane == 0) stamp(p, TR_EPI_LOADED);
+        tc_fence_before_sync();
+        named_barrier_arrive(1, 96);
+    } else if (warp == 1) {
+        // TMEM goes back before this CTA waits for its peers: more CTAs may share an SM than its 512 columns serve, and
+        // one of the peers may still wait for columns.  Two clusters that each held some and waited for the other's
+        // would hang.
+        named_barrier_sync(1, 96);         // both reading warps are done
+        if (*abort_flag != 0) drain_after_abort();
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, p.tmem_cols);
     }
+    __syncwarp();
     if (S > 1) cluster_wait_acquire();     // phase 1 complete: every peer's barriers and buffers are live
     if (p.pdl) pdl_wait_prior();           // D and the scales may belong to the preceding kernel
     __syncthreads();
@@ -332,12 +343,8 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
 
     // ---- teardown: after an abort give in-flight TMA copies time to land
-    if (*abort_flag != 0) {
-        for (int i = 0; i < 64; i++) __nanosleep(2000);
-    }
-    tc_fence_before_sync();
+    if (*abort_flag != 0) drain_after_abort();
     __syncthreads();
-    if (warp == 1) tmem_dealloc(tmem_base, p.tmem_cols);
     if (threadIdx.x == 0) stamp(p, TR_EXIT);
 }
 
