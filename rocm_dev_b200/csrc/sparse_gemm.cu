@@ -291,7 +291,18 @@ sparse_gemm_kernel(const __grid_constant__ GParams g) {
                 for (int j = 0; j < 16; j++) col[(c0 + j) * pitch] = v[j];
             }
         }
+        tc_fence_before_sync();
+        named_barrier_arrive(1, 160);
+    } else if (warp == 1) {
+        // TMEM goes back before this CTA waits for its peers: more CTAs may share an SM than its 512 columns serve, and
+        // one of the peers may still wait for columns.  Two clusters that each held some and waited for the other's
+        // would hang.
+        named_barrier_sync(1, 160);                        // the four reading warps are done
+        if (*abort_flag != 0) drain_after_abort();
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, p.tmem_cols);
     }
+    __syncwarp();
     if (S > 1) cluster_wait_acquire();
     __syncthreads();
     if (p.pdl) pdl_wait_prior();                       // D may still be read by the preceding kernel's successors
@@ -349,12 +360,8 @@ sparse_gemm_kernel(const __grid_constant__ GParams g) {
     }
 
     if (threadIdx.x == 0) stamp(p, 6);
-    if (*abort_flag != 0) {
-        for (int i = 0; i < 64; i++) __nanosleep(2000);
-    }
-    tc_fence_before_sync();
+    if (*abort_flag != 0) drain_after_abort();
     __syncthreads();
-    if (warp == 1) tmem_dealloc(tmem_base, p.tmem_cols);
     if (threadIdx.x == 0) stamp(p, 7);
 }
 

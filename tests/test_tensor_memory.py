@@ -21,7 +21,8 @@ def kernels(file):
     return {re.search(r"(\w+_kernel)\s*\(", p).group(1): p for p in parts}
 
 
-@pytest.mark.parametrize("file,kernel", [("fp4_gemm.cu", "split_kernel"), ("skinny_gemm.cu", "skinny_gemm_kernel")])
+@pytest.mark.parametrize("file,kernel", [("fp4_gemm.cu", "split_kernel"), ("skinny_gemm.cu", "skinny_gemm_kernel"),
+                                         ("sparse_gemm.cu", "sparse_gemm_kernel")])
 def test_columns_are_freed_before_peers_are_waited_for(file, kernel):
     body = kernels(file)[kernel]
     held = body[body.index("tmem_alloc("):]
