@@ -127,6 +127,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         __syncwarp();
     } else if (warp == 1) {
         // all lanes; see fp4_mma.cuh
+        pdl_wait_prior();                                // waits are limited: they count from when the data can come
         const uint32_t leader = elect_one();
         const int slot_cols = TILES * 4 * (1 + p.b_tiles);
         const int shift = (n0 & 127) / 32;               // a tile that starts inside a 128-row scale tile
@@ -169,6 +170,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     float* stg = reinterpret_cast<float*>(smem);
     const int pitch = R + 4;
     const int quad = warp & 3;
+    pdl_wait_prior();                                        // D may belong to the preceding kernel; and the wait for `done` counts from here
     if (quad * 32 < rows) {
         bool ok = mbar_wait(done, 0);
         if (!ok) { *abort_flag = 1; report_timeout(p.status); }
@@ -201,7 +203,6 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         cluster_arrive_release();
         cluster_wait_acquire();                              // every rank's partial sums are in place
     }
-    pdl_wait_prior();                                        // D may belong to the preceding kernel
     const float alpha = alpha_s;
     if (!aborted) {
         // columns in granules of four; rank r sums and stores [G r / S, G (r + 1) / S)

@@ -190,6 +190,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         __syncwarp();
     } else if (warp == 1) {
         if (lane == 0) {
+            if (p.pdl) pdl_wait_prior();   // waits are limited: they count from when the activations can come
             // 64-row MMAs for batches of up to 16 rows: rows 0-15 of a 64-row accumulator lie in TMEM lanes 0-15, where
             // the epilogue reads them; half the padded tensor work of a 128-row MMA, hence less power
             const uint32_t idesc = idesc_e4m3_f32(MPAD == 16 ? p.mma_m : 128, R);
@@ -233,6 +234,7 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     // (fp32, row pitch R+4) that reuses the drained pipeline stages.
     float* stg = reinterpret_cast<float*>(smem);
     const int pitch = R + 4;
+    if (p.pdl) pdl_wait_prior();           // D and the scales may belong to the preceding kernel; the waits below count from here
     if ((warp & 3) == 0) {
         bool ok = mbar_wait(tmem_full, 0);
         if (!ok) { *abort_flag = 1; report_timeout(p.status); }
@@ -276,7 +278,6 @@ skinny_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
     __syncwarp();
     if (S > 1) cluster_wait_acquire();     // phase 1 complete: every peer's barriers and buffers are live
-    if (p.pdl) pdl_wait_prior();           // D and the scales may belong to the preceding kernel
     __syncthreads();
     const float sc = *sc_s;
 

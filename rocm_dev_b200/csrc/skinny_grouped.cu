@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) skinny_grouped_kernel(const __
     } else if (warp == 2) {
         // ---- MMA issuer: one accumulator per segment (the part of a tile's K range inside this CTA's range)
         if (lane == 0) {
+            if (p.pdl) pdl_wait_prior();       // waits are limited: they count from when the activations can come
             int pi = 0, seg = 0;
             bool first = true;
             for (int u = lo, i = 0; u < hi; u++, i++) {

@@ -231,10 +231,11 @@ sparse_gemm_kernel(const __grid_constant__ GParams g) {
         // k-block into an accumulator of their own; the epilogue adds the accumulators.
         if (lane == 0) {
             const int which = warp - 1;
+            if (p.pdl) pdl_wait_prior();                   // waits are limited: they count from when the data can come
             if (which == p.issuers - 1) {
                 // the two scales are fetched while the weights stream: their global-load latency (about a microsecond
-                // when they miss L2) would otherwise sit between the last MMA and the first store
-                if (p.pdl) pdl_wait_prior();               // the scales may be the preceding kernel's output
+                // when they miss L2) would otherwise sit between the last MMA and the first store; they may be the
+                // preceding kernel's output
                 *sc_slot = __ldg(p.scale_a) * __ldg(p.scale_b);
             }
             const uint32_t idesc = idesc_sparse(BM, NB);
@@ -267,6 +268,7 @@ sparse_gemm_kernel(const __grid_constant__ GParams g) {
     // that writes 128 contiguous output bytes reads 32 floats that all lie in one bank) and write whole 128-byte lines.
     float* stg = reinterpret_cast<float*>(smem);
     constexpr int pitch = BM + 4;
+    if (p.pdl) pdl_wait_prior();                       // D may still be read by the preceding kernel's successors; the waits below count from here
     if (warp >= 2) {
         bool ok = mbar_wait(tmem_full, 0);
         if (!ok) { *abort_flag = 1; report_timeout(p.status); }
@@ -305,7 +307,6 @@ sparse_gemm_kernel(const __grid_constant__ GParams g) {
     __syncwarp();
     if (S > 1) cluster_wait_acquire();
     __syncthreads();
-    if (p.pdl) pdl_wait_prior();                       // D may still be read by the preceding kernel's successors
     const float sc = *sc_slot;
 
     // one bf16x2 store per item (batch row m, pair of weight rows); consecutive threads take consecutive pairs

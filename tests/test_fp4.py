@@ -829,3 +829,47 @@ def test_quantized_buffers_at_any_16_bytes(cuda_device, form, shift):
         for b, n, used in zip(bufs, sizes, (1, 1, both, both)):
             assert (b[:16 + shift] == 0xAB).all() and (b[16 + shift + n:] == 0xAB).all()
             assert used or (b == 0xAB).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("follow", ["skinny", "skinny, overlapping", "dense", "fp8 skinny", "fp8 list", "sparse"])
+def test_the_kernel_before_may_run_longer_than_a_wait_may_last(cuda_device, follow):
+    """Launches start while the one before them runs; their waits for data are limited (to 1 ms here, the kernel before runs
+    about 15 ms on two SMs) and may begin only when that one has finished."""
+    import rocm_dev_b200 as R
+    from rocm_dev_b200 import quant
+    A, B = held(draw(8192, 8192, 1), "mxfp4", cuda_device), held(draw(8192, 8192, 2), "mxfp4", cuda_device)
+    D = torch.empty(8192, 8192, dtype=torch.bfloat16, device=cuda_device)
+    a, w = held(draw(16, 2048, 3), "nvfp4", cuda_device), held(draw(1024, 2048, 4), "nvfp4", cuda_device)
+    qa, qw, sa, sw = (t.to(cuda_device) for t in quant.synthetic_gemm_operands(16, 1024, 2048, seed=5))
+    vals, meta = (t.to(cuda_device) for t in R.pack_2of4(R.prune_2of4(qw.cpu())))
+    out = torch.empty(16, 1024, dtype=torch.bfloat16, device=cuda_device)
+
+    def call():
+        out.zero_()
+        if long:
+            R.dense_gemm_fp4(A, B, out=D, tiling=2, max_ctas=2)
+        if follow == "dense":
+            R.dense_gemm_fp4(a, w, out=out, tiling=1)
+        elif follow == "fp8 skinny":
+            assert R.skinny_gemm_fp8_tuned(qa, qw, sa, sw, out, flags=R.OVERLAP_PRIOR_KERNEL) == 0
+        elif follow == "fp8 list":
+            assert R.skinny_gemm_fp8_grouped([(qa, qw, sa, sw, out)], flags=R.OVERLAP_PRIOR_KERNEL) == 0
+        elif follow == "sparse":
+            R.sparse_gemm_fp8(qa, vals, meta, sa, sw, out=out, flags=R.OVERLAP_PRIOR_KERNEL)
+        else:
+            R.skinny_gemm_fp4(a, w, out=out, flags=R.OVERLAP_PRIOR_KERNEL if "overlapping" in follow else 0)
+        torch.cuda.synchronize()
+        return out.clone()
+
+    long = False
+    want = call()
+    assert R.lib().rdb_device_status() == 0
+    long = True
+    assert R.lib().rdb_set_wait_budget_ns(1_000_000) == 0
+    try:
+        got = call()
+        status = R.lib().rdb_device_status()
+    finally:
+        assert R.lib().rdb_set_wait_budget_ns(1_000_000_000) == 0
+    assert status == 0 and torch.equal(got, want)
