@@ -57,7 +57,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     __shared__ uint64_t bars[2 * MAX_STAGES + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_s;
-    __shared__ float alpha_s;
+    __shared__ Alpha alpha_s;
     volatile int* abort_flag = &abort_s;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -160,7 +160,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
     } else if (warp == 2) {
         if (lane == 0) {
             pdl_wait_prior();
-            alpha_s = p.ta ? __ldg(p.ta) * __ldg(p.tb) : 1.0f;
+            alpha_s = alpha_of(p.ta, p.tb);
         }
         __syncwarp();
     }
@@ -203,7 +203,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
         cluster_arrive_release();
         cluster_wait_acquire();                              // every rank's partial sums are in place
     }
-    const float alpha = alpha_s;
+    const Alpha alpha = alpha_s;
     if (!aborted) {
         // columns in granules of four; rank r sums and stores [G r / S, G (r + 1) / S)
         const int G = R / 4, g0 = G * rank / S, ng = G * (rank + 1) / S - g0;
@@ -230,8 +230,7 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                             for (int j = 0; j < 4; j++) v[j] += x[src][j];
                         }
                 }
-#pragma unroll
-                for (int j = 0; j < 4; j++) v[j] *= alpha;
+                times<4>(v, alpha);
                 store4(p.D, p.out_type, p.N, m0 + m, n0 + c, v, p.vec);
             }
         }
@@ -404,19 +403,20 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         __syncwarp();
     } else {
         const int quad = warp & 3;
-        const float alpha = p.ta ? __ldg(p.ta) * __ldg(p.tb) : 1.0f;
+        const Alpha alpha = alpha_of(p.ta, p.tb);
         const uint32_t free_even = mapa_smem(acc_free, 0);
         uint8_t* out = smem + STAGES * STAGE + quad * 2 * pairs::OUT_BYTES;
         int turn = 0;
         // 32 columns of this warp's 32 rows: into shared memory in the layout of the copy's swizzle (128 or 64 bytes a
         // row, no bank conflicts), then one copy out.  A thread holds a row: its own stores would touch 32 lines each.
-        auto put = [&](int m0, int n, const float* v) {
+        auto put = [&](int m0, int n, float* v) {
             if (m0 >= p.M || n >= p.N) return;
+            times<32>(v, alpha);
             if (!p.tma_out) {                            // rows of D off 16 bytes: neighbouring lanes store neighbouring columns
                 float* mine = reinterpret_cast<float*>(out) + lane * 33;
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; j++) mine[j] = v[j] * alpha;
+                for (int j = 0; j < 32; j++) mine[j] = v[j];
                 __syncwarp();
                 const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
                 if (n + lane < static_cast<int>(p.N)) {
@@ -432,13 +432,13 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                 for (int j = 0; j < 8; j++)
                     *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                        make_float4(v[4 * j] * alpha, v[4 * j + 1] * alpha, v[4 * j + 2] * alpha, v[4 * j + 3] * alpha);
+                        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = pack2(p.out_type, v[8 * j + 2 * i] * alpha, v[8 * j + 2 * i + 1] * alpha);
+                    for (int i = 0; i < 4; i++) w[i] = pack2(p.out_type, v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
                     *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }

@@ -87,6 +87,30 @@ __device__ __forceinline__ void bulk_load_scales(uint32_t dst_smem, const void* 
                  ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
 }
 
+// The product of two tensor scales, ready for an accumulator v: (v * pre) * mul = v * ta * tb, rounded once.  As one fp32
+// number ta * tb underflows below 2^-126 (operands around 1e-16 and smaller) or overflows where the result need not.  pre
+// is a power of two, 1 unless the product's exponent leaves [-100, 100].  v * pre is exact: the accumulator is a multiple
+// of 2^-20 (the smallest element times scale, squared) below 2^54 (the largest, squared, 2^31 times), so |exponent of pre|
+// <= 106 keeps it a normal number; what is cut off there leaves fp32's range anyway.
+struct Alpha { float pre, mul; };
+__device__ __forceinline__ Alpha alpha_of(const float* ta, const float* tb) {
+    if (!ta) return {1.0f, 1.0f};
+    int ea, eb;
+    const float m = frexpf(__ldg(ta), &ea) * frexpf(__ldg(tb), &eb);     // in [1/4, 1)
+    const int e = ea + eb, near = min(max(e, -100), 100), rest = min(max(e - near, -106), 106);
+    return {ldexpf(1.0f, rest), ldexpf(m, near)};
+}
+// N values times the scales.
+template <int N>
+__device__ __forceinline__ void times(float* v, const Alpha& a) {
+    if (a.pre != 1.0f) {
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] *= a.pre;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] *= a.mul;
+}
+
 __device__ __forceinline__ uint32_t pack2(int type, float x, float y) {
     if (type == RDB_TYPE_BF16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);

@@ -873,3 +873,30 @@ def test_the_kernel_before_may_run_longer_than_a_wait_may_last(cuda_device, foll
     finally:
         assert R.lib().rdb_set_wait_budget_ns(1_000_000_000) == 0
     assert status == 0 and torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,tiling", [(5, 130, 4096, 0), (100, 200, 520, 1), (300, 270, 1000, 2)])
+@pytest.mark.parametrize("a,b", [(1e-20, 1e-20), (1e-16, 1e-16), (1e-30, 1e-7), (1e-35, 1e35), (1e-3, 1e-33), (1e37, 1e-6), (1e16, 1e16)])
+def test_tensor_scales_whose_product_leaves_fp32(cuda_device, M, N, K, tiling, a, b):
+    """The result counts, not ta * tb: operands of 1e-20 have scales of 4e-24 and a product of 1e-37 at K = 4096."""
+    import rocm_dev_b200 as R
+    x, y = (torch.randn((r, K), generator=torch.Generator().manual_seed(r)).abs() * s for r, s in ((M, a), (N, b)))
+    x[1] = 0.0
+    A, B = held(x, "nvfp4", cuda_device), held(y, "nvfp4", cuda_device)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = _product(A, B, out_dtype=dtype, **({"tiling": tiling} if tiling else {}))
+        check_product(got, A, B)
+        assert not got[1].any() and got[0].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,tiling", [(5, 0), (300, 2)])
+def test_tensor_scales_whose_product_is_infinite(cuda_device, M, tiling):
+    """Zeros stay zeros where every other value is beyond fp32, or vanishes."""
+    x, y = (torch.randn((r, 256), generator=torch.Generator().manual_seed(r)).abs() for r in (M, 70))
+    x[1] = 0.0
+    for a, b, want in ((1e30, 1e30, float("inf")), (1e-35, 1e-35, 0.0)):
+        A, B = held(x * a, "nvfp4", cuda_device), held(y * b, "nvfp4", cuda_device)
+        got = _product(A, B, out_dtype=torch.float32, **({"tiling": tiling} if tiling else {}))
+        assert not got[1].any() and (got[0] == want).all()
