@@ -179,19 +179,27 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
 // tells.  With inv near 1 / d: q = a * inv, then the step q + inv * (a - q d).  It is NEGATIVE quotients that are
 // computed: with -q and -1 / d the step keeps the sign of a zero.
 // fp32 numerators: inv = RN(1 / d) and two steps - after the first, q is within a unit of the last place, and from such a q
-// the second gives the rounded quotient (Markstein).  16-bit numerators: the approximate reciprocal (one unit off) and one
-// step leave q within 2^-21 units of the quotient before its rounding; a quotient of a significand of 11 bits by one of 24
-// comes no nearer than 2^-19 units to the rounding borders next to a border of e2m1 or e4m3 (all of them were solved
-// for), so the code or scale byte that follows is the same.
+// the second gives the rounded quotient (Markstein).  16-bit numerators: one step, after which the code or scale byte is the
+// division's - all quotients of 11-bit significands next to a border of e2m1 or e4m3 were gone through, with exact
+// arithmetic.  With inv = RN(1 / d) that holds for every divisor; with an approximate reciprocal (one unit off) for all but
+// those whose 23 bits are all set: a power of two over 2 - 2^-23 lies 2^-25 units from where the rounded quotient leaves the
+// border.  No tensor scale computed from a 16-bit maximum makes such a divisor; for a given one (PATCH) its reciprocal, whose
+// bits are known, replaces the approximation.  (RN(1 / d) for every block costs more: 4096 x 14336 bf16 by rows 32.4 us
+// in place of 25.4.)
 struct Scale {
     float t, t6, n6;             // tensor scale; 6 t and -1 / (6 t), both for numerators that are multiplied by `move`
     float move;                  // 1, or a power of two for tensor scales so far from 1 that the steps would leave fp32
 };
-template <class T>
+template <class T, bool PATCH>
 __device__ __forceinline__ float neg_reciprocal(float d) {
     if constexpr (sizeof(T) == 4) return -__frcp_rn(d);
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    if constexpr (PATCH) {
+        // 1 / (2^k (2 - 2^-23)) rounds to 2^(-k - 1) (1 + 2^-23): exponent field 253 less d's, lowest bit set
+        const uint32_t bits = __float_as_uint(d);
+        if ((~bits & 0x7FFFFFu) == 0) r = __uint_as_float(0x7F000000u - bits);
+    }
     return -r;
 }
 template <class T>
@@ -236,7 +244,7 @@ __device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, const 
         const uint32_t byte = e;
         float d = __half2float(__ushort_as_half(static_cast<unsigned short>(h2))) * sc.t;
         if constexpr (CAREFUL) d *= sc.move;
-        const float ninv = neg_reciprocal<T>(d);
+        const float ninv = neg_reciprocal<T, CAREFUL>(d);
         const Pair d2 = pair(d, d), n2 = pair(ninv, ninv);
         const uint32_t keep = byte != 0 ? ~0u : 0u;                  // a scale of zero: zeros
 #pragma unroll
@@ -257,23 +265,21 @@ __device__ __forceinline__ uint32_t encode_block(float* v, uint32_t amax, const 
     }
 }
 
-template <class T>
 __device__ __forceinline__ Scale scale_of(float t) {
     Scale sc;
     sc.t = t;
     sc.move = t < 8.6736174e-19f ? 18446744073709551616.0f : t > 1.1529215e18f ? 5.4210109e-20f : 1.0f;   // 2^-60, 2^64; 2^60, 2^-64
     sc.t6 = t * 6.0f * sc.move;
-    sc.n6 = neg_reciprocal<T>(sc.t6);
+    sc.n6 = -__frcp_rn(sc.t6);
     return sc;
 }
-template <class T>
 __device__ __forceinline__ Scale scale_of_maximum(uint32_t m) {
     constexpr float inv = 1.0f / 2688.0f;                // rounded to fp32 before it multiplies: part of the definition
-    return scale_of<T>(m == 0 ? 1.0f : fmaxf(__fmul_rn(__uint_as_float(m), inv), 1.17549435e-38f));
+    return scale_of(m == 0 ? 1.0f : fmaxf(__fmul_rn(__uint_as_float(m), inv), 1.17549435e-38f));
 }
 
 // The tensor scale (NVFP4: given, or from the first pass's partial maxima), for the whole block: every thread takes part.
-template <class T, int FMT, int THREADS>
+template <int FMT, int THREADS>
 __device__ __forceinline__ Scale fetch_scale(float* tscale, const float* given, const uint32_t* partial, int partials) {
     Scale sc = {1.0f, 6.0f, 0.0f, 1.0f};
     if constexpr (FMT == RDB_FP4_NVFP4) {
@@ -286,9 +292,9 @@ __device__ __forceinline__ Scale fetch_scale(float* tscale, const float* given, 
             __syncthreads();
 #pragma unroll
             for (int w = 0; w < THREADS / 32; w++) m = max(m, warp_max[w]);
-            sc = scale_of_maximum<T>(m);
+            sc = scale_of_maximum(m);
         } else {
-            sc = scale_of<T>(*given);
+            sc = scale_of(*given);
         }
         if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *tscale = sc.t;
     }
@@ -364,7 +370,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const T* __rest
                                                                  uint8_t* __restrict__ scales) {
     constexpr int B = Format<FMT>::BLOCK, WORDS = B * sizeof(T) / 4, HELD = WORDS > 16 ? 2 : 4;
     start_after_prior();
-    const Scale scale = fetch_scale<T, FMT, kThreads>(tscale, given, partial, partials);
+    const Scale scale = fetch_scale<FMT, kThreads>(tscale, given, partial, partials);
     const size_t pitch = row_bytes(K);
     const int tiles = scale_tiles_per_row(FMT, K);
     const int lane = threadIdx.x & 31, b = blockIdx.x * 32 + lane, blocks = K / B;
@@ -470,7 +476,7 @@ __global__ void __launch_bounds__(kSmallThreads) quantize_small_kernel(const T* 
         }
         cluster_arrive_release();                        // (waited for at the end: nobody leaves before all have read)
     }
-    const Scale scale = scale_of_maximum<T>(m);
+    const Scale scale = scale_of_maximum(m);
     if (first == 0) *tscale = scale.t;
     auto body = [&](auto careful) {
 #pragma unroll
@@ -601,7 +607,7 @@ quantize_tile_kernel(const T* __restrict__ x, long long ldx, int rows, int K, in
     int tr = static_cast<int>(tiles_y - 1 - blockIdx.x / tiles_x), tc = static_cast<int>(tiles_x - 1 - blockIdx.x % tiles_x);
     int ntr = tr, ntc = tc, turn = 0;
     fetch(tr, tc, buffers);
-    const Scale scale = fetch_scale<T, FMT, kTileThreads>(tscale, given, partial, partials);
+    const Scale scale = fetch_scale<FMT, kTileThreads>(tscale, given, partial, partials);
     auto body = [&](auto careful) {
     for (unsigned n = blockIdx.x; n < tiles_all; n += gridDim.x, turn ^= 1, tr = ntr, tc = ntc) {
         if (n + gridDim.x < tiles_all) {
@@ -756,7 +762,7 @@ quantize_both_kernel(const __grid_constant__ CUtensorMap tm, int rows, int K, un
     }
     __syncthreads();
     start_after_prior();
-    const Scale scale = fetch_scale<T, FMT, kBothThreads>(tscale, given, partial, partials);
+    const Scale scale = fetch_scale<FMT, kBothThreads>(tscale, given, partial, partials);
 
     const size_t pitch = row_bytes(K), pitch_t = row_bytes(rows);
     const bool wide = ((reinterpret_cast<uintptr_t>(codes) | pitch) & 31) == 0, wide_t = ((reinterpret_cast<uintptr_t>(codes_t) | pitch_t) & 31) == 0;

@@ -900,3 +900,83 @@ def test_tensor_scales_whose_product_is_infinite(cuda_device, M, tiling):
         A, B = held(x * a, "nvfp4", cuda_device), held(y * b, "nvfp4", cuda_device)
         got = _product(A, B, out_dtype=torch.float32, **({"tiling": tiling} if tiling else {}))
         assert not got[1].any() and (got[0] == want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("six", [False, True])
+def test_divisors_with_every_bit_set(cuda_device, dtype, six):
+    """Powers of two over a divisor 2^k (2 - 2^-23): the quotient rounds to just above a power of two, which is a border
+    between two codes (0.25) and between two scales (2^-10), and one unit in the divisor's reciprocal decides.  six: 6 t is
+    that divisor, not t."""
+    import rocm_dev_b200 as R
+    t = np.float32(1) - np.float32(2.0 ** -24)
+    if six:
+        near = np.float32(4 / 3) + np.arange(-64, 64, dtype=np.float32) * np.float32(2.0 ** -23)
+        t = near[((near * np.float32(6)).view(np.uint32) & 0x7FFFFF) == 0x7FFFFF][0]
+    x = torch.zeros(64, 160)
+    for i in range(14):                                              # block scales 2^-6 .. 2^7 where t is the divisor
+        x[i, ::16], x[i, 1::4], x[i, 2::4] = 6.0 * 2.0 ** (i - 6), 0.25 * 2.0 ** (i - 6), -0.25 * 2.0 ** (i - 6)
+    for i in range(14, 40):                                          # largest magnitudes 2^-16 .. 2^9
+        x[i, ::16], x[i, 3::16] = 2.0 ** (i - 30), 2.0 ** (i - 32)
+    x = x.to(dtype)
+    ts = torch.from_numpy(np.array([t])).to(cuda_device)
+    for v in (x, x.t().contiguous()):
+        for aligned in (True, False):
+            wide = torch.zeros(v.shape[0], v.shape[1] + 3, dtype=dtype)
+            wide[:, 1:-2] = v
+            y = v.to(cuda_device) if aligned else wide.to(cuda_device)[:, 1:-2]
+            r, c = R.quantize_fp4_both(y, "nvfp4", ts)
+            for got, want in ((r, v), (R.quantize_fp4(y, "nvfp4", ts), v), (c, v.t())):
+                check_quantized(got, np.ascontiguousarray(want.float().numpy()), "nvfp4", t)
+
+
+def test_16_bit_maxima_make_no_divisor_with_every_bit_set():
+    """Tensor scales computed from 16-bit maxima keep the quantiser's short quotient: none of their products with a block
+    scale's significand (1 to 15/8; 12/8 stands for 6 t too) has all 23 bits set, whatever the exponents."""
+    top = np.arange(1024, 2048, dtype=np.float32)                    # significands of fp16, those of bf16 among them
+    t = top * np.float32(1 / 2688)
+    for k in range(8, 16):
+        assert not ((t * np.float32(k)).view(np.uint32) & 0x7FFFFF == 0x7FFFFF).any()
+
+
+def _rounded(v):
+    """A Fraction to fp32 (no range limits), ties to even."""
+    from fractions import Fraction as F
+    if v == 0:
+        return v
+    a = abs(v)
+    e = a.numerator.bit_length() - a.denominator.bit_length()
+    step = F(2) ** (e - (F(2) ** e > a) - 23)
+    n, rest = divmod(a, step)
+    n += rest * 2 > step or rest * 2 == step and n % 2
+    return n * step * (1 if v > 0 else -1)
+
+
+def test_the_short_quotient_decides_as_the_division_does():
+    """Quotients of 11-bit significands next to every border of e2m1, and of e4m3's three lowest binades: q = RN(a inv), then
+    RN(q + inv RN(a - q d)).  With the rounded reciprocal the side of the border is the division's, always; with one a unit
+    off as well, but for divisors whose 23 bits are all set."""
+    from fractions import Fraction as F
+    tie = {F(1, 4): -1, F(3, 4): 1, F(5, 4): -1, F(7, 4): 1, F(5, 2): -1, F(7, 2): 1, F(5): -1}       # the even code's side
+    tie |= {F(2 * i + 1, 1024): 1 if i % 2 else -1 for i in range(16)}
+    side = lambda v, b: (v > b) - (v < b) or tie[b]  # noqa: E731
+    exceptions = set()
+    for b in tie:
+        for X in range(1024, 2048):
+            d0 = X / b                                               # brought into [1, 2): divisors next to X / border
+            k = d0.numerator.bit_length() - d0.denominator.bit_length()
+            k -= F(2) ** k > d0
+            a = F(X) / F(2) ** k
+            n0 = int(a / b * 2 ** 23)
+            for n in (n0 - 1, n0, n0 + 1):
+                d = F(n, 2 ** 23) if n >= 2 ** 23 else F(2 * n + 1, 2 ** 24)      # below 1: steps half as wide
+                want = side(_rounded(a / d), b)
+                inv = np.float32(float(_rounded(1 / d)))
+                for off in (inv, np.nextafter(inv, np.float32(0)), np.nextafter(inv, np.float32(9))):
+                    r = F(float(off))
+                    q = _rounded(a * r)
+                    if side(_rounded(q + r * _rounded(a - q * d)), b) != want:
+                        assert off != inv
+                        exceptions.add(d)
+    assert exceptions and all(d.numerator == 2 ** 24 - 1 for d in exceptions)
