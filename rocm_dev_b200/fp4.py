@@ -90,13 +90,16 @@ class Fp4Tensor:
         return (codes.data_ptr(), scales.data_ptr(), None if ts is None else ts.data_ptr()), dev
 
     def _views(self):
-        # a quantiser's result is one allocation, with the addresses in _held; its tensors are made when they are asked for
-        if self._parts is None:
-            buf, base = self._buffer, self._buffer.data_ptr()
-            codes, scales, ts = (a if a is None else a - base for a in self._held[0])
+        # a quantiser's result is one allocation, with the addresses in _held; its tensors are made when they are asked for,
+        # and from then on they say where the data lies
+        buf, held = self._buffer, self._held
+        if buf is not None and held is not None:             # (another thread may be here too: _parts is there before these go)
+            base = buf.data_ptr()
+            codes, scales, ts = (a if a is None else a - base for a in held[0])
             rb, sb = row_bytes(self.K), scale_bytes(self.format, self.rows, self.K)
             self._parts = (buf[codes:codes + self.rows * rb].view(self.rows, rb), buf[scales:scales + sb],
                            None if ts is None else buf[ts:ts + 4].view(torch.float32))
+            self._buffer = self._held = None
         return self._parts
 
     @property

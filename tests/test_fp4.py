@@ -980,3 +980,16 @@ def test_the_short_quotient_decides_as_the_division_does():
                         assert off != inv
                         exceptions.add(d)
     assert exceptions and all(d.numerator == 2 ** 24 - 1 for d in exceptions)
+
+
+@pytest.mark.gpu
+def test_parts_that_got_other_memory_are_read_where_they_lie(cuda_device):
+    """Of a quantiser's own result too, once its tensors have been asked for."""
+    import rocm_dev_b200 as R
+    x = draw(33, 300, 1).to(cuda_device)
+    t, other = R.quantize_fp4(x), R.quantize_fp4(draw(33, 300, 2).to(cuda_device))
+    shallow = copy.copy(t)
+    assert torch.equal(R.dequantize_fp4(shallow), R.dequantize_fp4(t)) and shallow.codes.data_ptr() == t.codes.data_ptr()
+    t.codes.data, t.scales.data, t.tensor_scale.data = other.codes.clone(), other.scales.clone(), other.tensor_scale.clone()
+    for q in (t, copy.deepcopy(t), pickle.loads(pickle.dumps(t))):
+        assert torch.equal(R.dequantize_fp4(q), R.dequantize_fp4(other))
