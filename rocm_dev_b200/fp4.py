@@ -23,7 +23,7 @@ BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 WORKSPACE_FLOATS = 1024
 MAX_EXTENT = 2 ** 31 - 1025                   # rows and columns of a tensor
-_BYTE = torch.uint8
+_BYTE, _FLOAT = torch.uint8, torch.float32
 
 # A step's calls are short: what a call costs on the host shows.  These two are the cheap forms of
 # torch.cuda.current_device() and torch.cuda.current_stream(dev).cuda_stream (0.1 us each instead of 0.2 and 2.2).
@@ -90,15 +90,19 @@ class Fp4Tensor:
         return (codes.data_ptr(), scales.data_ptr(), None if ts is None else ts.data_ptr()), dev
 
     def _views(self):
-        # a quantiser's result is one allocation, with the addresses in _held; its tensors are made when they are asked for,
-        # and from then on they say where the data lies
-        buf, held = self._buffer, self._held
-        if buf is not None and held is not None:             # (another thread may be here too: _parts is there before these go)
-            base = buf.data_ptr()
-            codes, scales, ts = (a if a is None else a - base for a in held[0])
+        # a quantiser's result is memory with the addresses in _held; its tensors are made when they are asked for, and from
+        # then on they say where the data lies
+        buffer, held = self._buffer, self._held
+        if buffer is not None and held is not None:          # (another thread may be here too: _parts is there before these go)
+            (at_codes, at_scales, at_ts), base = held[0], buffer.data_ptr()
             rb, sb = row_bytes(self.K), scale_bytes(self.format, self.rows, self.K)
-            self._parts = (buf[codes:codes + self.rows * rb].view(self.rows, rb), buf[scales:scales + sb],
-                           None if ts is None else buf[ts:ts + 4].view(torch.float32))
+            codes, scales = at_codes - base, at_scales - base
+            ts = None
+            if at_ts is not None:
+                # fp32 in the allocation of the bytes: a storage of its own over the same memory, since torch.save refuses
+                # tensors of two types in one
+                ts = torch.from_dlpack(torch.utils.dlpack.to_dlpack(buffer[at_ts - base:at_ts - base + 4].view(_FLOAT)))
+            self._parts = (buffer[codes:codes + self.rows * rb].view(self.rows, rb), buffer[scales:scales + sb], ts)
             self._buffer = self._held = None
         return self._parts
 
@@ -120,14 +124,44 @@ class Fp4Tensor:
 
     def to(self, device) -> "Fp4Tensor":
         """The same tensor on another device (or on the host, to be stored)."""
+        if torch.device(device) == self.device:
+            return self
         move = lambda t: None if t is None else t.to(device)  # noqa: E731
         return Fp4Tensor(*map(move, self._views()), self.format, self.rows, self.K)
 
-    def __reduce__(self):                        # copies and files hold the tensors, never an address
-        return Fp4Tensor, (*self._views(), self.format, self.rows, self.K)
+    def record_stream(self, stream) -> None:
+        """``torch.Tensor.record_stream`` for every part: for a tensor made on another stream than the one it is used on."""
+        buffer = self._buffer
+        for t in self._parts if buffer is None else (buffer,):
+            if t is not None:
+                t.record_stream(stream)
+
+    def __copy__(self) -> "Fp4Tensor":
+        return Fp4Tensor(*self._views(), self.format, self.rows, self.K)
+
+    def __reduce__(self):
+        # deep copies and files hold tensors, never an address: codes and scales once, and nothing else of their allocation
+        codes, scales, ts = self._views()
+        own = lambda t: t if t.untyped_storage().nbytes() == t.nbytes else t.clone()  # noqa: E731
+        ts, n = ts if ts is None else own(ts), codes.numel()
+        if codes.untyped_storage().data_ptr() == scales.untyped_storage().data_ptr() and scales.data_ptr() == codes.data_ptr() + n:
+            return _whole, (own(codes.as_strided((n + scales.numel(),), (1,))), ts, self.format, self.rows, self.K)
+        return Fp4Tensor, (codes, scales, ts, self.format, self.rows, self.K)
 
     def __repr__(self) -> str:
         return f"Fp4Tensor({self.format}, [{self.rows}, {self.K}], {self.device})"
+
+
+def _whole(buf: torch.Tensor, tensor_scale, format: str, rows: int, K: int) -> Fp4Tensor:
+    """What ``__reduce__`` took apart."""
+    _format(format)
+    if rows < 1 or K < 1 or buf.shape != (rows * row_bytes(K) + scale_bytes(format, rows, K),):
+        raise ValueError(f"codes and scales of {format} [{rows}, {K}] in one flat tensor expected, got {tuple(buf.shape)}")
+    n = rows * row_bytes(K)
+    return Fp4Tensor(buf[:n].view(rows, -1), buf[n:], tensor_scale, format, rows, K)
+
+
+torch.serialization.add_safe_globals([Fp4Tensor, _whole])        # torch.load reads them without weights_only=False
 
 
 def _index(dev: torch.device) -> int:
@@ -190,38 +224,38 @@ def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
         ldx = K
     elif rows == 1:
         ldx = K
-    # one allocation (every part a multiple of 16 bytes): codes and scales of either direction, then the tensor scale and
-    # the scratch that the call alone uses
     per_word = 2048 if fmt else 1024              # scale bytes of 128 rows x 256 elements
-    at_s = rows * ((K + 31) // 32 * 16)
-    size = at_ct = at_s + (rows + 127) // 128 * ((K + 255) // 256) * per_word
+    n = rows * ((K + 31) // 32 * 16)
+    size = n + (rows + 127) // 128 * ((K + 255) // 256) * per_word
+    m = size_t = 0
     if both:
-        at_st = at_ct + K * ((rows + 31) // 32 * 16)
-        size = at_st + (K + 127) // 128 * ((rows + 255) // 256) * per_word
-    given = scale = work = None
+        m = K * ((rows + 31) // 32 * 16)
+        size_t = m + (K + 127) // 128 * ((rows + 255) // 256) * per_word
+    given = at_ts = work = None
+    extra = 0                                     # the tensor scale and the scratch that the call alone uses
     if fmt == 0:
         if tensor_scale is not None:
             raise ValueError("mxfp4 has no tensor scale")
-        buffer = torch.empty(size, dtype=_BYTE, device=dev)
-        at = buffer.data_ptr()
+    elif tensor_scale is None:
+        extra = 16 + 4 * WORKSPACE_FLOATS
     else:
-        if tensor_scale is None:
-            buffer = torch.empty(size + 16 + 4 * WORKSPACE_FLOATS, dtype=_BYTE, device=dev)
-            at = buffer.data_ptr()
-            work = at + size + 16
-        else:
-            if not (tensor_scale.dtype is torch.float32 and tensor_scale.numel() == 1 and tensor_scale.device == dev):
-                raise ValueError(f"the tensor scale must be one fp32 on {dev}")
-            given = tensor_scale.data_ptr()
-            buffer = torch.empty(size + 16, dtype=_BYTE, device=dev)
-            at = buffer.data_ptr()
-        scale = at + size
+        if not (tensor_scale.dtype is _FLOAT and tensor_scale.numel() == 1 and tensor_scale.device == dev):
+            raise ValueError(f"the tensor scale must be one fp32 on {dev}")
+        given = tensor_scale.data_ptr()
+        extra = 16
+    buffer = torch.empty(size + size_t + extra, dtype=_BYTE, device=dev)      # every part a multiple of 16 bytes
+    at = buffer.data_ptr()
+    at_t = at + size
+    if extra:
+        at_ts = at_t + size_t
+    if extra > 16:
+        work = at_ts + 16
     if both:
-        _call(_QUANTIZE, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, scale, given, at, at + at_s, at + at_ct, at + at_st, work)
-        return (_result(format, fmt, rows, K, dev, buffer, (at, at + at_s, scale)),
-                _result(format, fmt, K, rows, dev, buffer, (at + at_ct, at + at_st, scale)))
-    _call(_QUANTIZE, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, scale, given, at, at + at_s, None, None, work)
-    return _result(format, fmt, rows, K, dev, buffer, (at, at + at_s, scale))
+        _call(_QUANTIZE, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, at_ts, given, at, at + n, at_t, at_t + m, work)
+        return (_result(format, fmt, rows, K, dev, buffer, (at, at + n, at_ts)),
+                _result(format, fmt, K, rows, dev, buffer, (at_t, at_t + m, at_ts)))
+    _call(_QUANTIZE, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, at_ts, given, at, at + n, None, None, work)
+    return _result(format, fmt, rows, K, dev, buffer, (at, at + n, at_ts))
 
 
 def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None) -> Fp4Tensor:

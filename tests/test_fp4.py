@@ -993,3 +993,53 @@ def test_parts_that_got_other_memory_are_read_where_they_lie(cuda_device):
     t.codes.data, t.scales.data, t.tensor_scale.data = other.codes.clone(), other.scales.clone(), other.tensor_scale.clone()
     for q in (t, copy.deepcopy(t), pickle.loads(pickle.dumps(t))):
         assert torch.equal(R.dequantize_fp4(q), R.dequantize_fp4(other))
+    s = torch.cuda.Stream(cuda_device)
+    with torch.cuda.stream(s):
+        q = R.quantize_fp4(x)
+    q.record_stream(torch.cuda.current_stream())
+    t.record_stream(s)
+
+
+def _stored(x):
+    import io
+    f = io.BytesIO()
+    torch.save(x, f)
+    return f.getvalue()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("asked", [False, True])
+@pytest.mark.parametrize("rows,K", [(256, 512), (2048, 4096)])
+def test_files_hold_a_quantised_tensor_and_nothing_else(cuda_device, form, asked, rows, K):
+    """torch.save, pickle and a state dict of the parts, for results of either quantiser, whether or not their tensors have
+    been asked for: no more bytes than codes, scales and tensor scale (and a kilobyte or so of names)."""
+    import io
+
+    import rocm_dev_b200 as R
+    x = draw(rows, K, 1).to(cuda_device)
+    for t in (R.quantize_fp4(x, form), *R.quantize_fp4_both(x, form), R.quantize_fp4(x, form, None if form == "mxfp4" else torch.ones(1, device=cuda_device))):
+        want = R.dequantize_fp4(t)
+        if asked:
+            t.codes, t.scales, t.tensor_scale
+        most = t.rows * R.fp4.row_bytes(t.K) + R.fp4.scale_bytes(form, t.rows, t.K) + 4096
+        data = _stored(t)
+        assert len(data) < most and len(pickle.dumps(t)) < most
+        for again in (torch.load(io.BytesIO(data)), torch.load(io.BytesIO(data), map_location="cpu").to(cuda_device), pickle.loads(pickle.dumps(t))):
+            assert repr(again) == repr(t) and torch.equal(R.dequantize_fp4(again), want)
+            assert len(_stored(again)) < most
+        parts = {k: v for k, v in (("codes", t.codes), ("scales", t.scales), ("tensor_scale", t.tensor_scale)) if v is not None}
+        back = torch.load(io.BytesIO(_stored(parts)))
+        own = R.Fp4Tensor(back["codes"], back["scales"], back.get("tensor_scale"), form, t.rows, t.K)
+        assert torch.equal(R.dequantize_fp4(own), want)
+
+
+def test_a_stored_tensor_of_the_wrong_size_is_refused():
+    from rocm_dev_b200 import fp4
+    n = 4 * fp4.row_bytes(64) + fp4.scale_bytes("nvfp4", 4, 64)
+    assert fp4._whole(torch.zeros(n, dtype=torch.uint8), torch.ones(1), "nvfp4", 4, 64).rows == 4
+    for bad in ((torch.zeros(n - 1, dtype=torch.uint8), torch.ones(1), "nvfp4", 4, 64), (torch.zeros(n), torch.ones(1), "nvfp4", 4, 64),
+                (torch.zeros((1, n), dtype=torch.uint8), torch.ones(1), "nvfp4", 4, 64), (torch.zeros(8, dtype=torch.uint8), torch.ones(1), "nvfp4", 4, 64),
+                (torch.zeros(n, dtype=torch.uint8), None, "nvfp4", 4, 64)):
+        with pytest.raises(ValueError):
+            fp4._whole(*bad)
