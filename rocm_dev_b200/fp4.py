@@ -24,6 +24,11 @@ _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 WORKSPACE_FLOATS = 1024
 MAX_EXTENT = 2 ** 31 - 1025                   # rows and columns of a tensor
 _BYTE, _FLOAT = torch.uint8, torch.float32
+# A quantiser's results of up to this many bytes are one allocation; larger ones have one for either direction, so that one
+# can be dropped without the other, and one for the tensor scale.  An allocation costs 1.6 us of host time (8 x 4096 NVFP4
+# 6.7 us a call in one, 8.4 in two; both directions 8.7 and 12.1), which shows until the device takes longer than the host:
+# at this size 12 us for one direction, 15 for both.
+ONE_ALLOCATION = 4 << 20
 
 # A step's calls are short: what a call costs on the host shows.  These two are the cheap forms of
 # torch.cuda.current_device() and torch.cuda.current_stream(dev).cuda_stream (0.1 us each instead of 0.2 and 2.2).
@@ -94,15 +99,15 @@ class Fp4Tensor:
         # then on they say where the data lies
         buffer, held = self._buffer, self._held
         if buffer is not None and held is not None:          # (another thread may be here too: _parts is there before these go)
-            (at_codes, at_scales, at_ts), base = held[0], buffer.data_ptr()
+            buf, ts = buffer
+            (at_codes, at_scales, at_ts), base = held[0], buf.data_ptr()
             rb, sb = row_bytes(self.K), scale_bytes(self.format, self.rows, self.K)
             codes, scales = at_codes - base, at_scales - base
-            ts = None
-            if at_ts is not None:
+            if ts is None and at_ts is not None:
                 # fp32 in the allocation of the bytes: a storage of its own over the same memory, since torch.save refuses
                 # tensors of two types in one
-                ts = torch.from_dlpack(torch.utils.dlpack.to_dlpack(buffer[at_ts - base:at_ts - base + 4].view(_FLOAT)))
-            self._parts = (buffer[codes:codes + self.rows * rb].view(self.rows, rb), buffer[scales:scales + sb], ts)
+                ts = torch.from_dlpack(torch.utils.dlpack.to_dlpack(buf[at_ts - base:at_ts - base + 4].view(_FLOAT)))
+            self._parts = (buf[codes:codes + self.rows * rb].view(self.rows, rb), buf[scales:scales + sb], ts if ts is None else ts[:1])
             self._buffer = self._held = None
         return self._parts
 
@@ -131,8 +136,7 @@ class Fp4Tensor:
 
     def record_stream(self, stream) -> None:
         """``torch.Tensor.record_stream`` for every part: for a tensor made on another stream than the one it is used on."""
-        buffer = self._buffer
-        for t in self._parts if buffer is None else (buffer,):
+        for t in self._buffer or self._parts:
             if t is not None:
                 t.record_stream(stream)
 
@@ -200,10 +204,10 @@ def _call(which: int, where: str, dev: int, *args) -> None:
         check(code, where)
 
 
-def _result(form: str, fmt: int, rows: int, K: int, dev, buffer, addresses) -> Fp4Tensor:
+def _result(form: str, fmt: int, rows: int, K: int, dev, buffer, scale, addresses) -> Fp4Tensor:
     t = Fp4Tensor.__new__(Fp4Tensor)
     t.format, t.rows, t.K, t._fmt = form, rows, K, fmt
-    t._parts, t._buffer, t._held = None, buffer, (addresses, dev)
+    t._parts, t._buffer, t._held = None, (buffer, scale), (addresses, dev)
     return t
 
 
@@ -231,7 +235,7 @@ def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
     if both:
         m = K * ((rows + 31) // 32 * 16)
         size_t = m + (K + 127) // 128 * ((rows + 255) // 256) * per_word
-    given = at_ts = work = None
+    given = at_ts = work = ts = None
     extra = 0                                     # the tensor scale and the scratch that the call alone uses
     if fmt == 0:
         if tensor_scale is not None:
@@ -243,19 +247,29 @@ def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
             raise ValueError(f"the tensor scale must be one fp32 on {dev}")
         given = tensor_scale.data_ptr()
         extra = 16
-    buffer = torch.empty(size + size_t + extra, dtype=_BYTE, device=dev)      # every part a multiple of 16 bytes
-    at = buffer.data_ptr()
-    at_t = at + size
-    if extra:
-        at_ts = at_t + size_t
+    if size + size_t <= ONE_ALLOCATION:           # every part a multiple of 16 bytes
+        buffer = buffer_t = torch.empty(size + size_t + extra, dtype=_BYTE, device=dev)
+        at = buffer.data_ptr()
+        at_t = at + size
+        if extra:
+            at_ts = at_t + size_t
+    else:
+        buffer = torch.empty(size, dtype=_BYTE, device=dev)
+        at, at_t, buffer_t = buffer.data_ptr(), 0, None
+        if both:
+            buffer_t = torch.empty(size_t, dtype=_BYTE, device=dev)
+            at_t = buffer_t.data_ptr()
+        if extra:
+            ts = torch.empty(extra // 4, dtype=_FLOAT, device=dev)
+            at_ts = ts.data_ptr()
     if extra > 16:
         work = at_ts + 16
     if both:
         _call(_QUANTIZE, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, at_ts, given, at, at + n, at_t, at_t + m, work)
-        return (_result(format, fmt, rows, K, dev, buffer, (at, at + n, at_ts)),
-                _result(format, fmt, K, rows, dev, buffer, (at_t, at_t + m, at_ts)))
+        return (_result(format, fmt, rows, K, dev, buffer, ts, (at, at + n, at_ts)),
+                _result(format, fmt, K, rows, dev, buffer_t, ts, (at_t, at_t + m, at_ts)))
     _call(_QUANTIZE, "rdb_quantize_fp4", index, x.data_ptr(), typ, ldx, rows, K, fmt, at_ts, given, at, at + n, None, None, work)
-    return _result(format, fmt, rows, K, dev, buffer, (at, at + n, at_ts))
+    return _result(format, fmt, rows, K, dev, buffer, ts, (at, at + n, at_ts))
 
 
 def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None) -> Fp4Tensor:
@@ -266,7 +280,9 @@ def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Ten
 
 
 def quantize_fp4_both(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None):
-    """(held form of x, held form of its transpose [K, rows] with blocks along x's columns), one tensor scale for both."""
+    """(held form of x, held form of its transpose [K, rows] with blocks along x's columns), one tensor scale for both.
+    Either frees its memory when it is dropped (a training step needs the first for the forward product alone), but where
+    both together have no more than 4 MB, which are then kept by either."""
     return _quantize(x, format, tensor_scale, True)
 
 

@@ -1043,3 +1043,20 @@ def test_a_stored_tensor_of_the_wrong_size_is_refused():
                 (torch.zeros(n, dtype=torch.uint8), None, "nvfp4", 4, 64)):
         with pytest.raises(ValueError):
             fp4._whole(*bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_either_direction_can_be_dropped(cuda_device, form):
+    import rocm_dev_b200 as R
+    x = draw(1024, 4096, 1).to(cuda_device)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated(cuda_device)
+    r, c = R.quantize_fp4_both(x, form)
+    both = torch.cuda.memory_allocated(cuda_device) - before
+    size = r.codes.numel() + r.scales.numel()
+    want = R.dequantize_fp4(c).clone()
+    del r
+    left = torch.cuda.memory_allocated(cuda_device) - before - want.numel() * 2
+    assert both - left >= size and left <= size + 16384
+    assert torch.equal(R.dequantize_fp4(c), want)
