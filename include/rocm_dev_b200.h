@@ -278,7 +278,8 @@ int rdb_skinny_gemm_fp4(const uint8_t *A, const uint8_t *scales_a, const float *
                         int format, unsigned flags, void *stream);
 
 /* rdb_dense_gemm_fp4 with the tiling chosen by the caller: 1 = 128-row tiles, K split over a cluster; 2 = 256 x 256 tiles
- * by pairs of CTAs, whose persistent grid max_ctas caps; 0 = automatic. */
+ * by pairs of CTAs, whose persistent grid max_ctas caps; 0 = automatic.  1 refuses N whose tiles (of 128 columns, or 256
+ * where there are more of those than SMs) number above 65535, and so do the knobs of rdb_skinny_gemm_fp4_tuned. */
 int rdb_dense_gemm_fp4_tuned(const uint8_t *A, const uint8_t *scales_a, const float *tensor_scale_a, const uint8_t *B,
                              const uint8_t *scales_b, const float *tensor_scale_b, void *D, int out_type, int M, int N,
                              int K, int format, int tiling, int max_ctas, void *stream);

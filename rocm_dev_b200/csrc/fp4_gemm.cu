@@ -677,10 +677,19 @@ static int check(const Product& q, int format) {
     return RDB_SUCCESS;
 }
 
+static bool split_fits(const SplitPlan& pl, const Product& q) {       // the grid's limits: 65535 tiles in y and z
+    return (q.N + pl.R - 1) / pl.R <= 65535 && (q.M + 127) / 128 <= 65535;
+}
+
+static int run_pairs(const Product& q, int format, int max_ctas, DeviceInfo* info, cudaStream_t stream) {
+    const long long tiles = static_cast<long long>((q.M + 255ll) / 256) * ((q.N + 255ll) / 256);
+    if (tiles > (1ll << 30)) return RDB_SIZE_ABOVE_LIMIT;
+    return format == RDB_FP4_NVFP4 ? launch_pair<RDB_FP4_NVFP4>(q, max_ctas, info, stream) : launch_pair<RDB_FP4_MXFP4>(q, max_ctas, info, stream);
+}
+
 static int run_split(const Product& q, int format, int r_hint, int s_hint, int stages_hint, unsigned flags, DeviceInfo* info, cudaStream_t stream) {
     const SplitPlan pl = split_plan(format, q.M, q.N, q.K, info->sm_count, r_hint, s_hint, stages_hint);
-    // grid limits: 65535 tiles in y and z
-    if ((q.N + pl.R - 1) / pl.R > 65535 || (q.M + 127) / 128 > 65535) return RDB_SIZE_ABOVE_LIMIT;
+    if (!split_fits(pl, q)) return RDB_SIZE_ABOVE_LIMIT;
     return format == RDB_FP4_NVFP4 ? launch_split<RDB_FP4_NVFP4>(q, pl, flags, info, stream) : launch_split<RDB_FP4_MXFP4>(q, pl, flags, info, stream);
 }
 
@@ -701,7 +710,11 @@ int rdb_skinny_gemm_fp4_tuned(const uint8_t* A, const uint8_t* scales_a, const f
     int err = 0;
     rdb::DeviceInfo* info = rdb::device_info(&err);
     if (!info) return err;
-    return rdb::fp4::run_split(q, format, columns_per_tile, split_k, stages, flags, info, static_cast<cudaStream_t>(stream));
+    auto st = static_cast<cudaStream_t>(stream);
+    // more columns than the split kernel's grid can have tiles (8.4 million): pairs, whose tiles are walked
+    if (columns_per_tile == 0 && split_k == 0 && stages == 0 && !rdb::fp4::split_fits(rdb::fp4::split_plan(format, M, N, K, info->sm_count, 0, 0, 0), q))
+        return rdb::fp4::run_pairs(q, format, 0, info, st);
+    return rdb::fp4::run_split(q, format, columns_per_tile, split_k, stages, flags, info, st);
 }
 
 int rdb_skinny_gemm_fp4(const uint8_t* A, const uint8_t* scales_a, const float* tensor_scale_a, const uint8_t* B,
@@ -721,19 +734,16 @@ int rdb_dense_gemm_fp4_tuned(const uint8_t* A, const uint8_t* scales_a, const fl
     rdb::DeviceInfo* info = rdb::device_info(&err);
     if (!info) return err;
     auto st = static_cast<cudaStream_t>(stream);
-    const long long tiles = static_cast<long long>((M + 255ll) / 256) * ((N + 255ll) / 256);
-    if (tiles > (1ll << 30)) return RDB_SIZE_ABOVE_LIMIT;
     if (tiling == 0) {
         // Pairs where their 256 x 256 tiles are enough for half of the machine and K is long, or there are more 128-row
         // tiles than SMs: 512 x 4096 x 4096 takes 11.0 us (12.3 with 128-row tiles), 256 x 4096 x 4096 10.9 (9.9), 1024^3
         // 6.8 (5.5).  Up to 128 rows a pair would multiply padding: 48 x 28672 x 4096 takes 20.9 us, 15.5 with 128 rows.
         const long long t128 = static_cast<long long>((M + 127ll) / 128) * ((N + 127ll) / 128);
         const bool pairs = M > 128 && (t128 > info->sm_count || (2 * t128 > info->sm_count && K > 8 * rdb::fp4::STAGE_K));
-        tiling = pairs ? 2 : 1;
+        // (Nor does the split kernel's grid hold every N.)
+        tiling = pairs || !rdb::fp4::split_fits(rdb::fp4::split_plan(format, M, N, K, info->sm_count, 0, 0, 0), q) ? 2 : 1;
     }
-    if (tiling == 2)
-        return format == RDB_FP4_NVFP4 ? rdb::fp4::launch_pair<RDB_FP4_NVFP4>(q, max_ctas, info, st)
-                                       : rdb::fp4::launch_pair<RDB_FP4_MXFP4>(q, max_ctas, info, st);
+    if (tiling == 2) return rdb::fp4::run_pairs(q, format, max_ctas, info, st);
     return rdb::fp4::run_split(q, format, 0, 0, 0, 0, info, st);
 }
 

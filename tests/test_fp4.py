@@ -1060,3 +1060,28 @@ def test_either_direction_can_be_dropped(cuda_device, form):
     left = torch.cuda.memory_allocated(cuda_device) - before - want.numel() * 2
     assert both - left >= size and left <= size + 16384
     assert torch.equal(R.dequantize_fp4(c), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,form", [(3, 65535 * 128 + 5, "mxfp4"), (3, 65535 * 128 + 5, "nvfp4"), (40, 65535 * 256 + 9, "mxfp4")])
+def test_more_columns_than_one_grid_has_tiles(cuda_device, M, N, form):
+    """The same as the two halves of B by themselves.  Positive operands: every sum of 32 products is off by no more than
+    (4 sqrt(32) + 3) 2^-24 of itself on either side."""
+    import rocm_dev_b200 as R
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    A, B = (R.quantize_fp4(torch.randn((r, 32), generator=g, device=cuda_device, dtype=torch.bfloat16).abs(), form) for r in (M, N))
+    half = N // 256 * 128                                            # whole scale tiles: both halves are views
+    per_tile = R.fp4.scale_bytes(form, 128, 32)
+    cuts = [R.Fp4Tensor(B.codes[a:b], B.scales[a // 128 * per_tile:-(-b // 128) * per_tile], B.tensor_scale, form, b - a, 32) for a, b in ((0, half), (half, N))]
+    calls = [R.dense_gemm_fp4] + ([R.skinny_gemm_fp4] if M <= 32 else [])
+    for f in calls:
+        got = f(A, B, out_dtype=torch.float32)
+        for cut, part in zip(cuts, (got[:, :half], got[:, half:])):
+            want = f(A, cut, out_dtype=torch.float32)
+            assert ((part - want).abs() <= 2 * (4 * 32 ** 0.5 + 4) * 2.0 ** -24 * want).all()
+        del got, part, want
+    torch.cuda.synchronize()
+    assert R.lib().rdb_device_status() == 0
+    with pytest.raises(R.RdbError) as e:
+        R.dense_gemm_fp4(A, B, tiling=1)
+    assert e.value.code == 11
