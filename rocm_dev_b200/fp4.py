@@ -331,10 +331,13 @@ def skinny_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
 
 
 def pack_fp4_scales(scales: torch.Tensor, format: str, K: int) -> torch.Tensor:
-    """Plain scale bytes [rows, ceil(K / block)] (as checkpoints hold them) -> the tiles that the kernels read."""
+    """Plain scale bytes [rows, ceil(K / block)] (as checkpoints hold them) -> the tiles that the kernels read.  ``nvfp4``: a
+    scale's sign bit must be 0 (the products take scales as unsigned numbers)."""
+    _format(format)
     b = BLOCK[format]
+    if scales.dtype is not _BYTE or scales.dim() != 2 or K < 1 or scales.shape[1] != (K + b - 1) // b:
+        raise ValueError(f"uint8 [rows, {(K + b - 1) // b}] expected, got {scales.dtype} {tuple(scales.shape)}")
     rows, blocks = scales.shape
-    assert scales.dtype == torch.uint8 and blocks == (K + b - 1) // b
     full = torch.zeros(((rows + 127) // 128 * 128, (K + 255) // 256 * (256 // b)), dtype=torch.uint8, device=scales.device)
     full[:rows, :blocks] = scales
     return full.reshape(full.shape[0] // 128, 4, 32, -1, 4).permute(0, 3, 2, 1, 4).reshape(-1)

@@ -1085,3 +1085,12 @@ def test_more_columns_than_one_grid_has_tiles(cuda_device, M, N, form):
     with pytest.raises(R.RdbError) as e:
         R.dense_gemm_fp4(A, B, tiling=1)
     assert e.value.code == 11
+
+
+def test_plain_scales_of_the_wrong_form_are_refused():
+    import rocm_dev_b200 as R
+    s = torch.zeros((5, 4), dtype=torch.uint8)
+    assert R.pack_fp4_scales(s, "nvfp4", 64).numel() == R.fp4.scale_bytes("nvfp4", 5, 64)
+    for bad in ((s, "fp4", 64), (s, "nvfp4", 65), (s, "mxfp4", 64), (s.int(), "nvfp4", 64), (s[0], "nvfp4", 64), (s, "nvfp4", 0)):
+        with pytest.raises(ValueError):
+            R.pack_fp4_scales(*bad)
