@@ -291,6 +291,10 @@ int rdb_skinny_gemm_fp4_tuned(const uint8_t *A, const uint8_t *scales_a, const f
                               int K, int format, int columns_per_tile, int split_k, int stages, unsigned flags,
                               void *stream);
 
+/* The plan those knobs have by themselves on the current device (a product in 128-row tiles, M of any size): width of a
+ * tile, CTAs that share its K, ring depth, shared memory of a CTA without its static part. */
+int rdb_fp4_split_plan(int M, int N, int K, int format, int *columns_per_tile, int *split_k, int *stages, int *smem_bytes);
+
 /* -------------------------------------------------------- 2:4 sparse GEMM
  * D[M,N] = bf16( (A . W^T) * scale_a[0] * scale_b[0] ), M <= 256, K % 256 == 0,
  * where W [N,K] has at most two non-zero bytes in every aligned group of four

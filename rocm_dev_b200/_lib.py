@@ -57,6 +57,7 @@ _SIGNATURES = {
     "rdb_dequantize_fp4": (i, [vp, vp, vp, i, i, i, vp, i, vp]),
     "rdb_dense_gemm_fp4": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, vp]),
     "rdb_dense_gemm_fp4_tuned": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, vp]),
+    "rdb_fp4_split_plan": (i, [i, i, i, i, vp, vp, vp, vp]),
     "rdb_skinny_gemm_fp4": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, C.c_uint, vp]),
     "rdb_skinny_gemm_fp4_tuned": (i, [vp, vp, vp, vp, vp, vp, vp, i, i, i, i, i, i, i, i, C.c_uint, vp]),
     "rdb_tiled_sum_reduce": (i, [vp, vp, vp, i, i, i, vp]),

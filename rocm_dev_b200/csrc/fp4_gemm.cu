@@ -11,8 +11,7 @@
 // skinny kernel: warp 0 loads, warp 1 issues the MMAs, then all warps move the accumulator to shared memory, and each
 // rank sums its share of the columns over all ranks through distributed shared memory, in rank order: deterministic, no
 // workspace, no atomics.
-#include <cstdlib>
-#include <mutex>
+#include <atomic>
 
 #include "fp4_mma.cuh"
 #include "host_util.h"
@@ -23,6 +22,8 @@ namespace rdb {
 namespace fp4 {
 
 constexpr int SMEM_LIMIT = 232448;         // 227 KiB opt-in maximum per CTA
+constexpr int SM_SMEM = 228 * 1024;        // an SM's, for all its CTAs
+constexpr int CTA_SMEM = 1024 + 160;       // what a CTA takes of it besides the dynamic part: the system's, and static
 constexpr int MAX_STAGES = 8;
 constexpr int SPLIT_THREADS = 256;
 constexpr int A_OPERAND_SPAN = 128 * 128;  // bytes the MMA reads for its 128-row A operand, whatever was loaded
@@ -510,63 +511,110 @@ static int ring_limit(int format, int mbox, int R, int b_tiles) {
     return st < MAX_STAGES ? st : MAX_STAGES;
 }
 
+// The rest of a plan whose R and S are set: stages (at most stage_cap), TMEM columns, shared memory.
+static void complete_plan(SplitPlan& pl, int format, int M, int K, int stage_cap) {
+    const int num_kb = (K + STAGE_K - 1) / STAGE_K, tiles = format == RDB_FP4_NVFP4 ? 4 : 2, rows = M < 128 ? M : 128;
+    pl.b_tiles = (pl.R + 127) / 128;
+    pl.stages = ring_limit(format, pl.mbox, pl.R, pl.b_tiles);
+    if (pl.stages > stage_cap) pl.stages = stage_cap;
+    const int kb = (num_kb + pl.S - 1) / pl.S;
+    if (pl.stages > kb) pl.stages = kb;
+    pl.tmem_cols = 32;
+    while (pl.tmem_cols < pl.R + pl.stages * tiles * 4 * (1 + pl.b_tiles)) pl.tmem_cols *= 2;
+    const int stage = format == RDB_FP4_NVFP4 ? split_stage_bytes<RDB_FP4_NVFP4>(pl.mbox, pl.R, pl.b_tiles)
+                                              : split_stage_bytes<RDB_FP4_MXFP4>(pl.mbox, pl.R, pl.b_tiles);
+    // the ring, what the last stage's A operand reads beyond its rows, and the staging tile that reuses both
+    int bytes = pl.stages * stage + A_OPERAND_SPAN;
+    const int stg = (rows + 31) / 32 * 32 * (pl.R + 4) * 4;
+    if (bytes < stg) bytes = stg;
+    pl.smem = 1024 + bytes;
+    // no more CTAs to an SM than its 512 columns serve: one more would only wait there for columns while another SM has room
+    const int least = SM_SMEM / (512 / pl.tmem_cols + 1);
+    if (pl.smem < least) pl.smem = least;
+}
+
+// Clusters of S CTAs that are resident at once on the current device with one CTA to an SM; 0 if that cannot be told.
+// (The query answers for one CTA to an SM however small its shared memory is.)
+static int query_resident(int S) {
+    const int smem = SMEM_LIMIT - 1024;
+    auto kernel = split_kernel<RDB_FP4_MXFP4>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) { cudaGetLastError(); return 0; }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S);
+    cfg.blockDim = dim3(SPLIT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) { cudaGetLastError(); return 0; }
+    return n;
+}
+
+// The same for a plan with up to `per_sm` (1 or 2) CTAs to an SM, as far as shared memory and TMEM columns allow.  Two: twice
+// as many at least.  More fit on the layout of SMs that answers kOne: up to kTwo[S] tiles of K = 14336 take one wave, a few
+// more 50 to 70 % longer.  These last ones start late, when the launch before has left the very SMs they need, which a long
+// K hides (six stages a CTA: 33 tiles 8.6 us cut in eight, 9.1 in six) and a short one does not (K = 4096, 32 tiles: 7.3 us
+// in eight, 6.9 in six).
+static int resident(const SplitPlan& pl, int per_sm, int num_kb) {
+    static const int kOne[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15}, kTwo[9] = {0, 296, 148, 92, 71, 55, 44, 37, 33};
+    static std::atomic<int> cache[kMaxDevices][9];                  // answer + 1
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+    std::atomic<int>& slot = cache[dev][pl.S];
+    int n = slot.load(std::memory_order_relaxed);
+    if (n == 0) slot.store(n = 1 + query_resident(pl.S), std::memory_order_relaxed);
+    n--;
+    if (per_sm == 1 || pl.tmem_cols > 256 || 2 * (pl.smem + CTA_SMEM) > SM_SMEM) return n;
+    return num_kb >= 6 * pl.S && n == kOne[pl.S] ? kTwo[pl.S] : 2 * n;
+}
+
 // Tile width and K split; 0 hints mean free choice.  Times are device times on 148 SMs, weights from HBM.
 static SplitPlan split_plan(int format, int M, int N, int K, int sm_count, int r_hint, int s_hint, int stages_hint) {
-    // clusters of 1..8 CTAs that are resident at once on 148 SMs (measured)
-    static const int resident[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
     const int num_kb = (K + STAGE_K - 1) / STAGE_K, m_tiles = (M + 127) / 128;
-    const int tiles = format == RDB_FP4_NVFP4 ? 4 : 2;
     SplitPlan best = {};
     best.mbox = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const int rows = M < 128 ? M : 128;
     auto tiles_of = [&](int R) { return static_cast<long long>((N + R - 1) / R) * m_tiles; };
     int stage_cap = MAX_STAGES;
     best.R = 128;
     best.S = 1;
+    // K is cut at most `most` times, and no further than all clusters are resident at once: what is left over would be a
+    // second wave (46 tiles of 32 x 128, K = 14336, MXFP4: 12.0 us cut in five, 19.6 in six, of which 44 are resident).
+    auto widest = [&](int most, int per_sm) {
+        for (int S = most < 8 ? most : 8; S >= 2; S--) {
+            SplitPlan pl = best;
+            pl.S = S;
+            complete_plan(pl, format, M, K, stage_cap);
+            if (tiles_of(pl.R) <= resident(pl, per_sm, num_kb)) return S;
+        }
+        return 1;
+    };
     if (r_hint > 0 || s_hint > 0) {
         if (r_hint > 0) best.R = r_hint;
         if (s_hint > 0) best.S = s_hint < num_kb ? s_hint : num_kb;
     } else if (M <= 32) {
         // A stream over B.  128 columns and four stages leave room for a second CTA on every SM, which may belong to the
-        // next launch: 28672 x 4096 at M = 16 takes 14.6 us, with one CTA of 256 columns 15.6.  K is cut as often as the
-        // clusters are all resident two to an SM: 8192 x 8192 takes 18.5 us uncut, 9.5 cut in four (64 clusters of at
-        // most 66), 15.9 cut in five.  A long K may overflow that a little (4096 x 14336: 9.4 us cut in seven, 10.3 in
-        // six); a short one is not cut below two stages a CTA (2048 x 2048: 4.5 us in four, 4.9 in eight).
+        // next launch: 28672 x 4096 at M = 16 takes 14.6 us, with one CTA of 256 columns 15.6.  (NVFP4 with 17 to 32 rows
+        // lacks 320 bytes for that: one CTA to an SM, unless K is short.)  K is cut as often as the clusters are all
+        // resident: 8192 x 8192 takes 18.5 us uncut, 9.5 cut in four, 15.9 cut in five.  Not below two stages a CTA (2048 x
+        // 2048: 4.5 us in four, 4.9 in eight); a K too short for that in four, in up to four with one CTA to an SM (NVFP4,
+        // 16 x 1024: 2048 rows of B take 3.8 us in four or two, 8192 rows 5.3 in four and 4.6 in two).
         if (N <= 64) best.R = 64;
         stage_cap = 4;
-        for (int S = 2; S <= 8 && S <= (num_kb < 8 ? 4 : num_kb / 2) && S <= num_kb; S++) {
-            int fit = 2 * resident[S] * sm_count / 148;
-            if (num_kb >= 6 * S) fit += fit / 14;
-            if (tiles_of(best.R) <= fit) best.S = S;
-        }
+        best.S = num_kb < 8 ? widest(num_kb < 4 ? num_kb : 4, 1) : widest(num_kb / 2, 2);
     } else if (tiles_of(128) <= sm_count) {
-        // One CTA to an SM: K is cut to fill the SMs, down to four stages a CTA (128 x 4096 x 4096: 8.5 us in four, 9.2 in
-        // two); a short K is not cut, tiles are narrower instead (1024^3: 5.5 us with 64 columns, 6.5 with 128).
-        best.S = static_cast<int>(sm_count / tiles_of(128));
-        if (best.S > num_kb / 4) best.S = num_kb / 4;
-        if (best.S > 8) best.S = 8;
-        if (best.S <= 1) {
-            best.S = 1;
-            if (num_kb <= 8 && tiles_of(64) <= sm_count) best.R = 64;
-        }
+        // One CTA to an SM: K is cut while the clusters are resident, down to four stages a CTA (128 x 4096 x 4096: 8.5 us in
+        // four, 9.2 in two; 128 x 6144 x 4096, 48 tiles: 9.8 in two, 17.5 in three, of which 45 are
+        // resident); a short K is not cut, tiles are narrower instead (1024^3: 5.5 us with 64 columns, 6.5 with 128).
+        best.S = widest(num_kb / 4, 1);
+        if (best.S <= 1 && num_kb <= 8 && tiles_of(64) <= sm_count) best.R = 64;
     } else {
         best.R = 256;       // 128 x 28672 x 4096: 19.4 us, with 128 columns in two waves 26
     }
-    best.b_tiles = (best.R + 127) / 128;
-    best.stages = ring_limit(format, best.mbox, best.R, best.b_tiles);
-    if (best.stages > stage_cap) best.stages = stage_cap;
-    if (stages_hint > 0 && stages_hint < best.stages) best.stages = stages_hint;
-    const int kb = (num_kb + best.S - 1) / best.S;
-    if (best.stages > kb) best.stages = kb;
-    best.tmem_cols = 32;
-    while (best.tmem_cols < best.R + best.stages * tiles * 4 * (1 + best.b_tiles)) best.tmem_cols *= 2;
-    const int stage = format == RDB_FP4_NVFP4 ? split_stage_bytes<RDB_FP4_NVFP4>(best.mbox, best.R, best.b_tiles)
-                                              : split_stage_bytes<RDB_FP4_MXFP4>(best.mbox, best.R, best.b_tiles);
-    // the ring, what the last stage's A operand reads beyond its rows, and the staging tile that reuses both
-    int bytes = best.stages * stage + A_OPERAND_SPAN;
-    const int stg = (rows + 31) / 32 * 32 * (best.R + 4) * 4;
-    if (bytes < stg) bytes = stg;
-    best.smem = 1024 + bytes;
+    complete_plan(best, format, M, K, stages_hint > 0 && stages_hint < stage_cap ? stages_hint : stage_cap);
     return best;
 }
 
@@ -715,6 +763,22 @@ int rdb_skinny_gemm_fp4_tuned(const uint8_t* A, const uint8_t* scales_a, const f
     if (columns_per_tile == 0 && split_k == 0 && stages == 0 && !rdb::fp4::split_fits(rdb::fp4::split_plan(format, M, N, K, info->sm_count, 0, 0, 0), q))
         return rdb::fp4::run_pairs(q, format, 0, info, st);
     return rdb::fp4::run_split(q, format, columns_per_tile, split_k, stages, flags, info, st);
+}
+
+int rdb_fp4_split_plan(int M, int N, int K, int format, int* columns_per_tile, int* split_k, int* stages, int* smem_bytes) {
+    if (M < 1 || N < 1 || K < 1) return RDB_BAD_SHAPE;
+    if (format != RDB_FP4_MXFP4 && format != RDB_FP4_NVFP4) return RDB_INVALID_CONFIG;
+    if (M > rdb::fp4::MAX_EXTENT || N > rdb::fp4::MAX_EXTENT || K > rdb::fp4::MAX_EXTENT) return RDB_SIZE_ABOVE_LIMIT;
+    if (!columns_per_tile || !split_k || !stages || !smem_bytes) return RDB_INVALID_CONFIG;
+    int err = 0;
+    rdb::DeviceInfo* info = rdb::device_info(&err);
+    if (!info) return err;
+    const rdb::fp4::SplitPlan pl = rdb::fp4::split_plan(format, M, N, K, info->sm_count, 0, 0, 0);
+    *columns_per_tile = pl.R;
+    *split_k = pl.S;
+    *stages = pl.stages;
+    *smem_bytes = pl.smem;
+    return RDB_SUCCESS;
 }
 
 int rdb_skinny_gemm_fp4(const uint8_t* A, const uint8_t* scales_a, const float* tensor_scale_a, const uint8_t* B,

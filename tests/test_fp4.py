@@ -1094,3 +1094,39 @@ def test_plain_scales_of_the_wrong_form_are_refused():
     for bad in ((s, "fp4", 64), (s, "nvfp4", 65), (s, "mxfp4", 64), (s.int(), "nvfp4", 64), (s[0], "nvfp4", 64), (s, "nvfp4", 0)):
         with pytest.raises(ValueError):
             R.pack_fp4_scales(*bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", FORMATS)
+def test_k_is_cut_no_further_than_the_clusters_are_resident(cuda_device, form):
+    """Over row counts, tile counts and depths: all clusters of a plan that cuts K fit on the device at once, counted by the
+    shared memory that the plan asks for, and no SM gets more CTAs than its 512 columns serve."""
+    import rocm_dev_b200 as R
+    L = R.lib()
+    if torch.cuda.get_device_properties(cuda_device).multi_processor_count != 148:
+        pytest.skip("the counts are those of 148 SMs")
+    one, two = [0, 148, 74, 45, 33, 26, 22, 15, 15], [0, 296, 148, 93, 71, 56, 45, 37, 33]
+    out = [ctypes.c_int() for _ in range(4)]
+
+    def plan(M, N, K):
+        assert L.rdb_fp4_split_plan(M, N, K, R.fp4.FORMATS[form], *map(ctypes.byref, out)) == 0
+        return [o.value for o in out]
+
+    cut = 0
+    for M in (1, 16, 17, 32, 33, 64, 128, 200, 256):
+        for K in (512, 1024, 2048, 4096, 8192, 14336, 100_000):
+            for tiles in (*range(1, 100), 120, 148, 149, 300):
+                N = 128 * tiles
+                columns, S, stages, smem = plan(M, N, K)
+                per_stage = 4 * (4 if form == "nvfp4" else 2) * (1 + -(-columns // 128))
+                per_sm = 233472 // (smem + 1184)
+                assert per_sm * max(32, 2 ** (columns + stages * per_stage - 1).bit_length()) <= 512
+                if S > 1:
+                    cut += 1
+                    assert -(-N // columns) * -(-M // 128) <= (one if per_sm == 1 or M > 32 else two)[S], (M, N, K, S)
+                    assert S <= -(-K // 256)
+    assert cut > 1000
+    assert plan(32, 8192, 8192)[1] == (2 if form == "nvfp4" else 4)          # one CTA to an SM, two
+    for bad in ((0, 1, 1, 1), (1, 1, 1, 2), (1, 2 ** 31 - 1, 1, 1)):
+        assert L.rdb_fp4_split_plan(*bad, *map(ctypes.byref, out)) in (6, 8, 11)
+    assert L.rdb_fp4_split_plan(1, 1, 1, 1, None, None, None, None) == 6
