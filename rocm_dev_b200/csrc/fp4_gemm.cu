@@ -231,7 +231,9 @@ split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CU
                             for (int j = 0; j < 4; j++) v[j] += x[src][j];
                         }
                 }
-                times<4>(v, alpha);
+                times_pre<4>(v, alpha);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] *= alpha.mul;
                 store4(p.D, p.out_type, p.N, m0 + m, n0 + c, v, p.vec);
             }
         }
@@ -412,12 +414,12 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         // row, no bank conflicts), then one copy out.  A thread holds a row: its own stores would touch 32 lines each.
         auto put = [&](int m0, int n, float* v) {
             if (m0 >= p.M || n >= p.N) return;
-            times<32>(v, alpha);
+            times_pre<32>(v, alpha);
             if (!p.tma_out) {                            // rows of D off 16 bytes: neighbouring lanes store neighbouring columns
                 float* mine = reinterpret_cast<float*>(out) + lane * 33;
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; j++) mine[j] = v[j];
+                for (int j = 0; j < 32; j++) mine[j] = v[j] * alpha.mul;
                 __syncwarp();
                 const int rows = p.M - m0 < 32 ? p.M - m0 : 32;
                 if (n + lane < static_cast<int>(p.N)) {
@@ -433,13 +435,13 @@ pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
                 for (int j = 0; j < 8; j++)
                     *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        make_float4(v[4 * j] * alpha.mul, v[4 * j + 1] * alpha.mul, v[4 * j + 2] * alpha.mul, v[4 * j + 3] * alpha.mul);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     uint32_t w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) w[i] = pack2(p.out_type, v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
+                    for (int i = 0; i < 4; i++) w[i] = pack2(p.out_type, v[8 * j + 2 * i] * alpha.mul, v[8 * j + 2 * i + 1] * alpha.mul);
                     *reinterpret_cast<uint4*>(buf + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }

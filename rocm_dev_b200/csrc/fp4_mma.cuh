@@ -100,15 +100,12 @@ __device__ __forceinline__ Alpha alpha_of(const float* ta, const float* tb) {
     const int e = ea + eb, near = min(max(e, -100), 100), rest = min(max(e - near, -106), 106);
     return {ldexpf(1.0f, rest), ldexpf(m, near)};
 }
-// N values times the scales.
 template <int N>
-__device__ __forceinline__ void times(float* v, const Alpha& a) {
+__device__ __forceinline__ void times_pre(float* v, const Alpha& a) {
     if (a.pre != 1.0f) {
 #pragma unroll
         for (int j = 0; j < N; j++) v[j] *= a.pre;
     }
-#pragma unroll
-    for (int j = 0; j < N; j++) v[j] *= a.mul;
 }
 
 __device__ __forceinline__ uint32_t pack2(int type, float x, float y) {
