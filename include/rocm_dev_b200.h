@@ -242,6 +242,8 @@ int rdb_dense_gemm_fp8_f32(const uint8_t *A, const uint8_t *B, float *D, int M, 
  *           tile at (r % 32) * 16 + (r / 32) * 4 + b; tiles run along K first, K filled up to a multiple of 256 with
  *           zero bytes (the products read them); bytes of rows past the last are of no meaning;
  *   tensor_scale  one fp32 on the device (RDB_FP4_NVFP4 only, else NULL).
+ * What a caller fills in by other means than the quantiser: codes behind K and scales behind K's last block are zero, e4m3
+ * scale bytes have no sign (0x00 to 0x7F).
  * codes and scales must be 16-byte aligned. */
 typedef enum rdb_fp4_format { RDB_FP4_MXFP4 = 0, RDB_FP4_NVFP4 = 1 } rdb_fp4_format;
 typedef enum rdb_type { RDB_TYPE_BF16 = 0, RDB_TYPE_FP16 = 1, RDB_TYPE_FP32 = 2 } rdb_type;

@@ -62,7 +62,8 @@ def _type(dtype: torch.dtype) -> int:
 
 class Fp4Tensor:
     """A held tensor [rows, K]: ``codes`` uint8 [rows, row_bytes(K)], ``scales`` uint8 in tiles (flat, scale_bytes(format,
-    rows, K)), ``tensor_scale`` fp32[1] (``nvfp4``) or None, all on ``device``."""
+    rows, K)), ``tensor_scale`` fp32[1] (``nvfp4``) or None, all on ``device``.  ``torch.save`` and pickle store it; the parts
+    by themselves are views of larger allocations (clone what a state dict is to hold)."""
     __slots__ = ("format", "rows", "K", "_fmt", "_parts", "_buffer", "_held")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, tensor_scale, format: str, rows: int, K: int):
@@ -274,8 +275,9 @@ def _quantize(x: torch.Tensor, format: str, tensor_scale, both: bool):
 
 def quantize_fp4(x: torch.Tensor, format: str = "nvfp4", tensor_scale: torch.Tensor | None = None) -> Fp4Tensor:
     """x [rows, K] (bf16, fp16 or fp32; rows may be a pitch apart) -> held form, blocks along the rows.
-    ``tensor_scale`` (``nvfp4``): a positive fp32[1] to use in place of max|x| / 2688 - a calibrated one, for which x is
-    read once instead of twice.  Its value is copied: changing it later leaves the result as it is."""
+    ``tensor_scale`` (``nvfp4``): a positive fp32[1] to use in place of max|x| * fp32(1 / 2688) - a calibrated one, for
+    which x is read once instead of twice.  Its value is copied: changing it later leaves the result as it is.  An x without
+    unit stride along its rows (a transposed view) is copied first; ``quantize_fp4_both`` makes both forms from one read."""
     return _quantize(x, format, tensor_scale, False)
 
 
@@ -324,7 +326,8 @@ def dense_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None,
 def skinny_gemm_fp4(A: Fp4Tensor, B: Fp4Tensor, out: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
                     flags: int = 0) -> torch.Tensor:
     """The same product for at most 32 rows of A (decode): a stream over B.  ``flags``: 0 or ``OVERLAP_PRIOR_KERNEL`` (the
-    launch may request B while the preceding kernel of the stream drains; that kernel must not write B)."""
+    launch may request B while the preceding kernel of the stream drains; that kernel must not write B, nor may the one
+    before it where the preceding one is an fp8 call with this flag)."""
     args, out, index = _product(A, B, out, out_dtype)
     _call(_SKINNY, "rdb_skinny_gemm_fp4", index, *args, flags)
     return out
