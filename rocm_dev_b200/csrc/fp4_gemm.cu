@@ -48,7 +48,7 @@ __host__ __device__ constexpr int split_stage_bytes(int mbox, int R, int b_tiles
 }
 
 // Bound by the stream of B and by fill and drain around it: NVFP4 16 x 28672 x 4096 takes 14 to 15 us (66 MB, 10.4 at the
-// copy rate; DRAM reads what the operands hold, once), 1 x 4096 x 4096 5.9 (1.5).
+// copy rate; DRAM reads what the operands hold, once), 1 x 4096 x 4096 5.3 (1.5).
 template <int FMT>
 __global__ void __launch_bounds__(SPLIT_THREADS, 1)
 split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const SplitParams p) {
